@@ -259,7 +259,7 @@ def _random(buf, step):
     start = (torch.cummax(start, 0).values * PAD).int().view(-1, 1)
     i = (torch.arange(n, device=dev, dtype=torch.int32).view(-1, PAD) - start).view(-1, 2)
     key = _mix(_mix(torch.tensor([SEED], dtype=torch.int32)) ^ step)
-    x = _mix(_mix(i[:, :1] >> 1) ^ int(key))
+    x = _mix((i[:, :1] >> 1) ^ int(key))
     return (torch.cat((x & 0xFFFF, (x >> 16) & 0xFFFF), 1) << 4 | 8).view(-1)
 
 
