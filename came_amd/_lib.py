@@ -43,6 +43,11 @@ EXPORTED_SYMBOLS = (
     "came8_side_stream_count",
     "came8_quantize_blockwise",
     "came8_dequantize_blockwise",
+    "came8_grad_norm_workspace_size",
+    "came8_grad_norm",
+    "came8_grad_clip",
+    "came8_adamw_step",
+    "came8_dequantize_second_moment",
 )
 
 
@@ -89,6 +94,50 @@ class Came8HParams(ctypes.Structure):
         ("clip_threshold", ctypes.c_double),
         ("weight_decay", ctypes.c_double),
         ("block_size", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
+class Came8GradTensor(ctypes.Structure):
+    """Mirror of ``came8_grad_tensor`` (include/came8.h)."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("numel", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class Came8AdamwTensor(ctypes.Structure):
+    """Mirror of ``came8_adamw_tensor`` (include/came8.h)."""
+
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p),
+        ("exp_avg_sq", ctypes.c_void_p),
+        ("exp_avg_absmax", ctypes.c_void_p),
+        ("exp_avg_sq_absmax", ctypes.c_void_p),
+        ("numel", ctypes.c_int64),
+        ("step", ctypes.c_int64),
+        ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32),
+    ]
+
+
+class Came8AdamwHParams(ctypes.Structure):
+    """Mirror of ``came8_adamw_hparams`` (include/came8.h)."""
+
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("bits", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("seed", ctypes.c_uint32),
         ("flags", ctypes.c_uint32),
     ]
 
@@ -164,6 +213,15 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.came8_quantize_blockwise.argtypes = [vp, i64, i32, i32, vp, vp, vp]
         lib.came8_dequantize_blockwise.restype = ctypes.c_int
         lib.came8_dequantize_blockwise.argtypes = [vp, vp, i64, i32, i32, vp, vp]
+        lib.came8_grad_norm_workspace_size.restype = sz
+        lib.came8_grad_norm_workspace_size.argtypes = [i32]
+        for name in ("came8_grad_norm", "came8_grad_clip"):
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = [vp, i32, ctypes.c_double, vp, vp, vp, sz, vp]
+        lib.came8_adamw_step.restype = ctypes.c_int
+        lib.came8_adamw_step.argtypes = [vp, i32, ctypes.POINTER(Came8AdamwHParams), vp, vp]
+        lib.came8_dequantize_second_moment.restype = ctypes.c_int
+        lib.came8_dequantize_second_moment.argtypes = [vp, vp, i64, i32, vp, vp]
         if lib.came8_abi_version() != ABI_VERSION:
             raise RuntimeError(f"came_amd: {p} has ABI {lib.came8_abi_version()}, expected {ABI_VERSION}")
         _lib = lib

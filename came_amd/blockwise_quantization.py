@@ -86,3 +86,26 @@ def dequantize_blockwise(q: torch.Tensor, absmax: torch.Tensor, *, signed: bool,
             "came8_dequantize_blockwise",
         )
     return out.to(dtype)
+
+
+def dequantize_second_moment(q: torch.Tensor, absmax: torch.Tensor, *, block_size: int) -> torch.Tensor:
+    """What the codes of ``AdamW8bit``'s second moment stand for (``came8_dequantize_second_moment``), in float32, shaped
+    like ``q``: unsigned 8-bit floats of 5 exponent and 3 fraction bits, 1.875 times ``2**0`` the largest, times
+    ``absmax * 8/15`` of their block."""
+    _require_cuda(q, "dequantize_second_moment")
+    if q.dtype != torch.uint8:
+        raise ValueError(f"dequantize_second_moment: codes are uint8, got {q.dtype}")
+    lib = _lib.load()
+    qc = q.contiguous()
+    ac = absmax.to(torch.float32).contiguous()
+    if ac.numel() < num_blocks(qc.numel(), block_size):
+        raise ValueError("absmax has fewer entries than the number of blocks")
+    out = torch.empty(qc.shape, device=qc.device, dtype=torch.float32)
+    with torch.cuda.device(qc.device):
+        stream = torch.cuda.current_stream(qc.device).cuda_stream
+        _lib.check(
+            lib.came8_dequantize_second_moment(qc.data_ptr(), ac.data_ptr(), qc.numel(), int(block_size), out.data_ptr(),
+                                               stream),
+            "came8_dequantize_second_moment",
+        )
+    return out

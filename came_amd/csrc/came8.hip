@@ -23,6 +23,7 @@
 #include "came8_dispatch.h"
 #include "came8_kernels.h"
 #include "came8_norm.h"
+#include "came8_ops.h"
 
 using namespace came8;
 
@@ -1451,6 +1452,11 @@ int plan_size(const came8_tensor* tensors, int32_t n_tensors, int32_t block_size
   return CAME8_OK;
 }
 }  // namespace
+
+namespace came8 {
+int op_fail(int code, const std::string& msg) { return fail(code, msg); }
+int op_check_launch(const char* what) { return check_launch(what); }
+}  // namespace came8
 
 extern "C" {
 

@@ -1,0 +1,561 @@
+// AdamW over many tensors (fp32 or 8-bit moments), the global gradient norm and the clip by it.
+//
+// All of it is one pass over memory: per element a few multiply-adds against 10 to 28 bytes.  The kernels are
+// multi-tensor: a table of up to 64 (192 for the norm) tensors travels in the kernel's arguments, a workgroup takes one
+// chunk of one tensor and finds it by comparing its number with the table's chunk starts, one a lane.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <limits>
+#include <vector>
+
+#include "../../include/came8.h"
+#include "came8_device.h"
+#include "came8_ops.h"
+
+namespace came8 {
+namespace {
+
+constexpr int kAdamTab = 64;    // tensors a launch: 60 bytes each of the 4 KB of arguments
+constexpr int kGradTab = 192;   // 20 bytes each
+constexpr int kAdamChunk = 8192;   // elements of a workgroup: 256 lanes x 4 rows x 8
+constexpr int kGradChunk = 16384;
+constexpr int kNormGroups = 2048;  // workgroups of a norm launch: eight a CU, what is resident
+constexpr float kTinyBlock = 0x1p-100f;  // 8-bit blocks whose largest is below hold zeros (127/a and 1.875/a stay finite)
+
+struct AdamTab {
+  void* p[kAdamTab];
+  const void* g[kAdamTab];
+  void* m[kAdamTab];
+  void* v[kAdamTab];
+  float* ma[kAdamTab];
+  float* va[kAdamTab];
+  int64_t n[kAdamTab];
+  int32_t start[kAdamTab];  // first chunk
+  int32_t count;
+  float b1, c1, b2, c2, eps;
+  float decay;      // 1 - lr * weight_decay
+  float step_size;  // lr / (1 - beta1^t)
+  float inv_bc2;    // 1 / sqrt(1 - beta2^t)
+  uint32_t key;
+  int32_t log2b;
+  const float* scale;
+};
+static_assert(sizeof(AdamTab) <= 4096, "kernel arguments");
+
+struct GradTab {
+  void* g[kGradTab];
+  uint32_t n_lo[kGradTab];
+  int32_t start[kGradTab];
+  uint16_t n_hi_dt[kGradTab];  // numel >> 32, and the type in the lowest two bits
+  int32_t count;
+  int32_t chunks;
+};
+static_assert(sizeof(GradTab) <= 4096, "kernel arguments");
+
+// The table's entry that chunk c belongs to: starts ascend from 0, so it is the number of starts <= c, less one.
+template <int N>
+__device__ __forceinline__ int find_tensor(const int32_t (&start)[N], int count, int c) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int k = 0;
+#pragma unroll
+  for (int i = 0; i < N; i += kWave)
+    k += __popcll(__ballot(i + lane < count && start[i + lane] <= c));
+  return __builtin_amdgcn_readfirstlane(k - 1);
+}
+
+// Eight elements at p[i], the ones from n on as zeros; any address the type allows.
+template <typename T>
+__device__ __forceinline__ void load_row(const CAME8_GLOBAL typename T::storage* p, int64_t i, int64_t n, float (&out)[8]) {
+  if (i + 8 <= n) {
+    if constexpr (sizeof(typename T::storage) == 4) {
+      load8u_f32((const CAME8_GLOBAL float*)p + i, out);
+    } else {
+      const u32x4u raw = *(const CAME8_GLOBAL u32x4u*)(p + i);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = T::elem(w, e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = i + e < n ? T::load(p[i + e]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(CAME8_GLOBAL typename T::storage* p, int64_t i, int64_t n, const float (&in)[8]) {
+  if (i + 8 <= n) {
+    if constexpr (sizeof(typename T::storage) == 4) {
+      *(CAME8_GLOBAL f32x4u*)(p + i) = f32x4{in[0], in[1], in[2], in[3]};
+      *(CAME8_GLOBAL f32x4u*)(p + i + 4) = f32x4{in[4], in[5], in[6], in[7]};
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = uint32_t(T::store(in[2 * e])) | uint32_t(T::store(in[2 * e + 1])) << 16;
+      *(CAME8_GLOBAL u32x4u*)(p + i) = u32x4{w[0], w[1], w[2], w[3]};
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) p[i + e] = T::store(in[e]);
+  }
+}
+
+__device__ __forceinline__ void load_codes(const CAME8_GLOBAL uint8_t* p, int64_t i, int64_t n, uint32_t (&w)[2]) {
+  if (i + 8 <= n) {
+    const u32x2u raw = *(const CAME8_GLOBAL u32x2u*)(p + i);
+    w[0] = raw.x, w[1] = raw.y;
+  } else {
+    w[0] = w[1] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) w[e >> 2] |= uint32_t(p[i + e]) << (8 * (e & 3));
+  }
+}
+
+__device__ __forceinline__ void store_codes(CAME8_GLOBAL uint8_t* p, int64_t i, int64_t n, const uint32_t (&w)[2]) {
+  if (i + 8 <= n) {
+    *(CAME8_GLOBAL u32x2u*)(p + i) = u32x2{w[0], w[1]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < n) p[i + e] = uint8_t(w[e >> 2] >> (8 * (e & 3)));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- fp32 moments
+template <typename P, typename G>
+__global__ __launch_bounds__(kThreads) void k_adamw32(const AdamTab tab) {
+  const int t = find_tensor(tab.start, tab.count, int(blockIdx.x));
+  const int64_t n = tab.n[t];
+  const int64_t base = int64_t(int(blockIdx.x) - tab.start[t]) * kAdamChunk;
+  auto* p = gbl(static_cast<typename P::storage*>(tab.p[t]));
+  auto* g = gbl(static_cast<const typename G::storage*>(tab.g[t]));
+  auto* m = gbl(static_cast<float*>(tab.m[t]));
+  auto* v = gbl(static_cast<float*>(tab.v[t]));
+  const float scale = tab.scale ? *tab.scale : 1.0f;
+  for (int u = 0; u < kAdamChunk; u += kThreads * 8) {
+    const int64_t i = base + u + threadIdx.x * 8;
+    if (i >= n) return;
+    float gr[8], pr[8], mr[8], vr[8];
+    load_row<G>(g, i, n, gr);
+    load_row<P>(p, i, n, pr);
+    load_row<F32>(m, i, n, mr);
+    load_row<F32>(v, i, n, vr);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = gr[e] * scale;
+      mr[e] = mr[e] * tab.b1 + x * tab.c1;
+      vr[e] = vr[e] * tab.b2 + (x * x) * tab.c2;
+      pr[e] = pr[e] * tab.decay - tab.step_size * (mr[e] / (sqrtf(vr[e]) * tab.inv_bc2 + tab.eps));
+    }
+    store_row<P>(p, i, n, pr);
+    store_row<F32>(m, i, n, mr);
+    store_row<F32>(v, i, n, vr);
+  }
+}
+
+// ----------------------------------------------------------------------------------------------- 8-bit moments
+// The second moment's codes: y in [0, 1.875] times 2^-96 puts the format's grid (5 exponent, 3 fraction bits) on fp32's
+// own, the format's subnormals on fp32's, so a code is the value's upper 12 bits and rounding adds below them.
+constexpr float kSmall = 0x1p-96f, kLarge = 0x1p96f;
+
+// 32 bits for a pair of elements, 16 to each
+__device__ __forceinline__ uint32_t pair_hash(uint32_t pair, uint32_t key) {
+  uint32_t x = (pair ^ key) * 0x9E3779B1u;
+  x = (x ^ (x >> 15)) * 0x85EBCA77u;
+  return x ^ (x >> 13);
+}
+
+// One wavefront takes 4 rows of 512 elements, 8 to a lane; a block is a part of a row, a row (K = 1), or K rows.
+template <typename P, typename G, int K>
+__global__ __launch_bounds__(kThreads) void k_adamw8(const AdamTab tab) {
+  const int t = find_tensor(tab.start, tab.count, int(blockIdx.x));
+  const int64_t n = tab.n[t];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int64_t base = int64_t(int(blockIdx.x) - tab.start[t]) * kAdamChunk + wave * 2048 + lane * 8;
+  auto* p = gbl(static_cast<typename P::storage*>(tab.p[t]));
+  auto* g = gbl(static_cast<const typename G::storage*>(tab.g[t]));
+  auto* mq = gbl(static_cast<uint8_t*>(tab.m[t]));
+  auto* vq = gbl(static_cast<uint8_t*>(tab.v[t]));
+  auto *ma = gbl(tab.ma[t]), *va = gbl(tab.va[t]);
+  const float scale = tab.scale ? *tab.scale : 1.0f;
+  const int lanes = K > 1 ? kWave : min(kWave, 1 << (tab.log2b - 3));  // of a block in a row
+#pragma unroll
+  for (int r0 = 0; r0 < 4; r0 += K) {
+    float m[K][8], v[K][8];
+    uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t i = base + (r0 + k) * 512;
+      float gr[8], pr[8];
+      uint32_t mw[2], vw[2];
+      load_row<G>(g, i, n, gr);
+      load_row<P>(p, i, n, pr);
+      load_codes(mq, i, n, mw);
+      load_codes(vq, i, n, vw);
+      const int64_t b = i >> tab.log2b;
+      const float sm = i < n ? scale_s8(ma[b]) : 0.0f, sv = i < n ? va[b] * float(8.0 / 15.0) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = gr[e] * scale;
+        const uint32_t c = (vw[e >> 2] >> (8 * (e & 3))) & 255u;
+        m[k][e] = (code_elem(mw, e) * sm) * tab.b1 + x * tab.c1;
+        v[k][e] = ((__uint_as_float(c << 20) * kLarge) * sv) * tab.b2 + (x * x) * tab.c2;
+        mtop = max(mtop, __float_as_uint(m[k][e]) & 0x7fffffffu);
+        vtop = max(vtop, __float_as_uint(v[k][e]) & 0x7fffffffu);
+        // hardware square root and reciprocal (an ulp each): p's update only, and the denominator is at least eps > 0
+        const float d = __builtin_amdgcn_sqrtf(v[k][e]) * tab.inv_bc2 + tab.eps;
+        pr[e] = pr[e] * tab.decay - tab.step_size * (m[k][e] * __builtin_amdgcn_rcpf(d));
+      }
+      store_row<P>(p, i, n, pr);
+    }
+    // bits of non-negative floats order as they do, with infinities and then NaNs on top: a block keeps its NaN
+    float am = __uint_as_float(group_max_bits_rt(mtop, lanes)), av = __uint_as_float(group_max_bits_rt(vtop, lanes));
+    const float im = am < kTinyBlock ? 0.0f : 127.0f / am, iv = av < kTinyBlock ? 0.0f : 1.875f / av;
+    if (am < kTinyBlock) am = 1.0f;
+    if (av < kTinyBlock) av = 1.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t i = base + (r0 + k) * 512;
+      if (i >= n) continue;
+      uint32_t mw[2] = {0, 0}, vw[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const uint32_t h = pair_hash(uint32_t((i + e) >> 1), tab.key);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int s = 8 * ((e + o) & 3);
+          const float q = fminf(127.0f, fmaxf(-127.0f, rintf(m[k][e + o] * im)));
+          mw[e >> 2] |= (uint32_t(int(q)) & 255u) << s;
+          const uint32_t random = (o ? h >> 16 : h & 0xffffu) << 4 | 8u;
+          const uint32_t bits = __float_as_uint((v[k][e + o] * iv) * kSmall) + random;
+          vw[e >> 2] |= min(bits >> 20, 255u) << s;
+        }
+      }
+      store_codes(mq, i, n, mw);
+      store_codes(vq, i, n, vw);
+      if (k == 0 && lane % lanes == 0) {
+        const int64_t b = i >> tab.log2b;
+        ma[b] = am;
+        va[b] = av;
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_dequantize_e5m3(const uint8_t* q, const float* absmax, int64_t n, int32_t block,
+                                                              float* out) {
+  const int64_t step = int64_t(gridDim.x) * kThreads;
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < n; i += step)
+    out[i] = (__uint_as_float(uint32_t(q[i]) << 20) * kLarge) * (absmax[i / block] * float(8.0 / 15.0));
+}
+
+// ------------------------------------------------------------------------------------------- norm and clip
+template <typename T>
+__device__ __forceinline__ float sum_squares(const void* data, int64_t base, int64_t n) {
+  auto* g = gbl(static_cast<const typename T::storage*>(data));
+  float acc[8] = {};
+#pragma unroll 4
+  for (int u = 0; u < kGradChunk; u += kThreads * 8) {
+    float x[8];
+    load_row<T>(g, base + u + threadIdx.x * 8, n, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = fmaf(x[e], x[e], acc[e]);
+  }
+  return ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+}
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+  v = wave_sum(v);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// One fp64 partial per workgroup, at its own place.
+__global__ __launch_bounds__(kThreads) void k_grad_squares(const GradTab tab, double* partial) {
+  __shared__ double lds[4];
+  double acc = 0.0;
+  for (int c = int(blockIdx.x); c < tab.chunks; c += int(gridDim.x)) {
+    const int t = find_tensor(tab.start, tab.count, c);
+    const int64_t n = int64_t(tab.n_lo[t]) | int64_t(tab.n_hi_dt[t] >> 2) << 32;
+    const int64_t base = int64_t(c - tab.start[t]) * kGradChunk;
+    switch (tab.n_hi_dt[t] & 3) {
+      case CAME8_F32: acc += double(sum_squares<F32>(tab.g[t], base, n)); break;
+      case CAME8_BF16: acc += double(sum_squares<BF16>(tab.g[t], base, n)); break;
+      default: acc += double(sum_squares<F16>(tab.g[t], base, n)); break;
+    }
+  }
+  acc = block_sum(acc, lds);
+  if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+// The partials' sum in the order of their places (the same bits whatever order they were written in), the norm and the
+// clip's factor.  A launch of its own: the alternative, the last workgroup to arrive, needs a counter that is zero.
+__global__ __launch_bounds__(kThreads) void k_grad_norm(const double* partial, int count, float max_norm, float* norm,
+                                                        float* factor) {
+  __shared__ double lds[4];
+  double acc = 0.0;
+  for (int i = int(threadIdx.x); i < count; i += kThreads) acc += partial[i];
+  acc = block_sum(acc, lds);
+  if (threadIdx.x != 0) return;
+  const float nrm = float(sqrt(acc));
+  *norm = nrm;
+  if (factor == nullptr) return;
+  const float f = max_norm / (nrm + 1e-6f);
+  *factor = f > 1.0f ? 1.0f : f;  // a NaN stays
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(void* data, int64_t base, int64_t n, float f) {
+  auto* g = gbl(static_cast<typename T::storage*>(data));
+#pragma unroll 4
+  for (int u = 0; u < kGradChunk; u += kThreads * 8) {
+    const int64_t i = base + u + threadIdx.x * 8;
+    if (i >= n) return;
+    float x[8];
+    load_row<T>(g, i, n, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= f;
+    store_row<T>(g, i, n, x);
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void k_grad_scale(const GradTab tab, const float* factor) {
+  const float f = *factor;
+  if (f == 1.0f) return;
+  for (int c = int(blockIdx.x); c < tab.chunks; c += int(gridDim.x)) {
+    const int t = find_tensor(tab.start, tab.count, c);
+    const int64_t n = int64_t(tab.n_lo[t]) | int64_t(tab.n_hi_dt[t] >> 2) << 32;
+    const int64_t base = int64_t(c - tab.start[t]) * kGradChunk;
+    switch (tab.n_hi_dt[t] & 3) {
+      case CAME8_F32: scale_chunk<F32>(tab.g[t], base, n, f); break;
+      case CAME8_BF16: scale_chunk<BF16>(tab.g[t], base, n, f); break;
+      default: scale_chunk<F16>(tab.g[t], base, n, f); break;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------ host
+int64_t chunks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
+bool type_ok(int32_t dt) { return dt == CAME8_F32 || dt == CAME8_BF16 || dt == CAME8_F16; }
+size_t size_of(int32_t dt) { return dt == CAME8_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+constexpr int64_t kMaxElements = int64_t(1) << 36;  // of a tensor; 192 tensors' chunks stay below 2^31
+constexpr int64_t kMaxGroups = int64_t(1) << 23;    // of a launch: its work items stay below 2^32
+
+using AdamFn = void (*)(AdamTab);
+
+template <typename P, typename G>
+AdamFn adam_kernel(int bits, int block) {
+  if (bits == 32) return k_adamw32<P, G>;
+  return block <= 512 ? k_adamw8<P, G, 1> : block == 1024 ? k_adamw8<P, G, 2> : k_adamw8<P, G, 4>;
+}
+template <typename P>
+AdamFn adam_kernel_g(int gdt, int bits, int block) {
+  return gdt == CAME8_F32 ? adam_kernel<P, F32>(bits, block)
+         : gdt == CAME8_BF16 ? adam_kernel<P, BF16>(bits, block) : adam_kernel<P, F16>(bits, block);
+}
+AdamFn adam_kernel_of(int pdt, int gdt, int bits, int block) {
+  return pdt == CAME8_F32 ? adam_kernel_g<F32>(gdt, bits, block)
+         : pdt == CAME8_BF16 ? adam_kernel_g<BF16>(gdt, bits, block) : adam_kernel_g<F16>(gdt, bits, block);
+}
+
+uint32_t mix(uint32_t x) {
+  x *= 0x9E3779B1u;
+  x = (x ^ (x >> 15)) * 0x85EBCA77u;
+  return x ^ (x >> 13);
+}
+
+int check_grads(const char* what, const came8_grad_tensor* ts, int32_t n) {
+  if (n < 0 || (n > 0 && ts == nullptr)) return op_fail(CAME8_EINVAL, std::string(what) + ": no tensors given");
+  for (int32_t i = 0; i < n; ++i) {
+    const came8_grad_tensor& t = ts[i];
+    const std::string at = std::string(what) + ": tensor " + std::to_string(i);
+    if (!type_ok(t.dtype)) return op_fail(CAME8_EINVAL, at + ": unknown dtype " + std::to_string(t.dtype));
+    if (t.numel < 0 || t.numel > kMaxElements) return op_fail(CAME8_EINVAL, at + ": bad numel " + std::to_string(t.numel));
+    if (t.numel > 0 && (t.data == nullptr || !aligned(t.data, size_of(t.dtype))))
+      return op_fail(CAME8_EINVAL, at + ": null or misaligned pointer");
+  }
+  return CAME8_OK;
+}
+
+// The tables of a tensor list, empty tensors left out.
+std::vector<GradTab> grad_tables(const came8_grad_tensor* ts, int32_t n) {
+  std::vector<GradTab> out;
+  for (int32_t i = 0; i < n; ++i) {
+    if (ts[i].numel == 0) continue;
+    const int64_t chunks = chunks_of(ts[i].numel, kGradChunk);
+    if (out.empty() || out.back().count == kGradTab) {
+      out.emplace_back();
+      out.back().count = out.back().chunks = 0;
+    }
+    GradTab& t = out.back();
+    const int k = t.count++;
+    t.g[k] = ts[i].data;
+    t.n_lo[k] = uint32_t(ts[i].numel);
+    t.n_hi_dt[k] = uint16_t(uint64_t(ts[i].numel) >> 32 << 2 | uint64_t(ts[i].dtype));
+    t.start[k] = t.chunks;
+    t.chunks += int32_t(chunks);
+  }
+  return out;
+}
+
+int grad_norm(const char* what, const std::vector<GradTab>& tabs, int32_t n, double max_norm, float* norm, float* factor,
+              void* workspace, size_t bytes, hipStream_t stream) {
+  if (norm == nullptr || workspace == nullptr) return op_fail(CAME8_EINVAL, std::string(what) + ": null pointer");
+  if (!(max_norm >= 0.0)) return op_fail(CAME8_EINVAL, std::string(what) + ": max_norm must be >= 0");
+  if (bytes < came8_grad_norm_workspace_size(n) || !aligned(workspace, 8))
+    return op_fail(CAME8_ESPACE, std::string(what) + ": workspace too small or misaligned");
+  double* partial = static_cast<double*>(workspace);
+  int total = 0;
+  for (const GradTab& t : tabs) {
+    const int groups = std::min(t.chunks, kNormGroups);
+    hipLaunchKernelGGL(k_grad_squares, dim3(groups), dim3(kThreads), 0, stream, t, partial + total);
+    total += groups;
+  }
+  hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(kThreads), 0, stream, partial, total, float(max_norm), norm, factor);
+  return op_check_launch("grad_norm");
+}
+
+}  // namespace
+}  // namespace came8
+
+using namespace came8;
+
+extern "C" {
+
+size_t came8_grad_norm_workspace_size(int32_t n_tensors) {
+  const size_t launches = n_tensors <= 0 ? 1 : (size_t(n_tensors) + kGradTab - 1) / kGradTab;
+  return launches * kNormGroups * sizeof(double);
+}
+
+int came8_grad_norm(const came8_grad_tensor* tensors, int32_t n_tensors, double max_norm, float* norm, float* factor,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    const int rc = check_grads("came8_grad_norm", tensors, n_tensors);
+    if (rc != CAME8_OK) return rc;
+    return grad_norm("came8_grad_norm", grad_tables(tensors, n_tensors), n_tensors, max_norm, norm, factor, workspace,
+                     workspace_bytes, static_cast<hipStream_t>(stream));
+  } catch (const std::exception& e) {
+    return op_fail(CAME8_EINVAL, std::string("came8_grad_norm: ") + e.what());
+  }
+}
+
+int came8_grad_clip(const came8_grad_tensor* tensors, int32_t n_tensors, double max_norm, float* norm, float* factor,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  try {
+    int rc = check_grads("came8_grad_clip", tensors, n_tensors);
+    if (rc != CAME8_OK) return rc;
+    if (factor == nullptr) return op_fail(CAME8_EINVAL, "came8_grad_clip: null pointer");
+    const std::vector<GradTab> tabs = grad_tables(tensors, n_tensors);
+    rc = grad_norm("came8_grad_clip", tabs, n_tensors, max_norm, norm, factor, workspace, workspace_bytes,
+                   static_cast<hipStream_t>(stream));
+    if (rc != CAME8_OK) return rc;
+    for (const GradTab& t : tabs)
+      hipLaunchKernelGGL(k_grad_scale, dim3(unsigned(std::min<int64_t>(t.chunks, kMaxGroups))), dim3(kThreads), 0, static_cast<hipStream_t>(stream), t, factor);
+    return op_check_launch("grad_scale");
+  } catch (const std::exception& e) {
+    return op_fail(CAME8_EINVAL, std::string("came8_grad_clip: ") + e.what());
+  }
+}
+
+int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const came8_adamw_hparams* hp,
+                     const float* grad_scale, void* stream) {
+  try {
+    if (hp == nullptr || n_tensors < 0 || (n_tensors > 0 && tensors == nullptr))
+      return op_fail(CAME8_EINVAL, "came8_adamw_step: no tensors or hyper-parameters given");
+    if (hp->bits != 32 && hp->bits != 8) return op_fail(CAME8_EINVAL, "came8_adamw_step: bits must be 32 or 8");
+    const int B = hp->block_size;
+    if (hp->bits == 8 && (B < 64 || B > 2048 || (B & (B - 1)) != 0))
+      return op_fail(CAME8_EINVAL, "came8_adamw_step: block_size must be a power of two in [64, 2048]");
+    if (!(hp->lr >= 0.0) || !(hp->beta1 >= 0.0 && hp->beta1 < 1.0) || !(hp->beta2 >= 0.0 && hp->beta2 < 1.0) ||
+        !(hp->eps >= 0.0) || !(hp->weight_decay >= 0.0))
+      return op_fail(CAME8_EINVAL, "came8_adamw_step: lr, eps and weight_decay must be >= 0, betas in [0, 1)");
+    if (hp->bits == 8 && !(float(hp->eps) >= std::numeric_limits<float>::min()))
+      return op_fail(CAME8_EINVAL, "came8_adamw_step: 8-bit moments need eps > 0 (a normal fp32 number)");
+    if (hp->flags != 0) return op_fail(CAME8_EINVAL, "came8_adamw_step: unknown flags");
+    for (int32_t i = 0; i < n_tensors; ++i) {
+      const came8_adamw_tensor& t = tensors[i];
+      const std::string at = "came8_adamw_step: tensor " + std::to_string(i);
+      if (!type_ok(t.param_dtype) || !type_ok(t.grad_dtype)) return op_fail(CAME8_EINVAL, at + ": unknown dtype");
+      if (t.numel < 0 || t.numel > kMaxElements) return op_fail(CAME8_EINVAL, at + ": bad numel");
+      if (t.step < 1) return op_fail(CAME8_EINVAL, at + ": step must be >= 1");
+      if (t.numel == 0) continue;
+      const size_t ms = hp->bits == 32 ? 4 : 1;
+      if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || !aligned(t.param, size_of(t.param_dtype)) ||
+          !aligned(t.grad, size_of(t.grad_dtype)) || !aligned(t.exp_avg, ms) || !aligned(t.exp_avg_sq, ms))
+        return op_fail(CAME8_EINVAL, at + ": null or misaligned pointer");
+      if (hp->bits == 8 && (!t.exp_avg_absmax || !t.exp_avg_sq_absmax || !aligned(t.exp_avg_absmax, 4) ||
+                            !aligned(t.exp_avg_sq_absmax, 4)))
+        return op_fail(CAME8_EINVAL, at + ": null or misaligned absmax");
+    }
+    // launches: tensors of one (types, step count) together, in the order given
+    std::vector<char> done(size_t(n_tensors), 0);
+    for (int32_t i = 0; i < n_tensors; ++i) {
+      if (done[size_t(i)] || tensors[i].numel == 0) continue;
+      const came8_adamw_tensor& f = tensors[i];
+      AdamTab tab;
+      const double t = double(f.step);
+      tab.b1 = float(hp->beta1);
+      tab.c1 = float(1.0 - hp->beta1);
+      tab.b2 = float(hp->beta2);
+      tab.c2 = float(1.0 - hp->beta2);
+      tab.eps = float(hp->eps);
+      tab.decay = float(1.0 - hp->lr * hp->weight_decay);
+      tab.step_size = float(hp->lr / (1.0 - std::pow(hp->beta1, t)));
+      tab.inv_bc2 = float(1.0 / std::sqrt(1.0 - std::pow(hp->beta2, t)));
+      tab.key = mix(mix(hp->seed) ^ uint32_t(f.step));
+      tab.log2b = hp->bits == 8 ? __builtin_ctz(unsigned(B)) : 0;
+      tab.scale = grad_scale;
+      const AdamFn fn = adam_kernel_of(f.param_dtype, f.grad_dtype, hp->bits, B);
+      int64_t chunks = 0;
+      tab.count = 0;
+      auto flush = [&]() {
+        if (tab.count > 0) hipLaunchKernelGGL(fn, dim3(unsigned(chunks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), tab);
+        tab.count = 0;
+        chunks = 0;
+      };
+      for (int32_t j = i; j < n_tensors; ++j) {
+        const came8_adamw_tensor& a = tensors[j];
+        if (done[size_t(j)] || a.numel == 0 || a.step != f.step || a.param_dtype != f.param_dtype || a.grad_dtype != f.grad_dtype)
+          continue;
+        done[size_t(j)] = 1;
+        const int64_t c = chunks_of(a.numel, kAdamChunk);
+        if (tab.count == kAdamTab || chunks + c > kMaxGroups) flush();
+        const int k = tab.count++;
+        tab.p[k] = a.param;
+        tab.g[k] = a.grad;
+        tab.m[k] = a.exp_avg;
+        tab.v[k] = a.exp_avg_sq;
+        tab.ma[k] = a.exp_avg_absmax;
+        tab.va[k] = a.exp_avg_sq_absmax;
+        tab.n[k] = a.numel;
+        tab.start[k] = int32_t(chunks);
+        chunks += c;
+      }
+      flush();
+    }
+    return op_check_launch("adamw_step");
+  } catch (const std::exception& e) {
+    return op_fail(CAME8_EINVAL, std::string("came8_adamw_step: ") + e.what());
+  }
+}
+
+int came8_dequantize_second_moment(const uint8_t* q, const float* absmax, int64_t n, int32_t block_size, float* out,
+                                   void* stream) {
+  if (block_size <= 0) return op_fail(CAME8_EINVAL, "came8_dequantize_second_moment: block_size must be > 0");
+  if (n < 0) return op_fail(CAME8_EINVAL, "came8_dequantize_second_moment: n must be >= 0");
+  if (n == 0) return CAME8_OK;
+  if (!q || !absmax || !out) return op_fail(CAME8_EINVAL, "came8_dequantize_second_moment: null pointer");
+  hipLaunchKernelGGL(k_dequantize_e5m3, dim3(unsigned(std::min<int64_t>(chunks_of(n, kThreads), 1 << 20))), dim3(kThreads), 0,
+                     static_cast<hipStream_t>(stream), q, absmax, n, block_size, out);
+  return op_check_launch("dequantize_second_moment");
+}
+
+}  // extern "C"

@@ -1,4 +1,5 @@
-// came8_host: descriptors of a param group's tensors for came8_step, filled natively.
+// came8_host: descriptors of a param group's tensors for came8_step (and for came8_adamw_step and the gradient norm),
+// filled natively.
 //
 // gather() does what the optimizers' Python does for every parameter of a group before a step (the checks of
 // _prepare_param and _check_state, the fields of _descriptors and _fill_desc, the step counts) for the plain case:
@@ -129,6 +130,48 @@ bool describe(const at::Tensor& p, const at::Tensor& g, PyObject* st, int kind, 
   return true;
 }
 
+// The parameters of a list that have a gradient, and the gradients; false: not the plain case.  The references to the
+// gradients are kept: a key's hash may run Python, which may replace one.
+bool collect(PyObject* params, int64_t cap, std::vector<PyObject*>& used, std::vector<at::Tensor>& grads) {
+  const Py_ssize_t n = PyList_GET_SIZE(params);
+  used.reserve(size_t(n));
+  grads.reserve(size_t(n));
+  const at::Tensor* first = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* po = PyList_GET_ITEM(params, i);
+    if (!THPVariable_CheckExact(po)) return false;  // subclasses may keep their data elsewhere
+    const at::Tensor& p = THPVariable_Unpack(po);
+    const at::Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    if (first == nullptr) first = &p;
+    if (g.key_set().has(c10::DispatchKey::Python) || int64_t(used.size()) >= cap || p.device() != first->device() ||
+        !plain(p, g))
+      return false;
+    used.push_back(po);
+    grads.push_back(g);
+  }
+  return true;
+}
+
+// The list of `used`, every state's step count advanced by one; null with a Python error set.
+PyObject* advanced(const std::vector<PyObject*>& used, const std::vector<std::pair<PyObject*, long>>& counts) {
+  static PyObject* k_step = key("step");
+  PyObject* res = PyList_New(Py_ssize_t(used.size()));
+  if (res == nullptr) return nullptr;
+  for (size_t i = 0; i < used.size(); ++i) {
+    Py_INCREF(used[i]);
+    PyList_SET_ITEM(res, Py_ssize_t(i), used[i]);
+    PyObject* v = PyLong_FromLong(counts[i].second + 1);
+    if (v == nullptr || PyDict_SetItem(counts[i].first, k_step, v) != 0) {
+      Py_XDECREF(v);
+      Py_DECREF(res);
+      return nullptr;
+    }
+    Py_DECREF(v);
+  }
+  return res;
+}
+
 // gather(params: list, state: dict, address: int, capacity: int, state_kind: int, block_size: int)
 //   -> list of the parameters with a gradient, whose came8_tensor descriptors now lie at `address` in that order and
 //      whose step counts are advanced; None: not the plain case, nothing changed.
@@ -142,26 +185,10 @@ PyObject* gather(PyObject*, PyObject* args) {
   if (block < 1) Py_RETURN_NONE;  // the blocks are counted by a division; the Python raises the error
   try {
     came8_tensor* out = reinterpret_cast<came8_tensor*>(static_cast<uintptr_t>(addr));
-    const Py_ssize_t n = PyList_GET_SIZE(params);
     std::vector<PyObject*> used;                     // the parameters with a gradient
     std::vector<std::pair<PyObject*, long>> counts;  // their states and step counts (the dicts outlive this call)
-    std::vector<at::Tensor> grads;                   // and those (a key's hash may run Python, which may replace one)
-    used.reserve(size_t(n));
-    grads.reserve(size_t(n));
-    const at::Tensor* first = nullptr;
-    for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject* po = PyList_GET_ITEM(params, i);
-      if (!THPVariable_CheckExact(po)) Py_RETURN_NONE;  // subclasses may keep their data elsewhere
-      const at::Tensor& p = THPVariable_Unpack(po);
-      const at::Tensor& g = p.grad();
-      if (!g.defined()) continue;
-      if (first == nullptr) first = &p;
-      if (g.key_set().has(c10::DispatchKey::Python) || int64_t(used.size()) >= cap || p.device() != first->device() ||
-          !plain(p, g))
-        Py_RETURN_NONE;
-      used.push_back(po);
-      grads.push_back(g);
-    }
+    std::vector<at::Tensor> grads;
+    if (!collect(params, cap, used, grads)) Py_RETURN_NONE;
     counts.reserve(used.size());
     for (size_t i = 0; i < used.size(); ++i) {
       const at::Tensor& p = THPVariable_Unpack(used[i]);
@@ -173,28 +200,109 @@ PyObject* gather(PyObject*, PyObject* args) {
       }
       counts.emplace_back(st, step);
     }
-    static PyObject* k_step = key("step");
-    PyObject* res = PyList_New(Py_ssize_t(used.size()));
-    if (res == nullptr) return nullptr;
-    for (size_t i = 0; i < used.size(); ++i) {
-      Py_INCREF(used[i]);
-      PyList_SET_ITEM(res, Py_ssize_t(i), used[i]);
-      PyObject* v = PyLong_FromLong(counts[i].second + 1);
-      if (v == nullptr || PyDict_SetItem(counts[i].first, k_step, v) != 0) {
-        Py_XDECREF(v);
-        Py_DECREF(res);
-        return nullptr;
-      }
-      Py_DECREF(v);
-    }
-    return res;
+    return advanced(used, counts);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
   }
 }
 
+// The buffer of a moment or its scales: contiguous, of the parameter's device; null otherwise.
+void* moment(PyObject* st, PyObject* name, const at::Tensor& p, at::ScalarType type, int64_t n) {
+  const at::Tensor* t = tensor_of(st, name);
+  return t != nullptr && t->scalar_type() == type && t->numel() == n && t->device() == p.device() && t->is_contiguous()
+             ? t->data_ptr()
+             : nullptr;
+}
+
+// gather_adamw(params: list, state: dict, address: int, capacity: int, bits: int, block_size: int)
+//   -> gather() for came8_adamw_tensor descriptors.
+PyObject* gather_adamw(PyObject*, PyObject* args) {
+  PyObject *params, *state;
+  unsigned long long addr;
+  long long cap, block;
+  int bits;
+  if (!PyArg_ParseTuple(args, "O!O!KLiL", &PyList_Type, &params, &PyDict_Type, &state, &addr, &cap, &bits, &block))
+    return nullptr;
+  if (block < 1) Py_RETURN_NONE;
+  static PyObject *k_step = key("step"), *k_m = key("exp_avg"), *k_v = key("exp_avg_sq"), *k_mq = key("exp_avg_q"),
+                  *k_vq = key("exp_avg_sq_q"), *k_ma = key("exp_avg_absmax"), *k_va = key("exp_avg_sq_absmax");
+  try {
+    came8_adamw_tensor* out = reinterpret_cast<came8_adamw_tensor*>(static_cast<uintptr_t>(addr));
+    std::vector<PyObject*> used;
+    std::vector<at::Tensor> grads;
+    if (!collect(params, cap, used, grads)) Py_RETURN_NONE;
+    std::vector<std::pair<PyObject*, long>> counts;
+    counts.reserve(used.size());
+    for (size_t i = 0; i < used.size(); ++i) {
+      const at::Tensor& p = THPVariable_Unpack(used[i]);
+      PyObject* st = PyDict_GetItemWithError(state, used[i]);
+      PyObject* so = st != nullptr && PyDict_Check(st) ? PyDict_GetItemWithError(st, k_step) : nullptr;
+      int over = 0;
+      const long step = so != nullptr && PyLong_CheckExact(so) ? PyLong_AsLongAndOverflow(so, &over) : -1;
+      if (step < 0 || over != 0) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+      came8_adamw_tensor& d = out[i];
+      d = came8_adamw_tensor{};
+      d.param = p.data_ptr();
+      d.grad = grads[i].data_ptr();
+      d.numel = p.numel();
+      d.step = step + 1;
+      d.param_dtype = dtype_code(p);
+      d.grad_dtype = dtype_code(grads[i]);
+      if (bits == 32) {
+        d.exp_avg = moment(st, k_m, p, at::kFloat, d.numel);
+        d.exp_avg_sq = moment(st, k_v, p, at::kFloat, d.numel);
+      } else {
+        d.exp_avg = moment(st, k_mq, p, at::kChar, d.numel);
+        d.exp_avg_sq = moment(st, k_vq, p, at::kByte, d.numel);
+        d.exp_avg_absmax = static_cast<float*>(moment(st, k_ma, p, at::kFloat, num_blocks(d.numel, block)));
+        d.exp_avg_sq_absmax = static_cast<float*>(moment(st, k_va, p, at::kFloat, num_blocks(d.numel, block)));
+      }
+      if (d.exp_avg == nullptr || d.exp_avg_sq == nullptr ||
+          (bits != 32 && (d.exp_avg_absmax == nullptr || d.exp_avg_sq_absmax == nullptr))) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+      counts.emplace_back(st, step);
+    }
+    return advanced(used, counts);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+// gather_grads(tensors: list or tuple, address: int, capacity: int) -> the number of came8_grad_tensor descriptors now at
+// `address`, one for each tensor; None: some tensor is not a plain contiguous one of the first's device.
+PyObject* gather_grads(PyObject*, PyObject* args) {
+  PyObject* tensors;
+  unsigned long long addr;
+  long long cap;
+  if (!PyArg_ParseTuple(args, "OKL", &tensors, &addr, &cap)) return nullptr;
+  if (!PyList_Check(tensors) && !PyTuple_Check(tensors)) Py_RETURN_NONE;
+  came8_grad_tensor* out = reinterpret_cast<came8_grad_tensor*>(static_cast<uintptr_t>(addr));
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(tensors);
+  if (n > cap) Py_RETURN_NONE;
+  const at::Tensor* first = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(tensors, i);
+    if (!THPVariable_CheckExact(o)) Py_RETURN_NONE;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (first == nullptr) first = &t;
+    if (!t.is_cuda() || t.device() != first->device() || t.layout() != at::kStrided || !t.is_contiguous() ||
+        t.is_neg() || dtype_code(t) < 0)
+      Py_RETURN_NONE;
+    out[i] = came8_grad_tensor{t.numel() > 0 ? t.data_ptr() : nullptr, t.numel(), dtype_code(t), 0};
+  }
+  return PyLong_FromSsize_t(n);
+}
+
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "descriptors of a param group's tensors"},
+                         {"gather_adamw", gather_adamw, METH_VARARGS, "AdamW descriptors of a param group's tensors"},
+                         {"gather_grads", gather_grads, METH_VARARGS, "descriptors of a list of gradients"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "came8_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

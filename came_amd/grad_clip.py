@@ -1,0 +1,90 @@
+"""The global gradient norm over many tensors, and the clip by it.
+
+One pass over the gradients, whatever their number and types, with the arithmetic of ``torch.nn.utils.clip_grad_norm_``
+(norm type 2): ``norm = sqrt(sum of squares)``, ``factor = min(1, max_norm / (norm + 1e-6))``, gradients times the factor
+in place.  No host synchronisation: the norm is a device tensor.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_DTYPE_CODE = {torch.float32: _lib.CAME8_F32, torch.bfloat16: _lib.CAME8_BF16, torch.float16: _lib.CAME8_F16}
+
+
+def _check(t: torch.Tensor, what: str, device) -> None:
+    if t.is_sparse:
+        raise RuntimeError(f"{what}: sparse gradients are not supported")
+    if not t.is_cuda:
+        raise RuntimeError(f"{what}: came_amd runs on the GPU; got a {t.device} tensor")
+    if t.dtype not in _DTYPE_CODE:
+        raise RuntimeError(f"{what}: unsupported dtype {t.dtype} (float32, bfloat16 and float16 are supported)")
+    if t.device != device:
+        raise RuntimeError(f"{what}: tensors on {device} and {t.device}; the norm is taken on one GPU")
+
+
+def _contiguous(tensors: list, what: str):
+    """The tensors as contiguous ones, and (tensor, contiguous copy) pairs of those that were not."""
+    out, copies = [], []
+    for t in tensors:
+        _check(t, what, tensors[0].device)
+        c = t if t.is_contiguous() else t.contiguous()
+        if c is not t:
+            copies.append((t, c))
+        out.append(c)
+    return out, copies
+
+
+def _reduce(tensors: list, max_norm: float | None, scale: bool, what: str):
+    """(norm, factor, keep): device scalars of one call; with `scale` the tensors are multiplied in place."""
+    lib = _lib.load()
+    n = len(tensors)
+    descs = (_lib.Came8GradTensor * max(n, 1))()
+    copies = []
+    if _lib.host().gather_grads(tensors, ctypes.addressof(descs), n) is None:
+        flat, copies = _contiguous(tensors, what)
+        for d, t in zip(descs, flat):
+            d.data, d.numel, d.dtype = (t.data_ptr() if t.numel() else None), t.numel(), _DTYPE_CODE[t.dtype]
+    device = tensors[0].device
+    with torch.cuda.device(device):
+        out = torch.empty(2, dtype=torch.float32, device=device)
+        size = lib.came8_grad_norm_workspace_size(n)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        call = lib.came8_grad_clip if scale else lib.came8_grad_norm
+        at = out.data_ptr()
+        _lib.check(call(descs, n, float(max_norm or 0.0), at, at + 4, ws.data_ptr(), size,
+                        torch.cuda.current_stream(device).cuda_stream),
+                   "came8_grad_clip" if scale else "came8_grad_norm")
+        if scale:
+            for t, c in copies:
+                t.copy_(c)
+    return out[0], out[1:]
+
+
+@torch.no_grad()
+def grad_norm(tensors) -> torch.Tensor:
+    """The 2-norm over all elements of the tensors (a 0-d float32 tensor on their device)."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    return _reduce(tensors, None, False, "grad_norm")[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale the parameters' gradients in place so that their 2-norm together is at most ``max_norm``; returns the norm
+    before that.  A norm that is infinite or NaN makes them 0 or NaN, as in torch; with ``error_if_nonfinite`` it raises
+    and leaves them as they were (and waits for the GPU to know)."""
+    if not float(max_norm) >= 0.0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if error_if_nonfinite and not bool(torch.isfinite(_reduce(grads, None, False, "clip_grad_norm_")[0])):
+        raise RuntimeError("clip_grad_norm_: the gradients' norm is not finite")
+    return _reduce(grads, max_norm, True, "clip_grad_norm_")[0]

@@ -288,6 +288,82 @@ int came8_quantize_blockwise(const float* x, int64_t n, int32_t is_signed, int32
 int came8_dequantize_blockwise(const void* q, const float* absmax, int64_t n, int32_t is_signed,
                                int32_t block_size, float* out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Training beside CAME: the global gradient norm, the clip by it, and AdamW over many tensors.  No counterpart
+ * in the reference.  As above: the caller owns every buffer, everything is enqueued on `stream`, nothing
+ * allocates, copies or synchronises.  The tensor lists travel in the kernels' arguments (64 to 192 tensors a
+ * launch), so no plan is kept and a call may be captured in a HIP graph.
+ * --------------------------------------------------------------------------------------------------------- */
+
+/* one gradient (or any tensor): n contiguous elements of type dtype, at any address its type allows */
+typedef struct came8_grad_tensor {
+  void* data;
+  int64_t numel;
+  int32_t dtype; /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t reserved;
+} came8_grad_tensor;
+
+/* Bytes of device workspace for came8_grad_norm and came8_grad_clip over n_tensors tensors. */
+size_t came8_grad_norm_workspace_size(int32_t n_tensors);
+
+/*
+ * norm[0] = sqrt(sum of all tensors' squares) and, where factor is not NULL,
+ * factor[0] = min(1, max_norm / (norm + 1e-6)) (device floats; the factor is NaN where the norm is, 0 where it is
+ * infinite).  Sums: fp32 over at most 64 elements, fp64 from there, in a fixed order: the same inputs
+ * give the same bits.  Squares that overflow fp32 give an infinite norm.
+ */
+int came8_grad_norm(const came8_grad_tensor* tensors, int32_t n_tensors, double max_norm, float* norm, float* factor,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* came8_grad_norm, then every tensor times the factor, in place (nothing is written where the factor is 1). */
+int came8_grad_clip(const came8_grad_tensor* tensors, int32_t n_tensors, double max_norm, float* norm, float* factor,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* one parameter of an AdamW step: contiguous buffers of numel elements; param and the moments are updated in place.
+ * bits = 32: exp_avg, exp_avg_sq are float[numel], the absmax pointers unused.
+ * bits = 8:  exp_avg is int8_t[numel], exp_avg_sq uint8_t[numel], the absmax arrays float[ceil(numel/block_size)]:
+ *   the first moment in the full8bit format (code * (absmax / 127)), the second as unsigned 8-bit floats of 5 exponent
+ *   and 3 fraction bits relative to the block's largest: code c stands for f(c) * (absmax * 8/15), with
+ *   f(c) = (1 + (c & 7)/8) * 2^((c >> 3) - 31) for c >= 8, c * 2^-33 below (f(255) = 1.875). */
+typedef struct came8_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_absmax;
+  float* exp_avg_sq_absmax;
+  int64_t numel;
+  int64_t step;        /* this tensor's step count, this step included (>= 1) */
+  int32_t param_dtype; /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t grad_dtype;
+} came8_adamw_tensor;
+
+typedef struct came8_adamw_hparams {
+  double lr, beta1, beta2, eps, weight_decay;
+  int32_t bits;       /* 32 or 8 */
+  int32_t block_size; /* bits = 8: a power of two in [64, 2048] */
+  uint32_t seed;      /* bits = 8: of the second moment's rounding */
+  uint32_t flags;     /* 0 */
+} came8_adamw_hparams;
+
+/*
+ * One AdamW step (decoupled weight decay) over all tensors; g' = g * grad_scale[0] (a device float, e.g.
+ * came8_grad_norm's factor; NULL: g), and with t = the tensor's step count
+ *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32, p rounded to its type.  bits = 8: p takes m and v before they are requantised; eps must be > 0, m's codes
+ * round to nearest, v's to one of its two neighbours at random in proportion (a decayed v moves by far less than a code
+ * a step: rounded to nearest it would never move), from a hash of seed, step count and element, so that a step repeats
+ * bit for bit.  A block whose largest is under 2^-100 holds zeros; one that takes an infinity or NaN holds no finite
+ * values from then on.
+ */
+int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const came8_adamw_hparams* hp,
+                     const float* grad_scale, void* stream);
+
+/* out[i] = what code q[i] of an 8-bit second moment stands for (came8_adamw_tensor). */
+int came8_dequantize_second_moment(const uint8_t* q, const float* absmax, int64_t n, int32_t block_size, float* out,
+                                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif
