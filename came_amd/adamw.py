@@ -156,10 +156,11 @@ class _AdamWBase(torch.optim.Optimizer):
             raise RuntimeError(f"{type(self).__name__}.step() cannot be captured: its step count is a host number")
         factor = None
         if self.max_grad_norm is not None:
-            grads = [g for g in [p.grad for group in self.param_groups for p in group["params"]] if g is not None]
-            if not grads:
+            every = list(chain.from_iterable(group["params"] for group in self.param_groups))
+            found = _reduce(every, self.max_grad_norm, False, type(self).__name__, True)
+            if found is None:
                 return loss
-            self.last_grad_norm, factor = _reduce(grads, self.max_grad_norm, False, type(self).__name__)
+            self.last_grad_norm, factor = found
         for group in self.param_groups:
             params = group["params"]
             descs = (_lib.Came8AdamwTensor * max(len(params), 1))()

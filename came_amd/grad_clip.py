@@ -38,30 +38,33 @@ def _contiguous(tensors: list, what: str):
     return out, copies
 
 
-def _reduce(tensors: list, max_norm: float | None, scale: bool, what: str):
-    """(norm, factor, keep): device scalars of one call; with `scale` the tensors are multiplied in place."""
+def _reduce(tensors: list, max_norm: float | None, scale: bool, what: str, of_parameters: bool = False):
+    """(norm, factor): device scalars of one call over the tensors, or the parameters' gradients; with `scale` those are
+    multiplied in place.  None where no parameter has a gradient."""
     lib = _lib.load()
-    n = len(tensors)
-    descs = (_lib.Came8GradTensor * max(n, 1))()
+    descs = (_lib.Came8GradTensor * max(len(tensors), 1))()
     copies = []
-    if _lib.host().gather_grads(tensors, ctypes.addressof(descs), n) is None:
-        flat, copies = _contiguous(tensors, what)
-        for d, t in zip(descs, flat):
+    n = _lib.host().gather_grads(tensors, ctypes.addressof(descs), len(tensors), of_parameters)
+    if n is None:
+        if of_parameters:
+            tensors = [g for g in [p.grad for p in tensors] if g is not None]
+        tensors, copies = _contiguous(tensors, what)
+        n = len(tensors)
+        for d, t in zip(descs, tensors):
             d.data, d.numel, d.dtype = (t.data_ptr() if t.numel() else None), t.numel(), _DTYPE_CODE[t.dtype]
-    device = tensors[0].device
+    if n == 0:
+        return None
+    device = tensors[0].device if copies or not of_parameters else next(p.grad for p in tensors if p.grad is not None).device
     with torch.cuda.device(device):
-        out = torch.empty(2, dtype=torch.float32, device=device)
         size = lib.came8_grad_norm_workspace_size(n)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-        call = lib.came8_grad_clip if scale else lib.came8_grad_norm
-        at = out.data_ptr()
-        _lib.check(call(descs, n, float(max_norm or 0.0), at, at + 4, ws.data_ptr(), size,
-                        torch.cuda.current_stream(device).cuda_stream),
-                   "came8_grad_clip" if scale else "came8_grad_norm")
-        if scale:
-            for t, c in copies:
-                t.copy_(c)
-    return out[0], out[1:]
+        ws = torch.empty(size // 4 + 2, dtype=torch.float32, device=device)  # and the two scalars
+        at = ws.data_ptr()
+        _lib.check((lib.came8_grad_clip if scale else lib.came8_grad_norm)(
+            descs, n, float(max_norm or 0.0), at + size, at + size + 4, at, size,
+            torch.cuda.current_stream(device).cuda_stream), "came8_grad_clip" if scale else "came8_grad_norm")
+        for t, c in copies if scale else ():
+            t.copy_(c)
+    return ws[-2], ws[-1:]
 
 
 @torch.no_grad()
@@ -82,9 +85,10 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [g for g in [p.grad for p in parameters] if g is not None]
-    if not grads:
-        return torch.tensor(0.0)
-    if error_if_nonfinite and not bool(torch.isfinite(_reduce(grads, None, False, "clip_grad_norm_")[0])):
-        raise RuntimeError("clip_grad_norm_: the gradients' norm is not finite")
-    return _reduce(grads, max_norm, True, "clip_grad_norm_")[0]
+    parameters = list(parameters)
+    if error_if_nonfinite:
+        found = _reduce(parameters, None, False, "clip_grad_norm_", True)
+        if found is not None and not bool(torch.isfinite(found[0])):
+            raise RuntimeError("clip_grad_norm_: the gradients' norm is not finite")
+    found = _reduce(parameters, max_norm, True, "clip_grad_norm_", True)
+    return torch.tensor(0.0) if found is None else found[0]
