@@ -48,6 +48,9 @@ EXPORTED_SYMBOLS = (
     "came8_grad_clip",
     "came8_adamw_step",
     "came8_dequantize_second_moment",
+    "came8_gated_ffn_workspace_size",
+    "came8_gated_ffn_forward",
+    "came8_gated_ffn_backward",
 )
 
 
@@ -142,6 +145,13 @@ class Came8AdamwHParams(ctypes.Structure):
     ]
 
 
+class Came8Ffn(ctypes.Structure):
+    """Mirror of ``came8_ffn`` (include/came8.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("tokens", "dim", "hidden", "out", "ld_x", "ld_gate", "ld_up", "ld_down")]
+    _fields_ += [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32)]
+
+
 class Came8PhaseStat(ctypes.Structure):
     """Mirror of ``came8_phase_stat`` (include/came8.h)."""
 
@@ -222,6 +232,12 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.came8_adamw_step.argtypes = [vp, i32, ctypes.POINTER(Came8AdamwHParams), vp, vp]
         lib.came8_dequantize_second_moment.restype = ctypes.c_int
         lib.came8_dequantize_second_moment.argtypes = [vp, vp, i64, i32, vp, vp]
+        lib.came8_gated_ffn_workspace_size.restype = ctypes.c_int
+        lib.came8_gated_ffn_workspace_size.argtypes = [ctypes.POINTER(Came8Ffn), i32, ctypes.POINTER(sz)]
+        lib.came8_gated_ffn_forward.restype = ctypes.c_int
+        lib.came8_gated_ffn_forward.argtypes = [ctypes.POINTER(Came8Ffn), vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.came8_gated_ffn_backward.restype = ctypes.c_int
+        lib.came8_gated_ffn_backward.argtypes = [ctypes.POINTER(Came8Ffn)] + [vp] * 12 + [sz, vp]
         if lib.came8_abi_version() != ABI_VERSION:
             raise RuntimeError(f"came_amd: {p} has ABI {lib.came8_abi_version()}, expected {ABI_VERSION}")
         _lib = lib

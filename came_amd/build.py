@@ -38,8 +38,9 @@ HIPCC_FLAGS = [
     "-Wno-unused-function",
 ]
 
-# translation units: the host code with the flat-pass kernels, AdamW with the gradient norm, and one per band-pass family
-UNITS = [("came8", "came8.hip", []), ("adamw", "came8_adamw.hip", [])] + [
+# translation units: the host code with the flat-pass kernels, AdamW with the gradient norm, the feed-forward block,
+# and one per band-pass family
+UNITS = [("came8", "came8.hip", []), ("adamw", "came8_adamw.hip", []), ("ffn", "came8_ffn.hip", [])] + [
     (f"band_{t.lower()}_p{p}", "came8_band.hip", [f"-DCAME8_BAND_TYPE={t}", f"-DCAME8_BAND_PASS={p}"])
     for t in ("F32", "BF16", "F16") for p in (1, 2)
 ]

@@ -289,8 +289,8 @@ int came8_dequantize_blockwise(const void* q, const float* absmax, int64_t n, in
                                int32_t block_size, float* out, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
- * Training beside CAME: the global gradient norm, the clip by it, and AdamW over many tensors.  No counterpart
- * in the reference.  As above: the caller owns every buffer, everything is enqueued on `stream`, nothing
+ * Training beside CAME: the global gradient norm, the clip by it, AdamW over many tensors, and the gated feed-forward
+ * block.  No counterpart in the reference.  As above: the caller owns every buffer, everything is enqueued on `stream`, nothing
  * allocates, copies or synchronises.  The tensor lists travel in the kernels' arguments (64 to 192 tensors a
  * launch), so no plan is kept and a call may be captured in a HIP graph.
  * --------------------------------------------------------------------------------------------------------- */
@@ -363,6 +363,37 @@ int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const
 /* out[i] = what code q[i] of an 8-bit second moment stands for (came8_adamw_tensor). */
 int came8_dequantize_second_moment(const uint8_t* q, const float* absmax, int64_t n, int32_t block_size, float* out,
                                    void* stream);
+
+/*
+ * The gated feed-forward block: x [tokens, dim], w_gate and w_up [hidden, dim], w_down [out, hidden], all of type dtype,
+ *   g = x w_gate^T,  u = x w_up^T,  h = act(g) * u,  y = h w_down^T            y [tokens, out]
+ * and its gradients
+ *   dh = dy w_down,  dg = dh * u * act'(g),  du = dh * act(g)
+ *   dx = dg w_gate + du w_up,  dw_gate = dg^T x,  dw_up = du^T x,  dw_down = dy^T h
+ * Sums are held in fp32.  h, dg and du are rounded to dtype once: they are operands of products of that type; g and u
+ * enter h and the gradients unrounded.  Every pointer is 4 bytes aligned.  No counterpart in the reference.
+ */
+#define CAME8_ACT_SILU 0
+#define CAME8_ACT_GELU 1      /* the exact one, by erf */
+#define CAME8_ACT_GELU_TANH 2
+typedef struct came8_ffn {
+  int64_t tokens, dim, hidden, out;
+  int64_t ld_x, ld_gate, ld_up, ld_down; /* elements from a row to the next, at most 2^21; every row is contiguous */
+  int32_t dtype;                         /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t activation;                    /* CAME8_ACT_* */
+} came8_ffn;
+
+/* Bytes of device workspace for the forward (backward = 0) or backward call of this shape. */
+int came8_gated_ffn_workspace_size(const came8_ffn* f, int32_t backward, size_t* bytes);
+
+/* y (contiguous); with g and u not NULL they are kept there for the backward call, float[tokens][hidden] each. */
+int came8_gated_ffn_forward(const came8_ffn* f, const void* x, const void* w_gate, const void* w_up, const void* w_down, void* y,
+                            float* g, float* u, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradients (contiguous; NULL: not wanted) from dy (contiguous) and the g and u that the forward call kept. */
+int came8_gated_ffn_backward(const came8_ffn* f, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                             const void* dy, const float* g, const float* u, void* dx, void* dw_gate, void* dw_up,
+                             void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
