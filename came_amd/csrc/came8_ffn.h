@@ -36,29 +36,39 @@ __device__ __forceinline__ f32x4 mfma_chunk(u32x4 a, u32x4 b, f32x4 c) {
 // ----------------------------------------------------------------------------------------------- activations
 enum { kSilu = 0, kGelu = 1, kGeluTanh = 2 };
 
-// act(g) and its derivative
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+// The hardware's exponential and reciprocal, a unit in the last place each: accurate ones and their divisions were as long
+// as the products (the backward epilogue 1135 us for 8192 by 11008 hidden values, 640 us of it the product).  The error, a
+// few 2^-24 of |g|, is that of one more term in the sums that g comes from.
+__device__ __forceinline__ float exp_hw(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + exp_hw(-g)); }
 
-__device__ __forceinline__ float act_value(float g, int act) {
-  if (act == kSilu) return g * sigmoid(g);
-  if (act == kGelu) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-  const float k = 0.79788456080286536f;
-  return 0.5f * g * (1.0f + tanhf(k * (g + 0.044715f * g * g * g)));
-}
-
-__device__ __forceinline__ float act_slope(float g, int act) {
+// act(g) and, with SLOPE, its derivative, of four values
+template <bool SLOPE>
+__device__ __forceinline__ void activate(const float (&g)[4], int act, float (&value)[4], float (&slope)[4]) {
   if (act == kSilu) {
-    const float s = sigmoid(g);
-    return s * (1.0f + g * (1.0f - s));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float s = sigmoid(g[e]);
+      value[e] = g[e] * s;
+      if (SLOPE) slope[e] = s * (1.0f + g[e] * (1.0f - s));
+    }
+  } else if (act == kGelu) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float c = 0.5f * (1.0f + erff(g[e] * 0.70710678118654752f));
+      value[e] = g[e] * c;
+      if (SLOPE) slope[e] = c + g[e] * exp_hw(-0.5f * g[e] * g[e]) * 0.39894228040143268f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // 0.5 (1 + tanh(x)) = sigmoid(2 x)
+      const float k = 2.0f * 0.79788456080286536f, gg = g[e] * g[e];
+      const float s = sigmoid(k * (g[e] + 0.044715f * gg * g[e]));
+      value[e] = g[e] * s;
+      const float q = s * (1.0f - s);  // 0 long before gg overflows
+      if (SLOPE) slope[e] = s + (q > 0.0f ? g[e] * q * k * (1.0f + 3.0f * 0.044715f * gg) : 0.0f);
+    }
   }
-  if (act == kGelu) {
-    const float c = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    return c + g * expf(-0.5f * g * g) * 0.39894228040143268f;
-  }
-  const float k = 0.79788456080286536f;
-  const float t = tanhf(k * (g + 0.044715f * g * g * g));
-  const float q = 1.0f - t * t;  // 0 long before g * g overflows
-  return 0.5f * (1.0f + t) + (q > 0.0f ? 0.5f * g * q * k * (1.0f + 3.0f * 0.044715f * g * g) : 0.0f);
 }
 
 // ------------------------------------------------------------------------------------------------- arguments
@@ -88,15 +98,25 @@ struct GemmArgs {
   int64_t ldg;
 };
 
-// A tile's view of an operand: reads past the matrix's end give zeros, whatever the tile.  The hardware checks words, and
-// rows start on words (k_ffn_pack), so the last word may count whole: it holds a byte of the matrix.
+// A tile's view of an operand from its next k on: reads past the matrix's end give zeros, whatever the tile.  The hardware
+// checks words, and rows start on words (k_ffn_pack), so the last word may count whole: it holds a byte of the matrix.
 typedef __amdgpu_buffer_rsrc_t Buffer;
-__device__ __forceinline__ Buffer view_at(const void* p, int64_t skip, int64_t total) {
-  const int64_t left = total - skip;
-  const int64_t bytes = left <= 0 ? 0 : ((left + 3) & ~int64_t(3));
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p) + (left <= 0 ? 0 : skip)), 0,
-                                           bytes > 0xfffffffcll ? 0xfffffffcu : uint32_t(bytes), 0x00027000);
-}
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every view's end (offsets within one stay below 2^31)
+struct View {
+  const char* p;
+  int64_t left;  // bytes to the matrix's end, below 1 past it
+  int64_t step;  // bytes to the next k step
+  int32_t ld;    // bytes from a row (or k) to the next
+
+  __device__ __forceinline__ Buffer buffer() const {
+    const int64_t bytes = left <= 0 ? 0 : left > 0x7ffffffcll ? 0x7ffffffcll : (left + 3) & ~int64_t(3);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, int32_t(bytes), 0x00027000);
+  }
+  __device__ __forceinline__ void next() {
+    p += step;
+    left -= step;
+  }
+};
 
 constexpr int kChunkBytes = 16;
 constexpr int kRowBytes = 128;  // of a tile in LDS: 8 chunks, 64 (fp32: 32) values of k
@@ -106,72 +126,73 @@ constexpr int kRowBytes = 128;  // of a tile in LDS: 8 chunks, 64 (fp32: 32) val
 __device__ __forceinline__ int swz(int r) { return (r ^ (r >> 3)) & 7; }
 
 // ------------------------------------------------------------------------------------------------ operands' way in
-// R rows by 8 chunks of k, 256 threads: 16-byte loads into registers (fetch), later written to LDS (put).
-template <typename T, int R, bool ROWS>
+// R rows by 8 chunks of k, NT threads: 16-byte loads into registers (fetch), later written to LDS (put).
+//
+// Rows: a thread loads chunk t % 8 of every NT / 8-th row from row t / 8 on; a chunk at or past k = K lies nowhere and gives
+// zeros (a chunk that K cuts holds zeros in memory).  Columns: a thread loads kLoads successive k of kVec rows, and k past K
+// lie past the end.  HALF > 0: rows taken in turns of HALF from two matrices (the gate's and the up projection's weights);
+// loads i of a thread go to the one and the other in turn.
+template <typename T, int R, int NT, bool ROWS, int HALF = 0>
 struct Stage {
   static constexpr int kElem = int(sizeof(typename T::storage));
   static constexpr int kVec = kChunkBytes / kElem;        // elements of a chunk
-  static constexpr int kLoads = R / 32;                   // 16-byte loads a thread
-  static constexpr int kGroups = kThreads / (R / kVec);   // columns: groups of k values, kLoads each
+  static constexpr int kLoads = R * 8 / NT;               // 16-byte loads a thread
+  static constexpr int kStep = NT / 8;                    // rows: from a load's to the next
   u32x4 v[kLoads];
 
-  __device__ __forceinline__ uint32_t offset(int64_t ld) const {
-    const int t = int(threadIdx.x);
-    if constexpr (ROWS) return uint32_t((t >> 3) * ld * kElem + (t & 7) * kChunkBytes);
-    return uint32_t((t / (R / kVec)) * kLoads * ld * kElem + (t % (R / kVec)) * kChunkBytes);
-  }
-  // rows: rows 32 apart; columns: successive k
-  __device__ __forceinline__ void fetch(Buffer a, uint32_t off, int64_t ld) {
-    const uint32_t step = uint32_t((ROWS ? 32 : 1) * ld * kElem);
+  // left: K less the view's first k
+  __device__ __forceinline__ void fetch(const View& a, const View& a1, int left) {
+    const uint32_t t = threadIdx.x;
+    if constexpr (!ROWS) {
+      const Buffer buf = a.buffer();
+      const uint32_t off = t / (R / kVec) * kLoads * a.ld + t % (R / kVec) * kChunkBytes;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(a, off + i * step, 0, 0);
-  }
-  // rows split over two buffers by halves of `half` rows (the gate's and the up projection's weights)
-  __device__ __forceinline__ void fetch2(Buffer a0, Buffer a1, uint32_t off0, uint32_t off1, int64_t ld0, int64_t ld1, int half) {
-    static_assert(ROWS, "");
+      for (int i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(buf, off + i * a.ld, 0, 0);
+    } else {
+      const bool out = int(t & 7) * kVec >= left;
+      const Buffer buf = a.buffer();
+      const uint32_t off = out ? kNowhere : (t >> 3) * a.ld + (t & 7) * kChunkBytes;
+      if constexpr (HALF == 0) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int row = 32 * i, piece = row / half;
-      const int src = (piece >> 1) * half + row % half;  // row of its matrix's tile
-      v[i] = (piece & 1) ? __builtin_amdgcn_raw_buffer_load_b128(a1, off1 + uint32_t(src * ld1 * kElem), 0, 0)
-                         : __builtin_amdgcn_raw_buffer_load_b128(a0, off0 + uint32_t(src * ld0 * kElem), 0, 0);
-    }
-  }
-  // rows: k >= left becomes zero (left counts from the tile's first k)
-  __device__ __forceinline__ void mask(int left) {
-    if constexpr (ROWS) {
-      const int k0 = (int(threadIdx.x) & 7) * kVec;
+        for (int i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(buf, off + i * kStep * a.ld, 0, 0);
+      } else {
+        const Buffer buf1 = a1.buffer();
+        const uint32_t off1 = out ? kNowhere : (t >> 3) * a1.ld + (t & 7) * kChunkBytes;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          if constexpr (kElem == 4) {
-            if (k0 + w >= left) v[i][w] = 0;
-          } else {
-            if (k0 + 2 * w >= left) v[i][w] = 0;
-            else if (k0 + 2 * w + 1 >= left) v[i][w] &= 0xffffu;
-          }
-        }
+        for (int i = 0; i < kLoads; ++i)
+          v[i] = (i & 1) ? __builtin_amdgcn_raw_buffer_load_b128(buf1, off1 + i / 2 * kStep * a1.ld, 0, 0)
+                         : __builtin_amdgcn_raw_buffer_load_b128(buf, off + i / 2 * kStep * a.ld, 0, 0);
+      }
     }
   }
   __device__ __forceinline__ void put(char* lds) const {
     const int t = int(threadIdx.x);
     if constexpr (ROWS) {
-      const int c = t & 7, r = t >> 3;
+      constexpr int H = HALF == 0 ? kStep : HALF;
+      // the first load's row; load i's is `row` further, which changes the row's swz by an exclusive or
+      const int c = t & 7, r = HALF == 0 ? t >> 3 : (t >> 3) / H * 2 * H + (t >> 3) % H;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        *reinterpret_cast<u32x4*>(lds + (r + 32 * i) * kRowBytes + ((c ^ swz(r + 32 * i)) * kChunkBytes)) = v[i];
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = HALF == 0 ? i * kStep : i / 2 * 2 * kStep + (i & 1) * HALF;
+        *reinterpret_cast<u32x4*>(lds + (r * kRowBytes + ((c ^ swz(r)) ^ (row >> 3 & 7)) * kChunkBytes) + row * kRowBytes) = v[i];
+      }
     } else if constexpr (kElem == 4) {
       const int r = (t % (R / kVec)) * kVec, k = (t / (R / kVec)) * kLoads;  // first row, first k
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (kLoads >= 4) {
 #pragma unroll
-        for (int c = 0; c < kLoads / 4; ++c)
-          *reinterpret_cast<u32x4*>(lds + (r + e) * kRowBytes + (((k / 4 + c) ^ swz(r + e)) * kChunkBytes)) =
-              u32x4{v[4 * c][e], v[4 * c + 1][e], v[4 * c + 2][e], v[4 * c + 3][e]};
+          for (int c = 0; c < kLoads / 4; ++c)
+            *reinterpret_cast<u32x4*>(lds + (r + e) * kRowBytes + (((k / 4 + c) ^ swz(r + e)) * kChunkBytes)) =
+                u32x4{v[4 * c][e], v[4 * c + 1][e], v[4 * c + 2][e], v[4 * c + 3][e]};
+        } else {
+          *reinterpret_cast<u32x2*>(lds + (r + e) * kRowBytes + (((k / 4) ^ swz(r + e)) * kChunkBytes) + (k % 4) * 4) =
+              u32x2{v[0][e], v[1][e]};
+        }
+      }
     } else {
       const int r = (t % (R / kVec)) * kVec, k = (t / (R / kVec)) * kLoads;
-      // v[j] word w holds columns 2w, 2w + 1 of k + j: halves of two words make one word of a row
+      // v[j] word w holds rows 2w, 2w + 1 of k + j: halves of two words make one word of a row
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         uint32_t w[kLoads / 2];
@@ -180,50 +201,128 @@ struct Stage {
           w[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
         char* at = lds + (r + e) * kRowBytes + (((k / 8) ^ swz(r + e)) * kChunkBytes) + (k % 8) * 2;
         if constexpr (kLoads == 8) *reinterpret_cast<u32x4*>(at) = u32x4{w[0], w[1], w[2], w[3]};
-        else *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
+        else if constexpr (kLoads == 4) *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
+        else *reinterpret_cast<uint32_t*>(at) = w[0];
       }
     }
   }
 };
 
+// V consecutive values to a row of N elements at any address, those past N left out (unless the row is padded past it)
+template <typename T>
+__device__ __forceinline__ void store4(void* row, int n, int N, const float (&x)[4]) {
+  using S = typename T::storage;
+  CAME8_GLOBAL S* p = gbl(static_cast<S*>(row)) + n;
+  if (n + 4 <= N) {
+    if constexpr (sizeof(S) == 4)
+      *(CAME8_GLOBAL f32x4u*)p = f32x4u{x[0], x[1], x[2], x[3]};
+    else
+      *(CAME8_GLOBAL u32x2u*)p = u32x2u{uint32_t(T::store(x[0])) | uint32_t(T::store(x[1])) << 16,
+                                        uint32_t(T::store(x[2])) | uint32_t(T::store(x[3])) << 16};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < N) p[e] = T::store(x[e]);
+  }
+}
+
+__device__ __forceinline__ void load4(const float* row, int n, int N, float (&x)[4]) {
+  const CAME8_GLOBAL float* p = gbl(row) + n;
+  if (n + 4 <= N) {
+    const f32x4u v = *(const CAME8_GLOBAL f32x4u*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = n + e < N ? p[e] : 0.0f;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------ product
-// Workgroups of 4 wavefronts, 2 by 2, on a tile of BM by BN.  kGate: the tile's BN rows of weights are, in turns of BN / 4,
-// gate and up projection, so that a wavefront holds both values of its BN / 4 columns of h.
-template <typename T, int BM, int BN, bool AROWS, bool BROWS, Epilogue EPI>
-__global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void k_ffn_gemm(const GemmArgs args) {
+// Asks the scheduler to spread `count` instructions of the given kinds evenly among `products` matrix instructions, and to
+// move nothing past the end of the phase.
+constexpr int kMfma = 0x008, kVmemRead = 0x020, kDsRead = 0x100, kDsWrite = 0x200;
+template <int KINDS, int COUNT, int PRODUCTS, int K = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (K < COUNT) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, PRODUCTS * (K + 1) / COUNT - PRODUCTS * K / COUNT, 0);
+    __builtin_amdgcn_sched_group_barrier(KINDS, 1, 0);
+    interleave<KINDS, COUNT, PRODUCTS, K + 1>();
+  } else {
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Workgroups of 2 by WAVES_N wavefronts on a tile of BM by BN; an accumulator lane holds 4 consecutive columns of a row.
+// kGate: the tile's BN rows of weights are, in turns of half a wavefront's, gate and up projection, so that a wavefront
+// holds both values of its columns of h.
+//
+// Step t of k: half of its fragments are multiplied while the other half is read from LDS and the operands of step t + 1 go
+// from registers to the other LDS buffer; after the step's one barrier the second half is multiplied while step t + 1's first
+// fragments are read and the operands of step t + 2 are loaded.  So neither LDS reads nor global loads are waited for at the
+// barrier.  Steps past the end load zeros.
+template <typename T, int BM, int BN, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
+__global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmArgs args) {
   using S = typename T::storage;
   constexpr int kElem = int(sizeof(S));
   constexpr int BK = kRowBytes / kElem;
-  constexpr int WM = BM / 2, WN = BN / 2, FM = WM / 16, FN = WN / 16;
-  constexpr int kHalf = BN / 4;
+  constexpr int NT = 2 * WAVES_N * kWave;
+  constexpr int WM = BM / 2, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
   constexpr int kTileBytes = (BM + BN) * kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[2 * kTileBytes];
 
-  const int tm = int(blockIdx.x) % args.tiles_m, tn = int(blockIdx.x) / args.tiles_m;
+  // Workgroups go to the 8 XCDs in turn: each XCD gets a run of successive tiles, 8 tiles of rows by the columns.
+  int tm, tn;
+  {
+    const int tiles = args.tiles_m * args.tiles_n, b = int(blockIdx.x);
+    const int each = tiles / kXcds, more = tiles % kXcds, x = b % kXcds;
+    const int id = x * each + min(x, more) + b / kXcds;
+    constexpr int kGroup = 8;
+    const int first = id / (kGroup * args.tiles_n) * kGroup, rows = min(kGroup, args.tiles_m - first);
+    const int in = id - first * args.tiles_n;
+    tm = first + in % rows;
+    tn = in / rows;
+  }
   const int m0 = tm * BM, n0 = tn * (EPI == kGate ? BN / 2 : BN);
   const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
   const int wm = wave & 1, wn = wave >> 1;
 
-  Stage<T, BM, AROWS> sa;
-  Stage<T, BN, BROWS> sb;
+  Stage<T, BM, NT, AROWS> sa;
+  Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0> sb;
   const int steps = (args.K + BK - 1) / BK, total = steps * args.nseg;
-  auto view = [&](const Operand& o, bool rows, int at, int extent, int k0) {
-    const int64_t skip = (rows ? int64_t(at) * o.ld + k0 : int64_t(k0) * o.ld + at) * kElem;
-    const int64_t end = (rows ? int64_t(extent - 1) * o.ld + args.K : int64_t(args.K - 1) * o.ld + extent) * kElem;
-    return view_at(o.p, skip, end);
+  auto view = [&](const Operand& o, bool rows, int at, int extent) {
+    const int64_t ld = o.ld * kElem;
+    View v;
+    v.p = static_cast<const char*>(o.p) + (rows ? at * ld : int64_t(at) * kElem);
+    v.left = rows ? (extent - at) * ld : (args.K - 1) * ld + int64_t(extent - at) * kElem;
+    v.step = rows ? kRowBytes : BK * ld;
+    v.ld = int32_t(ld);
+    return v;
   };
-  auto fetch = [&](int t) {
-    const int s = t >= steps ? 1 : 0, k0 = (t - s * steps) * BK;
-    const Segment& seg = args.seg[s];
-    sa.fetch(view(seg.a, AROWS, m0, args.M, k0), sa.offset(seg.a.ld), seg.a.ld);
-    if constexpr (EPI == kGate)
-      sb.fetch2(view(seg.b, true, n0, args.N, k0), view(args.b2, true, n0, args.N, k0), sb.offset(seg.b.ld),
-                sb.offset(args.b2.ld), seg.b.ld, args.b2.ld, kHalf);
-    else
-      sb.fetch(view(seg.b, BROWS, n0, args.N, k0), sb.offset(seg.b.ld), seg.b.ld);
-    if (k0 + BK > args.K) {
-      sa.mask(args.K - k0);
-      sb.mask(args.K - k0);
+  View va = view(args.seg[0].a, AROWS, m0, args.M), vb = view(args.seg[0].b, EPI == kGate || BROWS, n0, args.N);
+  // the second segment's (kGate: the up projection's weights)
+  const View va1 = args.nseg > 1 ? view(args.seg[1].a, AROWS, m0, args.M) : va;
+  View vb1 = EPI == kGate ? view(args.b2, true, n0, args.N) : args.nseg > 1 ? view(args.seg[1].b, BROWS, n0, args.N) : vb;
+  int ahead = 0, left = args.K;  // the step that is fetched next, and K less its first k
+  auto fetch = [&]() __attribute__((always_inline)) {
+    sa.fetch(va, va, left);
+    sb.fetch(vb, vb1, left);
+    va.next();
+    vb.next();
+    left -= BK;
+    if constexpr (EPI == kGate) {
+      vb1.next();
+    } else {
+      const bool turn = ++ahead == steps && args.nseg > 1;
+      va.p = turn ? va1.p : va.p;
+      va.left = turn ? va1.left : va.left;
+      va.step = turn ? va1.step : va.step;
+      va.ld = turn ? va1.ld : va.ld;
+      vb.p = turn ? vb1.p : vb.p;
+      vb.left = turn ? vb1.left : vb.left;
+      vb.step = turn ? vb1.step : vb.step;
+      vb.ld = turn ? vb1.ld : vb.ld;
+      left = turn ? args.K : left;
     }
   };
   auto put = [&](int t) {
@@ -231,81 +330,154 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void k_ffn_gemm(const 
     sa.put(to);
     sb.put(to + BM * kRowBytes);
   };
+  // Fragment i of half s: row 16 i + lane % 16 of the wavefront's, chunk 4 s + lane / 16, at place
+  // (lane / 16) ^ swz(the wavefront's first row + lane % 16) ^ 4 s ^ 2 (i & 3).
+  const int fr = lane % 16;
+  uint32_t pa[4], pb[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    pa[v] = uint32_t((wm * WM + fr) * kRowBytes + (lane / 16 ^ swz(wm * (WM % 64) + fr) ^ (2 * v)) * kChunkBytes);
+    pb[v] = uint32_t((BM + wn * WN + fr) * kRowBytes + (lane / 16 ^ swz(wn * (WN % 64) + fr) ^ (2 * v)) * kChunkBytes);
+  }
+  u32x4 lo[FM / 2], hi[FM / 2], fb[2][FN];
+  auto read_a = [&](u32x4(&f)[FM / 2], int t, int s, int i0) __attribute__((always_inline)) {
+    const char* a = lds + (t & 1) * kTileBytes;
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i)
+      f[i] = *reinterpret_cast<const u32x4*>(a + pa[(2 * s) ^ ((i0 + i) & 3)] + (i0 + i) * 16 * kRowBytes);
+  };
+  auto read_b = [&](int t, int s, int j0) __attribute__((always_inline)) {
+    const char* b = lds + (t & 1) * kTileBytes;
+#pragma unroll
+    for (int j = j0; j < j0 + FN / 2; ++j)
+      fb[s][j] = *reinterpret_cast<const u32x4*>(b + pb[(2 * s) ^ (j & 3)] + j * 16 * kRowBytes);
+  };
 
   f32x4 acc[FM][FN] = {};
-  fetch(0);
+  auto multiply = [&](const u32x4(&f)[FM / 2], int s, int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i0 + i][j] = mfma_chunk<T>(fb[s][j], f[i], acc[i0 + i][j]);
+  };
+  constexpr int kProducts = FM / 2 * FN * (kElem == 4 ? 4 : 1);  // of a phase
+  fetch();
+  put(0);
+  fetch();
+  __syncthreads();
+  read_a(lo, 0, 0, 0);
+  read_b(0, 0, 0);
+  read_b(0, 0, FN / 2);
   for (int t = 0; t < total; ++t) {
-    put(t);
-    if (t + 1 < total) fetch(t + 1);
+    read_a(hi, t, 0, FM / 2);
+    read_b(t, 1, 0);
+    read_b(t, 1, FN / 2);
+    multiply(lo, 0, 0);
+    interleave<kDsRead, FM / 2 + FN, kProducts>();
+    read_a(lo, t, 1, 0);
+    put(t + 1);
+    multiply(hi, 0, FM / 2);
+    interleave<kDsRead | kDsWrite, FM / 2 + FM + FN, kProducts>();
     __syncthreads();
-    const char* at = lds + (t & 1) * kTileBytes;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4 a[FM], b[FN];
-      const int c = s * 4 + lane / 16;
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int r = wm * WM + i * 16 + lane % 16;
-        a[i] = *reinterpret_cast<const u32x4*>(at + r * kRowBytes + (c ^ swz(r)) * kChunkBytes);
-      }
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int r = wn * WN + j * 16 + lane % 16;
-        b[j] = *reinterpret_cast<const u32x4*>(at + (BM + r) * kRowBytes + (c ^ swz(r)) * kChunkBytes);
-      }
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_chunk<T>(b[j], a[i], acc[i][j]);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    read_a(hi, t, 1, FM / 2);
+    read_b(t + 1, 0, 0);
+    read_b(t + 1, 0, FN / 2);
+    multiply(lo, 1, 0);
+    interleave<kDsRead, FM / 2 + FN, kProducts>();
+    fetch();
+    read_a(lo, t + 1, 0, 0);
+    multiply(hi, 1, FM / 2);
+    interleave<kDsRead | kVmemRead, FM / 2 + FM + FN, kProducts>();
   }
 
-  // acc[i][j][e]: row m0 + wm WM + 16 i + lane % 16, column n0 + wn WN + 16 j + 4 (lane / 16) + e (kGate: of the weights' rows)
+  // acc[i][j][e]: row 16 i + lane % 16 of the wavefront's, column 16 j + 4 (lane / 16) + e.  Up to 64 rows at a time go
+  // through the wavefront's own part of LDS, so that lanes of successive columns read and write memory together; chunk c of
+  // row r lies at c ^ r.  Several rounds' reads of g and u are in flight before the first is used.
+  constexpr int kPart = FM < 4 ? FM : 4;
+  constexpr int kChunks = WN / 4;
+  static_assert(2 * WAVES_N * kPart * 16 * WN * 4 <= 2 * kTileBytes, "");
+  char* mine = lds + wave * (kPart * 16 * WN * 4);
+  constexpr int kCols = EPI == kGate ? WN / 2 : WN;  // of the output
+  constexpr int kLanes = kCols / 4, kRows = kWave / kLanes, kRounds = kPart * 16 / kRows;
+  constexpr int kBatch = kRounds < 4 ? kRounds : 4;
+  const int cc = lane % kLanes, r0 = lane / kLanes, n = n0 + wn * kCols + cc * 4;
+  auto slot = [&](int r, int c) { return reinterpret_cast<f32x4*>(mine + r * (WN * 4) + ((c ^ r) & (kChunks - 1)) * 16); };
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + wm * WM + i * 16 + lane % 16;
-    if (m >= args.M) continue;
+  for (int part = 0; part < FM / kPart; ++part) {
 #pragma unroll
-    for (int j = 0; j < (EPI == kGate ? FN / 2 : FN); ++j) {
-      const int n = n0 + wn * (EPI == kGate ? kHalf : WN) + j * 16 + (lane / 16) * 4;
-      if (n >= args.N) continue;
-      const int64_t o = int64_t(m) * args.ldo + n, og = int64_t(m) * args.ldg + n;
+    for (int i = 0; i < kPart; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n + e >= args.N) break;
+      for (int j = 0; j < FN; ++j) *slot(i * 16 + lane % 16, j * 4 + lane / 16) = acc[part * kPart + i][j];
+#pragma unroll 1
+    for (int q = 0; q < kRounds; q += kBatch) {
+      const int m = m0 + wm * WM + part * kPart * 16 + q * kRows + r0;
+      float g[kBatch][4], u[kBatch][4];
+      if constexpr (EPI == kBack) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (m + k * kRows < args.M) {
+            load4(args.g + int64_t(m + k * kRows) * args.ldg, n, args.N, g[k]);
+            load4(args.u + int64_t(m + k * kRows) * args.ldg, n, args.N, u[k]);
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = (q + k) * kRows + r0;
+        if (m + k * kRows >= args.M) break;
+        const int64_t row = m + k * kRows;
+        const f32x4 c = *slot(r, cc);
+        S* out = static_cast<S*>(args.out) + row * args.ldo;
         if constexpr (EPI == kStore) {
-          static_cast<S*>(args.out)[o + e] = T::store(acc[i][j][e]);
+          store4<T>(out, n, args.N, {c[0], c[1], c[2], c[3]});
         } else if constexpr (EPI == kGate) {
-          const float g = acc[i][j][e], u = acc[i][j + FN / 2][e];
-          static_cast<S*>(args.out)[o + e] = T::store(act_value(g, args.act) * u);
+          const f32x4 d = *slot(r, cc + kChunks / 2);
+          float h[4], none[4];
+          activate<false>({c[0], c[1], c[2], c[3]}, args.act, h, none);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] *= d[e];
+          store4<T>(out, n, int(args.ldo), h);  // zeros up to the padded end
           if (args.g) {
-            args.g[og + e] = g;
-            args.u[og + e] = u;
+            store4<F32>(args.g + row * args.ldg, n, args.N, {c[0], c[1], c[2], c[3]});
+            store4<F32>(args.u + row * args.ldg, n, args.N, {d[0], d[1], d[2], d[3]});
           }
         } else {
-          const float g = args.g[og + e], u = args.u[og + e], dh = acc[i][j][e], a = act_value(g, args.act);
-          static_cast<S*>(args.out)[o + e] = T::store(dh * u * act_slope(g, args.act));
-          static_cast<S*>(args.out2)[o + e] = T::store(dh * a);
-          if (args.out3) static_cast<S*>(args.out3)[o + e] = T::store(a * u);
+          float h[4], dg[4], du[4];
+          activate<true>(g[k], args.act, h, dg);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            du[e] = c[e] * h[e];
+            dg[e] *= c[e] * u[k][e];
+            h[e] *= u[k][e];
+          }
+          store4<T>(out, n, int(args.ldo), dg);
+          store4<T>(static_cast<S*>(args.out2) + row * args.ldo, n, int(args.ldo), du);
+          if (args.out3) store4<T>(static_cast<S*>(args.out3) + row * args.ldo, n, int(args.ldo), h);
         }
       }
     }
   }
 }
 
-// Rows of 16-bit elements at an odd stride, copied to an even one: a row that starts in the middle of a word would have its
-// last element in a word that the hardware's check of a buffer's end refuses.
-__global__ __launch_bounds__(kThreads) void k_ffn_pack(const uint16_t* from, int64_t ld, uint16_t* to, int64_t ldt, int64_t rows,
-                                                       int32_t cols) {
+// A copy of an operand's rows with zeros up to the stride ldt, a multiple of a chunk: for rows that do not start on words (a
+// row that starts in the middle of one would have its last element in a word that the hardware's check of a buffer's end
+// refuses) and for rows that end inside a chunk.
+template <typename S>
+__global__ __launch_bounds__(kThreads) void k_ffn_pack(const S* from, int64_t ld, S* to, int64_t ldt, int64_t rows, int32_t cols) {
+  constexpr int V = 16 / int(sizeof(S));
+  typedef S vec __attribute__((ext_vector_type(V), aligned(sizeof(S))));
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int32_t c = int32_t(threadIdx.x) * 8; c < cols; c += kThreads * 8) {
-      const CAME8_GLOBAL uint16_t* p = gbl(from) + r * ld + c;
-      CAME8_GLOBAL uint16_t* q = gbl(to) + r * ldt + c;
-      if (c + 8 <= cols) {
-        *(CAME8_GLOBAL u32x4*)q = *(const CAME8_GLOBAL u32x4u*)p;
+    for (int32_t c = int32_t(threadIdx.x) * V; c < ldt; c += kThreads * V) {
+      const CAME8_GLOBAL S* p = gbl(from) + r * ld + c;
+      vec x;
+      if (c + V <= cols) {
+        x = *(const CAME8_GLOBAL vec*)p;
       } else {
-        for (int e = 0; c + e < cols; ++e) q[e] = p[e];
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = c + e < cols ? p[e] : S(0);
       }
+      *(CAME8_GLOBAL vec*)(gbl(to) + r * ldt + c) = x;
     }
 }
 

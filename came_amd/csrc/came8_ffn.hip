@@ -15,8 +15,8 @@ namespace {
 
 int64_t up(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 
-// What lies in the workspace: h (and dg, du), and copies of the operands whose rows do not start on words (k_ffn_pack).
-// Every row there starts 16 bytes aligned.
+// What lies in the workspace: h (and dg, du), and copies of the operands whose rows do not start on words or end inside a
+// chunk (k_ffn_pack).  Every row there starts 16 bytes aligned and ends in zeros.
 struct Layout {
   int64_t ldh = 0;  // elements
   size_t h = 0, dg = 0, du = 0, bytes = 0;
@@ -26,7 +26,9 @@ struct Layout {
   } x, gate, up, down, dy;
 };
 
-bool odd(const came8_ffn* f, int64_t ld) { return f->dtype != CAME8_F32 && ld % 2 != 0; }
+bool ragged(const came8_ffn* f, int64_t cols, int64_t ld) {
+  return f->dtype == CAME8_F32 ? cols % 4 != 0 : cols % 8 != 0 || ld % 2 != 0;
+}
 
 Layout layout_of(const came8_ffn* f, bool backward) {
   Layout l;
@@ -37,8 +39,8 @@ Layout layout_of(const came8_ffn* f, bool backward) {
     return at;
   };
   auto copy = [&](Layout::Copy& c, int64_t rows, int64_t cols, int64_t ld) {
-    if (!odd(f, ld)) return;
-    c.ld = up(cols, 8);
+    if (!ragged(f, cols, ld)) return;
+    c.ld = up(cols, 16 / es);
     c.at = take(rows, c.ld);
   };
   l.ldh = up(f->hidden, 16 / es);
@@ -56,15 +58,16 @@ Layout layout_of(const came8_ffn* f, bool backward) {
 }
 
 // The operand as the kernels read it: itself, or its copy in the workspace.
+template <typename S>
 Operand operand(const void* p, int64_t rows, int64_t cols, int64_t ld, const Layout::Copy& c, char* ws, hipStream_t stream) {
   if (c.ld == 0) return {p, ld};
-  hipLaunchKernelGGL(k_ffn_pack, dim3(unsigned(std::min<int64_t>(rows, 1 << 16))), dim3(kThreads), 0, stream,
-                     static_cast<const uint16_t*>(p), ld, reinterpret_cast<uint16_t*>(ws + c.at), c.ld, rows, int32_t(cols));
+  hipLaunchKernelGGL(k_ffn_pack<S>, dim3(unsigned(std::min<int64_t>(rows, 1 << 16))), dim3(kThreads), 0, stream,
+                     static_cast<const S*>(p), ld, reinterpret_cast<S*>(ws + c.at), c.ld, rows, int32_t(cols));
   return {ws + c.at, c.ld};
 }
 
 constexpr int64_t kMaxTokens = int64_t(1) << 24;
-constexpr int64_t kMaxStride = int64_t(1) << 21;   // of rows, in elements: a tile's 256 rows stay below 2^32 bytes
+constexpr int64_t kMaxStride = int64_t(1) << 20;   // of rows, in elements: a tile's 256 rows stay below 2^31 bytes
 constexpr int64_t kMaxMatrix = int64_t(1) << 36;   // elements: a launch's work items stay below 2^32
 
 int check(const char* what, const came8_ffn* f) {
@@ -75,11 +78,11 @@ int check(const char* what, const came8_ffn* f) {
   if (f->activation < CAME8_ACT_SILU || f->activation > CAME8_ACT_GELU_TANH)
     return op_fail(CAME8_EINVAL, at + "unknown activation " + std::to_string(f->activation));
   if (f->tokens < 0 || f->tokens > kMaxTokens || f->dim < 1 || f->hidden < 1 || f->out < 1 || f->out > kMaxStride)
-    return op_fail(CAME8_EINVAL, at + "tokens must be in [0, 2^24], dim, hidden and out in [1, 2^21]");
+    return op_fail(CAME8_EINVAL, at + "tokens must be in [0, 2^24], dim, hidden and out in [1, 2^20]");
   const int64_t strides[4][2] = {{f->ld_x, f->dim}, {f->ld_gate, f->dim}, {f->ld_up, f->dim}, {f->ld_down, f->hidden}};
   for (const auto& s : strides)
     if (s[0] < s[1] || s[0] > kMaxStride)
-      return op_fail(CAME8_EINVAL, at + "a row stride must be at least the row's length and at most 2^21");
+      return op_fail(CAME8_EINVAL, at + "a row stride must be at least the row's length and at most 2^20");
   for (const int64_t n : {f->tokens * f->hidden, f->tokens * f->out, f->tokens * f->dim, f->hidden * f->dim, f->hidden * f->out})
     if (n > kMaxMatrix) return op_fail(CAME8_EINVAL, at + "a matrix of more than 2^36 elements");
   return CAME8_OK;
@@ -92,14 +95,29 @@ int check_pointers(const char* what, std::initializer_list<const void*> ps) {
   return CAME8_OK;
 }
 
-template <typename T, bool AROWS, bool BROWS, Epilogue EPI>
-void launch(GemmArgs a, hipStream_t stream) {
-  constexpr int BM = 128, BN = 128;
-  a.tiles_m = (a.M + BM - 1) / BM;
-  constexpr int cols = EPI == kGate ? BN / 2 : BN;
+template <typename T, int B, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
+bool launch_tiles(GemmArgs a, int64_t least, hipStream_t stream) {
+  constexpr int cols = EPI == kGate ? B / 2 : B;
+  a.tiles_m = (a.M + B - 1) / B;
   a.tiles_n = (a.N + cols - 1) / cols;
-  hipLaunchKernelGGL((k_ffn_gemm<T, BM, BN, AROWS, BROWS, EPI>), dim3(unsigned(a.tiles_m) * unsigned(a.tiles_n)),
-                     dim3(kThreads), 0, stream, a);
+  const int64_t tiles = int64_t(a.tiles_m) * a.tiles_n;
+  if (tiles < least) return false;
+  hipLaunchKernelGGL((k_ffn_gemm<T, B, B, WAVES_N, AROWS, BROWS, EPI>), dim3(unsigned(tiles)), dim3(2 * WAVES_N * kWave), 0, stream, a);
+  return true;
+}
+
+template <typename T, bool AROWS, bool BROWS, Epilogue EPI>
+void launch(const GemmArgs& a, hipStream_t stream) {
+#ifndef MIN256
+#define MIN256 200
+#endif
+#ifndef MIN128
+#define MIN128 200
+#endif
+  if constexpr (!std::is_same<T, F32>::value)
+    if (launch_tiles<T, 256, 4, AROWS, BROWS, EPI>(a, MIN256, stream)) return;
+  if (launch_tiles<T, 128, 2, AROWS, BROWS, EPI>(a, MIN128, stream)) return;
+  launch_tiles<T, 64, 2, AROWS, BROWS, EPI>(a, 0, stream);
 }
 
 template <typename T>
@@ -109,16 +127,16 @@ void forward(const came8_ffn* f, const void* x, const void* wg, const void* wu, 
   a.nseg = 1;
   a.act = f->activation;
   a.M = int32_t(f->tokens), a.N = int32_t(f->hidden), a.K = int32_t(f->dim);
-  a.seg[0] = {operand(x, f->tokens, f->dim, f->ld_x, l.x, ws, stream),
-              operand(wg, f->hidden, f->dim, f->ld_gate, l.gate, ws, stream)};
-  a.b2 = operand(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream);
+  a.seg[0] = {operand<typename T::storage>(x, f->tokens, f->dim, f->ld_x, l.x, ws, stream),
+              operand<typename T::storage>(wg, f->hidden, f->dim, f->ld_gate, l.gate, ws, stream)};
+  a.b2 = operand<typename T::storage>(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream);
   a.out = ws + l.h, a.ldo = l.ldh;
   a.g = g, a.u = u, a.ldg = f->hidden;
   launch<T, true, true, kGate>(a, stream);
   GemmArgs d{};
   d.nseg = 1;
   d.M = int32_t(f->tokens), d.N = int32_t(f->out), d.K = int32_t(f->hidden);
-  d.seg[0] = {{ws + l.h, l.ldh}, operand(wd, f->out, f->hidden, f->ld_down, l.down, ws, stream)};
+  d.seg[0] = {{ws + l.h, l.ldh}, operand<typename T::storage>(wd, f->out, f->hidden, f->ld_down, l.down, ws, stream)};
   d.out = y, d.ldo = f->out;
   launch<T, true, true, kStore>(d, stream);
 }
@@ -130,9 +148,9 @@ void backward(const came8_ffn* f, const void* x, const void* wg, const void* wu,
   a.nseg = 1;
   a.act = f->activation;
   a.M = int32_t(f->tokens), a.N = int32_t(f->hidden), a.K = int32_t(f->out);
-  const Operand pdy = operand(dy, f->tokens, f->out, f->out, l.dy, ws, stream);
-  const Operand px = operand(x, f->tokens, f->dim, f->ld_x, l.x, ws, stream);
-  a.seg[0] = {pdy, operand(wd, f->out, f->hidden, f->ld_down, l.down, ws, stream)};
+  const Operand pdy = operand<typename T::storage>(dy, f->tokens, f->out, f->out, l.dy, ws, stream);
+  const Operand px = operand<typename T::storage>(x, f->tokens, f->dim, f->ld_x, l.x, ws, stream);
+  a.seg[0] = {pdy, operand<typename T::storage>(wd, f->out, f->hidden, f->ld_down, l.down, ws, stream)};
   a.out = ws + l.dg, a.out2 = ws + l.du, a.out3 = dwd ? ws + l.h : nullptr, a.ldo = l.ldh;
   a.g = const_cast<float*>(g), a.u = const_cast<float*>(u), a.ldg = f->hidden;
   launch<T, true, false, kBack>(a, stream);
@@ -140,8 +158,8 @@ void backward(const came8_ffn* f, const void* x, const void* wg, const void* wu,
   if (dx) {
     d.nseg = 2;
     d.M = int32_t(f->tokens), d.N = int32_t(f->dim), d.K = int32_t(f->hidden);
-    d.seg[0] = {{ws + l.dg, l.ldh}, operand(wg, f->hidden, f->dim, f->ld_gate, l.gate, ws, stream)};
-    d.seg[1] = {{ws + l.du, l.ldh}, operand(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream)};
+    d.seg[0] = {{ws + l.dg, l.ldh}, operand<typename T::storage>(wg, f->hidden, f->dim, f->ld_gate, l.gate, ws, stream)};
+    d.seg[1] = {{ws + l.du, l.ldh}, operand<typename T::storage>(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream)};
     d.out = dx, d.ldo = f->dim;
     launch<T, true, false, kStore>(d, stream);
   }

@@ -21,7 +21,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-D tensor whose rows are contiguous and do not overlap, at a 4-byte aligned address (a copy where they are not, or
     lie too far apart)."""
     n = t.shape[1]
-    if (t.stride(1) == 1 or n == 1) and (t.shape[0] == 1 or n <= t.stride(0) <= 1 << 21) and t.data_ptr() % 4 == 0:
+    if (t.stride(1) == 1 or n == 1) and (t.shape[0] == 1 or n <= t.stride(0) <= 1 << 20) and t.data_ptr() % 4 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -378,7 +378,7 @@ int came8_dequantize_second_moment(const uint8_t* q, const float* absmax, int64_
 #define CAME8_ACT_GELU_TANH 2
 typedef struct came8_ffn {
   int64_t tokens, dim, hidden, out;
-  int64_t ld_x, ld_gate, ld_up, ld_down; /* elements from a row to the next, at most 2^21; every row is contiguous */
+  int64_t ld_x, ld_gate, ld_up, ld_down; /* elements from a row to the next, at most 2^20; every row is contiguous */
   int32_t dtype;                         /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
   int32_t activation;                    /* CAME8_ACT_* */
 } came8_ffn;
