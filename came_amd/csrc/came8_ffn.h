@@ -88,6 +88,8 @@ struct GemmArgs {
   int32_t nseg;
   int32_t M, N, K;  // K: of each segment
   int32_t tiles_m, tiles_n;
+  int32_t splits;   // workgroups that share a tile's sum (kStore, kBack)
+  float* part;      // splits > 1: their sums, [splits][M][N up to a multiple of 4], for k_ffn_join; else null
   int32_t act;
   void* out;        // kStore: C; kGate: h; kBack: dg
   int64_t ldo;
@@ -112,9 +114,9 @@ struct View {
     const int64_t bytes = left <= 0 ? 0 : left > 0x7ffffffcll ? 0x7ffffffcll : (left + 3) & ~int64_t(3);
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, int32_t(bytes), 0x00027000);
   }
-  __device__ __forceinline__ void next() {
-    p += step;
-    left -= step;
+  __device__ __forceinline__ void next(int64_t steps = 1) {
+    p += step * steps;
+    left -= step * steps;
   }
 };
 
@@ -238,6 +240,26 @@ __device__ __forceinline__ void load4(const float* row, int n, int N, float (&x)
   }
 }
 
+// dg, du and h of four values, from dh, g and u (zeros past N, where rows are padded)
+template <typename T>
+__device__ __forceinline__ void store_back(const GemmArgs& args, int64_t row, int n, const float (&dh)[4], const float (&g)[4],
+                                           const float (&u)[4]) {
+  using S = typename T::storage;
+  float h[4], dg[4], du[4];
+  activate<true>(g, args.act, h, dg);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool in = n + e < args.N;  // past N dh is of no column, and may hold anything
+    du[e] = in ? dh[e] * h[e] : 0.0f;
+    dg[e] = in ? dg[e] * (dh[e] * u[e]) : 0.0f;
+    h[e] = in ? h[e] * u[e] : 0.0f;
+  }
+  const int ld = int(args.ldo);
+  store4<T>(static_cast<S*>(args.out) + row * args.ldo, n, ld, dg);
+  store4<T>(static_cast<S*>(args.out2) + row * args.ldo, n, ld, du);
+  if (args.out3) store4<T>(static_cast<S*>(args.out3) + row * args.ldo, n, ld, h);
+}
+
 // ------------------------------------------------------------------------------------------------------ product
 // Asks the scheduler to spread `count` instructions of the given kinds evenly among `products` matrix instructions, and to
 // move nothing past the end of the phase.
@@ -262,21 +284,22 @@ __device__ __forceinline__ void interleave() {
 // fragments are read and the operands of step t + 2 are loaded.  So neither LDS reads nor global loads are waited for at the
 // barrier.  Steps past the end load zeros.
 template <typename T, int BM, int BN, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
-__global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmArgs args) {
+__device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) {
   using S = typename T::storage;
   constexpr int kElem = int(sizeof(S));
   constexpr int BK = kRowBytes / kElem;
   constexpr int NT = 2 * WAVES_N * kWave;
   constexpr int WM = BM / 2, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
   constexpr int kTileBytes = (BM + BN) * kRowBytes;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kTileBytes];
 
   // Workgroups go to the 8 XCDs in turn: each XCD gets a run of successive tiles, 8 tiles of rows by the columns.
-  int tm, tn;
+  int tm, tn, split;
   {
-    const int tiles = args.tiles_m * args.tiles_n, b = int(blockIdx.x);
-    const int each = tiles / kXcds, more = tiles % kXcds, x = b % kXcds;
-    const int id = x * each + min(x, more) + b / kXcds;
+    const int tiles = args.tiles_m * args.tiles_n, all = tiles * args.splits;
+    const int each = all / kXcds, more = all % kXcds, x = b % kXcds;
+    int id = x * each + min(x, more) + b / kXcds;
+    split = id / tiles;
+    id -= split * tiles;
     constexpr int kGroup = 8;
     const int first = id / (kGroup * args.tiles_n) * kGroup, rows = min(kGroup, args.tiles_m - first);
     const int in = id - first * args.tiles_n;
@@ -289,7 +312,10 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmA
 
   Stage<T, BM, NT, AROWS> sa;
   Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0> sb;
-  const int steps = (args.K + BK - 1) / BK, total = steps * args.nseg;
+  const int steps = (args.K + BK - 1) / BK;
+  const int every = steps * args.nseg;
+  int ahead = int(int64_t(every) * split / args.splits);  // the step that is fetched next
+  const int total = int(int64_t(every) * (split + 1) / args.splits) - ahead;
   auto view = [&](const Operand& o, bool rows, int at, int extent) {
     const int64_t ld = o.ld * kElem;
     View v;
@@ -303,7 +329,13 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmA
   // the second segment's (kGate: the up projection's weights)
   const View va1 = args.nseg > 1 ? view(args.seg[1].a, AROWS, m0, args.M) : va;
   View vb1 = EPI == kGate ? view(args.b2, true, n0, args.N) : args.nseg > 1 ? view(args.seg[1].b, BROWS, n0, args.N) : vb;
-  int ahead = 0, left = args.K;  // the step that is fetched next, and K less its first k
+  if (EPI != kGate && ahead >= steps && args.nseg > 1) {
+    va = va1;
+    vb = vb1;
+  }
+  int left = args.K - (ahead % steps) * BK;  // K less the next step's first k
+  va.next(ahead % steps);
+  vb.next(ahead % steps);
   auto fetch = [&]() __attribute__((always_inline)) {
     sa.fetch(va, va, left);
     sb.fetch(vb, vb1, left);
@@ -414,7 +446,7 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmA
     for (int q = 0; q < kRounds; q += kBatch) {
       const int m = m0 + wm * WM + part * kPart * 16 + q * kRows + r0;
       float g[kBatch][4], u[kBatch][4];
-      if constexpr (EPI == kBack) {
+      if (EPI == kBack && args.part == nullptr) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
           if (m + k * kRows < args.M) {
@@ -425,9 +457,16 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmA
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int r = (q + k) * kRows + r0;
-        if (m + k * kRows >= args.M) break;
+        if (m + k * kRows >= args.M) continue;
         const int64_t row = m + k * kRows;
         const f32x4 c = *slot(r, cc);
+        if constexpr (EPI != kGate) {
+          if (args.part) {
+            const int pitch = (args.N + 3) & ~3;
+            store4<F32>(args.part + (int64_t(split) * args.M + row) * pitch, n, pitch, {c[0], c[1], c[2], c[3]});
+            continue;
+          }
+        }
         S* out = static_cast<S*>(args.out) + row * args.ldo;
         if constexpr (EPI == kStore) {
           store4<T>(out, n, args.N, {c[0], c[1], c[2], c[3]});
@@ -443,19 +482,61 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmA
             store4<F32>(args.u + row * args.ldg, n, args.N, {d[0], d[1], d[2], d[3]});
           }
         } else {
-          float h[4], dg[4], du[4];
-          activate<true>(g[k], args.act, h, dg);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            du[e] = c[e] * h[e];
-            dg[e] *= c[e] * u[k][e];
-            h[e] *= u[k][e];
-          }
-          store4<T>(out, n, int(args.ldo), dg);
-          store4<T>(static_cast<S*>(args.out2) + row * args.ldo, n, int(args.ldo), du);
-          if (args.out3) store4<T>(static_cast<S*>(args.out3) + row * args.ldo, n, int(args.ldo), h);
+          store_back<T>(args, row, n, {c[0], c[1], c[2], c[3]}, g[k], u[k]);
         }
       }
+    }
+  }
+}
+
+template <typename T, int B, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
+__global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmArgs args) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * B * kRowBytes];
+  product<T, B, B, WAVES_N, AROWS, BROWS, EPI>(args, int(blockIdx.x), lds);
+}
+
+// The products that only wait for dg, du and h: dx and the weights' gradients, one launch, the longest sums first.  The last
+// tiles of one fill the CUs beside the first of the next.
+struct GradArgs {
+  GemmArgs dx;
+  GemmArgs dw[3];
+  int32_t first[4];  // workgroups before each dw, and all
+};
+template <typename T, int B, int WAVES_N>
+__global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_grads(const GradArgs args) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * B * kRowBytes];
+  const int b = int(blockIdx.x);
+  if (b < args.first[0]) {
+    product<T, B, B, WAVES_N, true, false, kStore>(args.dx, b, lds);
+  } else {
+    const int k = (b >= args.first[1]) + (b >= args.first[2]);
+    product<T, B, B, WAVES_N, false, false, kStore>(args.dw[k], b - args.first[k], lds);
+  }
+}
+
+// The shares of tiles whose sums were split, added in order, and the epilogue.
+template <typename T, Epilogue EPI>
+__global__ __launch_bounds__(kThreads) void k_ffn_join(const GemmArgs args) {
+  const int pitch = (args.N + 3) & ~3, quads = pitch / 4;
+  const int64_t all = int64_t(args.M) * quads;
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < all; i += int64_t(gridDim.x) * kThreads) {
+    const int64_t row = i / quads;
+    const int n = int(i - row * quads) * 4;
+    f32x4 sum = {};
+    for (int s = 0; s < args.splits; ++s)
+      sum += *(const CAME8_GLOBAL f32x4*)(gbl(args.part) + (int64_t(s) * args.M + row) * pitch + n);
+    const float x[4] = {sum[0], sum[1], sum[2], sum[3]};
+    if constexpr (EPI == kStore) {
+      store4<T>(static_cast<typename T::storage*>(args.out) + row * args.ldo, n, args.N, x);
+    } else {
+      float g[4], u[4];
+      load4(args.g + row * args.ldg, n, args.N, g);
+      load4(args.u + row * args.ldg, n, args.N, u);
+      store_back<T>(args, row, n, x, g, u);
+      // the padded end of the row, where it is more than a quad past N
+      const float none[4] = {};
+      if (n + 4 == pitch)
+        for (int p = pitch; p < int(args.ldo); p += 4) store_back<T>(args, row, p, none, none, none);
     }
   }
 }

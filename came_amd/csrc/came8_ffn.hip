@@ -3,7 +3,6 @@
 
 #include <algorithm>
 #include <exception>
-#include <limits>
 #include <type_traits>
 
 #include "../../include/came8.h"
@@ -19,7 +18,7 @@ int64_t up(int64_t n, int64_t a) { return (n + a - 1) / a * a; }
 // chunk (k_ffn_pack).  Every row there starts 16 bytes aligned and ends in zeros.
 struct Layout {
   int64_t ldh = 0;  // elements
-  size_t h = 0, dg = 0, du = 0, bytes = 0;
+  size_t h = 0, dg = 0, du = 0, part = 0, bytes = 0;
   struct Copy {
     int64_t ld = 0;  // 0: read where it is
     size_t at = 0;
@@ -29,6 +28,95 @@ struct Layout {
 bool ragged(const came8_ffn* f, int64_t cols, int64_t ld) {
   return f->dtype == CAME8_F32 ? cols % 4 != 0 : cols % 8 != 0 || ld % 2 != 0;
 }
+
+// How a product is cut: tiles of `tile` by `tile` (gate and up: half as many columns of h), `splits` workgroups a tile.
+struct Cut {
+  int tile = 0, splits = 1;
+};
+struct Size {
+  int64_t M, N, K;
+  int nseg;
+};
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// What a tile size runs at: workgroups at once on the GPU, and a step of k (128 bytes) of one, microseconds.
+struct Speed {
+  int tile, at_once;
+  double half, full;  // 16-bit types, fp32
+};
+constexpr Speed kSpeeds[] = {{256, 256, 1.87, 0.0}, {128, 512, 1.22, 3.8}, {64, 1024, 1.19, 1.9}};
+constexpr int kSplitSteps = 4;   // a share of a sum has at least these steps
+constexpr int kMaxSplits = 16;
+constexpr double kJoinBytes = 4e6;  // a microsecond of k_ffn_join: shares written and read
+
+int64_t steps_of(const came8_ffn* f, const Size& z) { return ceil_div(z.K, f->dtype == CAME8_F32 ? 32 : 64) * z.nseg; }
+
+// The cut with the least estimated time: rounds of workgroups by their steps, and three more for the first loads and the
+// epilogue, and what joining the shares moves.
+Cut cut_of(const came8_ffn* f, const Size& z, bool gate) {
+  Cut best;
+  double least = 1e300;
+  for (const Speed& v : kSpeeds) {
+    const double us = f->dtype == CAME8_F32 ? v.full : v.half;
+    if (us == 0.0) continue;
+    const int64_t tiles = ceil_div(z.M, v.tile) * ceil_div(z.N, gate ? v.tile / 2 : v.tile), steps = steps_of(f, z);
+    for (int s = 1; s <= (gate ? 1 : kMaxSplits); ++s) {
+      if (s > 1 && steps / s < kSplitSteps) break;
+      const double t = double(ceil_div(tiles * s, v.at_once)) * (double(ceil_div(steps, s)) + 3.0) * us +
+                       (s > 1 ? 4.0 + double(s) * double(z.M) * double(z.N) * 8.0 / kJoinBytes : 0.0);
+      if (t < least) {
+        least = t;
+        best.tile = v.tile;
+        best.splits = s;
+      }
+    }
+  }
+  return best;
+}
+
+// The cuts of several products in one launch: one tile size, the one whose tiles keep the GPU busy for the least time; a
+// product whose sums are longer than an even share of all work is split.
+void cut_together(const came8_ffn* f, const Size* z, int count, Cut* cuts) {
+  double least = 1e300;
+  for (const Speed& v : kSpeeds) {
+    const double us = f->dtype == CAME8_F32 ? v.full : v.half;
+    if (us == 0.0) continue;
+    double work = 0.0, join = 0.0;
+    int64_t longest = 0;
+    for (int i = 0; i < count; ++i)
+      work += double(ceil_div(z[i].M, v.tile) * ceil_div(z[i].N, v.tile)) * (double(steps_of(f, z[i])) + 3.0);
+    const int64_t share = std::max<int64_t>(2 * kSplitSteps, int64_t(work / v.at_once));
+    int splits[4];
+    for (int i = 0; i < count; ++i) {
+      const int64_t steps = steps_of(f, z[i]);
+      splits[i] = int(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, ceil_div(steps, share), steps / kSplitSteps})));
+      longest = std::max(longest, ceil_div(steps, splits[i]) + 3);
+      if (splits[i] > 1) join += 4.0 + double(splits[i]) * double(z[i].M) * double(z[i].N) * 8.0 / kJoinBytes;
+    }
+    const double t = (std::max(work / v.at_once, double(longest)) + 0.5 * double(longest)) * us + join;
+    if (t < least) {
+      least = t;
+      for (int i = 0; i < count; ++i) cuts[i].tile = v.tile, cuts[i].splits = splits[i];
+    }
+  }
+}
+
+struct Cuts {
+  Cut gate, down;          // forward
+  Cut back, grads[4];      // backward: dh; dx, dw_gate, dw_up, dw_down
+};
+Cuts cuts_of(const came8_ffn* f) {
+  Cuts c;
+  c.gate = cut_of(f, {f->tokens, f->hidden, f->dim, 1}, true);
+  c.down = cut_of(f, {f->tokens, f->out, f->hidden, 1}, false);
+  c.back = cut_of(f, {f->tokens, f->hidden, f->out, 1}, false);
+  const Size z[4] = {{f->tokens, f->dim, f->hidden, 2}, {f->hidden, f->dim, f->tokens, 1}, {f->hidden, f->dim, f->tokens, 1},
+                     {f->out, f->hidden, f->tokens, 1}};
+  cut_together(f, z, 4, c.grads);
+  return c;
+}
+
+int64_t part_floats(const Cut& c, int64_t M, int64_t N) { return c.splits > 1 ? c.splits * M * up(N, 4) : 0; }
 
 Layout layout_of(const came8_ffn* f, bool backward) {
   Layout l;
@@ -54,6 +142,15 @@ Layout layout_of(const came8_ffn* f, bool backward) {
   copy(l.gate, f->hidden, f->dim, f->ld_gate);
   copy(l.up, f->hidden, f->dim, f->ld_up);
   copy(l.down, f->out, f->hidden, f->ld_down);
+  // shares of split sums; dh's are joined before the others are written
+  const Cuts c = cuts_of(f);
+  int64_t part = part_floats(c.down, f->tokens, f->out);
+  if (backward)
+    part = std::max(part_floats(c.back, f->tokens, f->hidden),
+                    part_floats(c.grads[0], f->tokens, f->dim) + part_floats(c.grads[1], f->hidden, f->dim) +
+                        part_floats(c.grads[2], f->hidden, f->dim) + part_floats(c.grads[3], f->out, f->hidden));
+  l.part = l.bytes;
+  l.bytes += size_t(up(part * 4, 256));
   return l;
 }
 
@@ -95,29 +192,33 @@ int check_pointers(const char* what, std::initializer_list<const void*> ps) {
   return CAME8_OK;
 }
 
-template <typename T, int B, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
-bool launch_tiles(GemmArgs a, int64_t least, hipStream_t stream) {
-  constexpr int cols = EPI == kGate ? B / 2 : B;
-  a.tiles_m = (a.M + B - 1) / B;
-  a.tiles_n = (a.N + cols - 1) / cols;
-  const int64_t tiles = int64_t(a.tiles_m) * a.tiles_n;
-  if (tiles < least) return false;
-  hipLaunchKernelGGL((k_ffn_gemm<T, B, B, WAVES_N, AROWS, BROWS, EPI>), dim3(unsigned(tiles)), dim3(2 * WAVES_N * kWave), 0, stream, a);
-  return true;
+void tile(GemmArgs& a, const Cut& c, bool gate) {
+  const int cols = gate ? c.tile / 2 : c.tile;
+  a.tiles_m = int32_t(ceil_div(a.M, c.tile));
+  a.tiles_n = int32_t(ceil_div(a.N, cols));
+  a.splits = c.splits;
 }
 
-template <typename T, bool AROWS, bool BROWS, Epilogue EPI>
-void launch(const GemmArgs& a, hipStream_t stream) {
-#ifndef MIN256
-#define MIN256 200
-#endif
-#ifndef MIN128
-#define MIN128 200
-#endif
-  if constexpr (!std::is_same<T, F32>::value)
-    if (launch_tiles<T, 256, 4, AROWS, BROWS, EPI>(a, MIN256, stream)) return;
-  if (launch_tiles<T, 128, 2, AROWS, BROWS, EPI>(a, MIN128, stream)) return;
-  launch_tiles<T, 64, 2, AROWS, BROWS, EPI>(a, 0, stream);
+template <typename T, Epilogue EPI>
+void join(const GemmArgs& a, hipStream_t stream) {
+  if (a.splits == 1) return;
+  const int64_t quads = int64_t(a.M) * ((a.N + 3) / 4);
+  hipLaunchKernelGGL((k_ffn_join<T, EPI>), dim3(unsigned(std::min<int64_t>(ceil_div(quads, kThreads), 1 << 16))), dim3(kThreads), 0,
+                     stream, a);
+}
+
+// One product over its tiles.  256 by 256 only for 16-bit types: fp32 products are bound by the matrix units at any size.
+template <typename T, bool BROWS, Epilogue EPI>
+void launch(GemmArgs a, const Cut& c, float* part, hipStream_t stream) {
+  tile(a, c, EPI == kGate);
+  a.part = c.splits > 1 ? part : nullptr;
+  const dim3 grid(unsigned(a.tiles_m) * unsigned(a.tiles_n) * unsigned(a.splits));
+  if constexpr (!std::is_same<T, F32>::value) {
+    if (c.tile == 256) hipLaunchKernelGGL((k_ffn_gemm<T, 256, 4, true, BROWS, EPI>), grid, dim3(512), 0, stream, a);
+  }
+  if (c.tile == 128) hipLaunchKernelGGL((k_ffn_gemm<T, 128, 2, true, BROWS, EPI>), grid, dim3(256), 0, stream, a);
+  if (c.tile == 64) hipLaunchKernelGGL((k_ffn_gemm<T, 64, 2, true, BROWS, EPI>), grid, dim3(256), 0, stream, a);
+  if constexpr (EPI != kGate) join<T, EPI>(a, stream);
 }
 
 template <typename T>
@@ -132,13 +233,15 @@ void forward(const came8_ffn* f, const void* x, const void* wg, const void* wu, 
   a.b2 = operand<typename T::storage>(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream);
   a.out = ws + l.h, a.ldo = l.ldh;
   a.g = g, a.u = u, a.ldg = f->hidden;
-  launch<T, true, true, kGate>(a, stream);
+  const Cuts c = cuts_of(f);
+  float* part = reinterpret_cast<float*>(ws + l.part);
+  launch<T, true, kGate>(a, c.gate, part, stream);
   GemmArgs d{};
   d.nseg = 1;
   d.M = int32_t(f->tokens), d.N = int32_t(f->out), d.K = int32_t(f->hidden);
   d.seg[0] = {{ws + l.h, l.ldh}, operand<typename T::storage>(wd, f->out, f->hidden, f->ld_down, l.down, ws, stream)};
   d.out = y, d.ldo = f->out;
-  launch<T, true, true, kStore>(d, stream);
+  launch<T, true, kStore>(d, c.down, part, stream);
 }
 
 template <typename T>
@@ -153,35 +256,49 @@ void backward(const came8_ffn* f, const void* x, const void* wg, const void* wu,
   a.seg[0] = {pdy, operand<typename T::storage>(wd, f->out, f->hidden, f->ld_down, l.down, ws, stream)};
   a.out = ws + l.dg, a.out2 = ws + l.du, a.out3 = dwd ? ws + l.h : nullptr, a.ldo = l.ldh;
   a.g = const_cast<float*>(g), a.u = const_cast<float*>(u), a.ldg = f->hidden;
-  launch<T, true, false, kBack>(a, stream);
-  GemmArgs d{};
+  const Cuts c = cuts_of(f);
+  float* part = reinterpret_cast<float*>(ws + l.part);
+  launch<T, false, kBack>(a, c.back, part, stream);
+
+  GradArgs r{};
+  int32_t groups = 0, count = 0;
+  auto add = [&](GemmArgs& g, const Cut& cut, int64_t M, int64_t N, int64_t K, void* out) {
+    g.nseg = std::max(g.nseg, 1);
+    g.M = int32_t(M), g.N = int32_t(N), g.K = int32_t(K);
+    g.out = out, g.ldo = N;
+    tile(g, cut, false);
+    if (cut.splits > 1) {
+      g.part = part;
+      part += part_floats(cut, M, N);
+    }
+    groups += g.tiles_m * g.tiles_n * g.splits;
+  };
   if (dx) {
-    d.nseg = 2;
-    d.M = int32_t(f->tokens), d.N = int32_t(f->dim), d.K = int32_t(f->hidden);
-    d.seg[0] = {{ws + l.dg, l.ldh}, operand<typename T::storage>(wg, f->hidden, f->dim, f->ld_gate, l.gate, ws, stream)};
-    d.seg[1] = {{ws + l.du, l.ldh}, operand<typename T::storage>(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream)};
-    d.out = dx, d.ldo = f->dim;
-    launch<T, true, false, kStore>(d, stream);
+    r.dx.nseg = 2;
+    r.dx.seg[0] = {{ws + l.dg, l.ldh}, operand<typename T::storage>(wg, f->hidden, f->dim, f->ld_gate, l.gate, ws, stream)};
+    r.dx.seg[1] = {{ws + l.du, l.ldh}, operand<typename T::storage>(wu, f->hidden, f->dim, f->ld_up, l.up, ws, stream)};
+    add(r.dx, c.grads[0], f->tokens, f->dim, f->hidden, dx);
   }
-  d.nseg = 1;
-  d.K = int32_t(f->tokens);
-  d.M = int32_t(f->hidden), d.N = int32_t(f->dim), d.ldo = f->dim;
-  if (dwg) {
-    d.seg[0] = {{ws + l.dg, l.ldh}, px};
-    d.out = dwg;
-    launch<T, false, false, kStore>(d, stream);
+  auto add_dw = [&](const Cut& cut, int64_t M, int64_t N, void* out, const Operand& first, const Operand& second) {
+    if (out == nullptr) return;
+    r.first[count] = groups;
+    GemmArgs& g = r.dw[count++];
+    g.seg[0] = {first, second};
+    add(g, cut, M, N, f->tokens, out);
+  };
+  add_dw(c.grads[1], f->hidden, f->dim, dwg, {ws + l.dg, l.ldh}, px);
+  add_dw(c.grads[2], f->hidden, f->dim, dwu, {ws + l.du, l.ldh}, px);
+  add_dw(c.grads[3], f->out, f->hidden, dwd, pdy, {ws + l.h, l.ldh});
+  for (int k = count; k < 4; ++k) r.first[k] = groups;
+  if (groups == 0) return;
+  const int t = c.grads[0].tile;
+  if constexpr (!std::is_same<T, F32>::value) {
+    if (t == 256) hipLaunchKernelGGL((k_ffn_grads<T, 256, 4>), dim3(unsigned(groups)), dim3(512), 0, stream, r);
   }
-  if (dwu) {
-    d.seg[0] = {{ws + l.du, l.ldh}, px};
-    d.out = dwu;
-    launch<T, false, false, kStore>(d, stream);
-  }
-  if (dwd) {
-    d.M = int32_t(f->out), d.N = int32_t(f->hidden), d.ldo = f->hidden;
-    d.seg[0] = {pdy, {ws + l.h, l.ldh}};
-    d.out = dwd;
-    launch<T, false, false, kStore>(d, stream);
-  }
+  if (t == 128) hipLaunchKernelGGL((k_ffn_grads<T, 128, 2>), dim3(unsigned(groups)), dim3(256), 0, stream, r);
+  if (t == 64) hipLaunchKernelGGL((k_ffn_grads<T, 64, 2>), dim3(unsigned(groups)), dim3(256), 0, stream, r);
+  if (dx) join<T, kStore>(r.dx, stream);
+  for (int k = 0; k < count; ++k) join<T, kStore>(r.dw[k], stream);
 }
 
 }  // namespace
