@@ -123,9 +123,12 @@ struct View {
 constexpr int kChunkBytes = 16;
 constexpr int kRowBytes = 128;  // of a tile in LDS: 8 chunks, 64 (fp32: 32) values of k
 
-// Chunk c of row r lies at place c ^ swz(r) of its row: eight lanes that read one chunk of eight consecutive rows, or write
-// one chunk of rows 8 apart (columns on their way in), touch eight different places, which is all banks once.
-__device__ __forceinline__ int swz(int r) { return (r ^ (r >> 3)) & 7; }
+// Chunk c of row r lies at place c ^ swz(r) of its row.  A 16-byte read takes 16 lanes at a time, and not in order: lanes 0-3,
+// 12-15, 20-23 and 24-27 go together (and 4-11, 16-19, 28-31).  With a fragment's lanes, row l % 16 and chunk l / 16, these
+// are 16 different places of two rows' length, all 64 banks once; eight lanes that write a chunk of rows 8 apart (columns on
+// their way in) touch eight places.  (With places that only 8 lanes in order tell apart, every read took twice its time.)
+// swz is linear: of rows whose bits do not overlap it is the exclusive or.
+__host__ __device__ constexpr int swz(int r) { return (r >> 3 & 1) | ((r ^ r >> 4) & 2) | ((r ^ r >> 1 ^ r >> 2) & 4); }
 
 // ------------------------------------------------------------------------------------------------ operands' way in
 // R rows by 8 chunks of k, NT threads: 16-byte loads into registers (fetch), later written to LDS (put).
@@ -171,12 +174,12 @@ struct Stage {
     const int t = int(threadIdx.x);
     if constexpr (ROWS) {
       constexpr int H = HALF == 0 ? kStep : HALF;
-      // the first load's row; load i's is `row` further, which changes the row's swz by an exclusive or
+      // the first load's row; load i's is `row` further
       const int c = t & 7, r = HALF == 0 ? t >> 3 : (t >> 3) / H * 2 * H + (t >> 3) % H;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = HALF == 0 ? i * kStep : i / 2 * 2 * kStep + (i & 1) * HALF;
-        *reinterpret_cast<u32x4*>(lds + (r * kRowBytes + ((c ^ swz(r)) ^ (row >> 3 & 7)) * kChunkBytes) + row * kRowBytes) = v[i];
+        *reinterpret_cast<u32x4*>(lds + (r * kRowBytes + ((c ^ swz(r)) ^ swz(row)) * kChunkBytes) + row * kRowBytes) = v[i];
       }
     } else if constexpr (kElem == 4) {
       const int r = (t % (R / kVec)) * kVec, k = (t / (R / kVec)) * kLoads;  // first row, first k
@@ -363,7 +366,7 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     sb.put(to + BM * kRowBytes);
   };
   // Fragment i of half s: row 16 i + lane % 16 of the wavefront's, chunk 4 s + lane / 16, at place
-  // (lane / 16) ^ swz(the wavefront's first row + lane % 16) ^ 4 s ^ 2 (i & 3).
+  // (lane / 16) ^ swz(the wavefront's first row + lane % 16) ^ 4 s ^ swz(16 i), one of four that differ by 2 v.
   const int fr = lane % 16;
   uint32_t pa[4], pb[4];
 #pragma unroll
@@ -376,13 +379,13 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     const char* a = lds + (t & 1) * kTileBytes;
 #pragma unroll
     for (int i = 0; i < FM / 2; ++i)
-      f[i] = *reinterpret_cast<const u32x4*>(a + pa[(2 * s) ^ ((i0 + i) & 3)] + (i0 + i) * 16 * kRowBytes);
+      f[i] = *reinterpret_cast<const u32x4*>(a + pa[(4 * s ^ swz(16 * (i0 + i))) / 2] + (i0 + i) * 16 * kRowBytes);
   };
   auto read_b = [&](int t, int s, int j0) __attribute__((always_inline)) {
     const char* b = lds + (t & 1) * kTileBytes;
 #pragma unroll
     for (int j = j0; j < j0 + FN / 2; ++j)
-      fb[s][j] = *reinterpret_cast<const u32x4*>(b + pb[(2 * s) ^ (j & 3)] + j * 16 * kRowBytes);
+      fb[s][j] = *reinterpret_cast<const u32x4*>(b + pb[(4 * s ^ swz(16 * j)) / 2] + j * 16 * kRowBytes);
   };
 
   f32x4 acc[FM][FN] = {};
@@ -393,6 +396,9 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
       for (int j = 0; j < FN; ++j) acc[i0 + i][j] = mfma_chunk<T>(fb[s][j], f[i], acc[i0 + i][j]);
   };
   constexpr int kProducts = FM / 2 * FN * (kElem == 4 ? 4 : 1);  // of a phase
+  // Step t + 2 is loaded as soon as step t + 1 has left the registers, a whole step before its use (8192 tokens forward and
+  // backward 6555 us with loads half a step ahead, 6452 so); with columns, whose way to LDS takes registers, a quarter later.
+  constexpr bool kEarly = AROWS && BROWS;
   fetch();
   put(0);
   fetch();
@@ -408,19 +414,20 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     interleave<kDsRead, FM / 2 + FN, kProducts>();
     read_a(lo, t, 1, 0);
     put(t + 1);
+    if constexpr (kEarly) fetch();
     multiply(hi, 0, FM / 2);
-    interleave<kDsRead | kDsWrite, FM / 2 + FM + FN, kProducts>();
+    interleave<kDsRead | kDsWrite | kVmemRead, FM / 2 + FM + FN + (kEarly ? 8 : 0), kProducts>();
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
     read_a(hi, t, 1, FM / 2);
     read_b(t + 1, 0, 0);
     read_b(t + 1, 0, FN / 2);
+    if constexpr (!kEarly) fetch();
     multiply(lo, 1, 0);
-    interleave<kDsRead, FM / 2 + FN, kProducts>();
-    fetch();
+    interleave<kDsRead | kVmemRead, FM / 2 + FN + (kEarly ? 0 : 8), kProducts>();
     read_a(lo, t + 1, 0, 0);
     multiply(hi, 1, FM / 2);
-    interleave<kDsRead | kVmemRead, FM / 2 + FM + FN, kProducts>();
+    interleave<kDsRead, FM / 2, kProducts>();
   }
 
   // acc[i][j][e]: row 16 i + lane % 16 of the wavefront's, column 16 j + 4 (lane / 16) + e.  Up to 64 rows at a time go
@@ -435,6 +442,7 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   constexpr int kBatch = kRounds < 4 ? kRounds : 4;
   const int cc = lane % kLanes, r0 = lane / kLanes, n = n0 + wn * kCols + cc * 4;
   auto slot = [&](int r, int c) { return reinterpret_cast<f32x4*>(mine + r * (WN * 4) + ((c ^ r) & (kChunks - 1)) * 16); };
+  float gn[kBatch][4] = {}, un[kBatch][4] = {};  // of the next rounds
   __syncthreads();
 #pragma unroll
   for (int part = 0; part < FM / kPart; ++part) {
@@ -442,17 +450,31 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     for (int i = 0; i < kPart; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) *slot(i * 16 + lane % 16, j * 4 + lane / 16) = acc[part * kPart + i][j];
+    const int m1 = m0 + wm * WM + part * kPart * 16 + r0;
+    auto load = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int m = m1 + (q + k) * kRows;
+        if (m < args.M) {
+          load4(args.g + int64_t(m) * args.ldg, n, args.N, gn[k]);
+          load4(args.u + int64_t(m) * args.ldg, n, args.N, un[k]);
+        }
+      }
+    };
+    if (EPI == kBack && args.part == nullptr) load(0);
 #pragma unroll 1
     for (int q = 0; q < kRounds; q += kBatch) {
-      const int m = m0 + wm * WM + part * kPart * 16 + q * kRows + r0;
+      const int m = m1 + q * kRows;
       float g[kBatch][4], u[kBatch][4];
       if (EPI == kBack && args.part == nullptr) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
-          if (m + k * kRows < args.M) {
-            load4(args.g + int64_t(m + k * kRows) * args.ldg, n, args.N, g[k]);
-            load4(args.u + int64_t(m + k * kRows) * args.ldg, n, args.N, u[k]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            g[k][e] = gn[k][e];
+            u[k][e] = un[k][e];
           }
+        if (q + kBatch < kRounds) load(q + kBatch);
       }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
