@@ -282,10 +282,10 @@ __device__ __forceinline__ void interleave() {
 // kGate: the tile's BN rows of weights are, in turns of half a wavefront's, gate and up projection, so that a wavefront
 // holds both values of its columns of h.
 //
-// Step t of k: half of its fragments are multiplied while the other half is read from LDS and the operands of step t + 1 go
-// from registers to the other LDS buffer; after the step's one barrier the second half is multiplied while step t + 1's first
-// fragments are read and the operands of step t + 2 are loaded.  So neither LDS reads nor global loads are waited for at the
-// barrier.  Steps past the end load zeros.
+// Step t of k is four phases, each of a quarter of its products, with the LDS reads of the next phase among them; in the second
+// the operands of step t + 1 go from registers to the other LDS buffer, and those of step t + 2 are loaded.  The step's one
+// barrier stands before the last phase, whose reads are the first of step t + 1.  So neither LDS reads nor global loads are
+// waited for at the barrier.  Steps past the end load zeros.
 template <typename T, int BM, int BN, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
 __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) {
   using S = typename T::storage;
@@ -417,17 +417,18 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     if constexpr (kEarly) fetch();
     multiply(hi, 0, FM / 2);
     interleave<kDsRead | kDsWrite | kVmemRead, FM / 2 + FM + FN + (kEarly ? 8 : 0), kProducts>();
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
     read_a(hi, t, 1, FM / 2);
-    read_b(t + 1, 0, 0);
-    read_b(t + 1, 0, FN / 2);
     if constexpr (!kEarly) fetch();
     multiply(lo, 1, 0);
-    interleave<kDsRead | kVmemRead, FM / 2 + FN + (kEarly ? 0 : 8), kProducts>();
+    interleave<kDsRead | kVmemRead, FM / 2 + (kEarly ? 0 : 8), kProducts>();
+    // every wavefront has read its last of step t, whose place the next put takes, and written its part of step t + 1
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
     read_a(lo, t + 1, 0, 0);
+    read_b(t + 1, 0, 0);
+    read_b(t + 1, 0, FN / 2);
     multiply(hi, 1, FM / 2);
-    interleave<kDsRead, FM / 2, kProducts>();
+    interleave<kDsRead, FM / 2 + FN, kProducts>();
   }
 
   // acc[i][j][e]: row 16 i + lane % 16 of the wavefront's, column 16 j + 4 (lane / 16) + e.  Up to 64 rows at a time go
@@ -560,6 +561,131 @@ __global__ __launch_bounds__(kThreads) void k_ffn_join(const GemmArgs args) {
       if (n + 4 == pitch)
         for (int p = pitch; p < int(args.ldo); p += 4) store_back<T>(args, row, p, none, none, none);
     }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- few rows of x
+// Up to 64 rows: the weights are read once and are all there is to wait for, so no tile goes through LDS.  A workgroup has
+// 16 rows of the weights (kGate: of both) and all rows of x; its NW wavefronts take steps of 128 bytes of k in turn, a lane
+// two chunks of a row at once, whole lines of a row by four lanes, four steps in flight; their sums are added in order in
+// LDS.  Rows may start at any element.
+struct FewArgs {
+  const void* x;
+  int64_t ldx;
+  const void* w[2];  // kGate: gate and up
+  int64_t ldw[2];
+  int32_t M, N, K, act;
+  void* out;
+  int64_t ldo;
+  float* g;
+  float* u;
+  int64_t ldg;
+};
+
+// a chunk at any address its type allows
+typedef uint32_t u32x4w __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T>
+using AnyChunk = typename std::conditional<sizeof(typename T::storage) == 4, u32x4w, u32x4u>::type;
+
+// chunk at k of a row of K elements, what is past K as zeros
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const CAME8_GLOBAL typename T::storage* row, int k, int K) {
+  using S = typename T::storage;
+  constexpr int V = kChunkBytes / int(sizeof(S));
+  using raw = AnyChunk<T>;
+  if (k + V <= K) return *(const CAME8_GLOBAL raw*)(row + k);
+  u32x4 v = {};
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (k + e < K) {
+      if constexpr (sizeof(S) == 4) v[e] = __float_as_uint(row[k + e]);
+      else v[e / 2] |= uint32_t(row[k + e]) << (16 * (e & 1));
+    }
+  return v;
+}
+
+template <typename T, int MT, int NW, bool GATE>
+__global__ __launch_bounds__(NW * kWave) void k_ffn_few(const FewArgs args) {
+  using S = typename T::storage;
+  using raw = AnyChunk<T>;
+  constexpr int V = kChunkBytes / int(sizeof(S)), BK = kRowBytes / int(sizeof(S)), G = GATE ? 2 : 1;
+  constexpr int U = MT == 4 ? 2 : 4;  // steps in flight
+  __shared__ f32x4 sums[NW][G * MT][kWave];
+  const int lane = int(threadIdx.x) % kWave, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int n0 = int(blockIdx.x) * 16, q = lane / 16 * 2 * V;
+  const CAME8_GLOBAL S *w[G], *x[MT];
+#pragma unroll
+  for (int i = 0; i < G; ++i)  // rows past the end are not stored: any row will do
+    w[i] = gbl(static_cast<const S*>(args.w[i])) + int64_t(min(n0 + lane % 16, args.N - 1)) * args.ldw[i] + q;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+    x[i] = gbl(static_cast<const S*>(args.x)) + int64_t(min(i * 16 + lane % 16, args.M - 1)) * args.ldx + q;
+
+  f32x4 acc[G][MT] = {};
+  const int full = args.K / BK;
+  for (int s0 = wave; s0 < full; s0 += NW * U) {
+    u32x4 wv[U][G][2], xv[U][MT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * NW < full) {
+        const int64_t k = int64_t(s0 + u * NW) * BK;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int i = 0; i < G; ++i) wv[u][i][c] = __builtin_nontemporal_load((const CAME8_GLOBAL raw*)(w[i] + k + c * V));
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xv[u][i][c] = *(const CAME8_GLOBAL raw*)(x[i] + k + c * V);
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u * NW < full)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[g][i] = mfma_chunk<T>(wv[u][g][c], xv[u][i][c], acc[g][i]);
+  }
+  if (full * BK < args.K && full % NW == wave) {
+    const int k = full * BK, left = args.K - q;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const u32x4 xv = load_chunk<T>(x[i], k + c * V, left);
+#pragma unroll
+        for (int g = 0; g < G; ++g) acc[g][i] = mfma_chunk<T>(load_chunk<T>(w[g], k + c * V, left), xv, acc[g][i]);
+      }
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[wave][g * MT + i][lane] = acc[g][i];
+  __syncthreads();
+  if (wave >= MT) return;
+  const int m = wave * 16 + lane % 16, n = n0 + lane / 16 * 4;
+  f32x4 total[G] = {};
+#pragma unroll
+  for (int i = 0; i < NW; ++i)
+#pragma unroll
+    for (int g = 0; g < G; ++g) total[g] += sums[i][g * MT + wave][lane];
+  if (m >= args.M) return;
+  S* out = static_cast<S*>(args.out) + int64_t(m) * args.ldo;
+  const float a[4] = {total[0][0], total[0][1], total[0][2], total[0][3]};
+  if constexpr (GATE) {
+    const float b[4] = {total[1][0], total[1][1], total[1][2], total[1][3]};
+    float h[4], none[4];
+    activate<false>(a, args.act, h, none);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] *= b[e];
+    store4<T>(out, n, args.N, h);
+    if (args.g) {
+      store4<F32>(args.g + int64_t(m) * args.ldg, n, args.N, a);
+      store4<F32>(args.u + int64_t(m) * args.ldg, n, args.N, b);
+    }
+  } else {
+    store4<T>(out, n, args.N, a);
   }
 }
 

@@ -101,6 +101,12 @@ void cut_together(const came8_ffn* f, const Size* z, int count, Cut* cuts) {
   }
 }
 
+// Rows of x up to which the forward products read the weights straight into registers (k_ffn_few).
+#ifndef FEW
+#define FEW 64
+#endif
+constexpr int64_t kFewTokens = FEW;
+
 struct Cuts {
   Cut gate, down;          // forward
   Cut back, grads[4];      // backward: dh; dx, dw_gate, dw_up, dw_down
@@ -138,6 +144,7 @@ Layout layout_of(const came8_ffn* f, bool backward) {
     l.du = take(f->tokens, l.ldh);
     copy(l.dy, f->tokens, f->out, f->out);
   }
+  if (!backward && f->tokens <= kFewTokens) return l;
   copy(l.x, f->tokens, f->dim, f->ld_x);
   copy(l.gate, f->hidden, f->dim, f->ld_gate);
   copy(l.up, f->hidden, f->dim, f->ld_up);
@@ -221,9 +228,33 @@ void launch(GemmArgs a, const Cut& c, float* part, hipStream_t stream) {
   if constexpr (EPI != kGate) join<T, EPI>(a, stream);
 }
 
+template <typename T, bool GATE>
+void launch_few(const FewArgs& a, hipStream_t stream) {
+  const unsigned groups = unsigned(ceil_div(a.N, 16));
+  if (a.M <= 16) hipLaunchKernelGGL((k_ffn_few<T, 1, 8, GATE>), dim3(groups), dim3(512), 0, stream, a);
+  else if (a.M <= 32) hipLaunchKernelGGL((k_ffn_few<T, 2, 8, GATE>), dim3(groups), dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL((k_ffn_few<T, 4, 8, GATE>), dim3(groups), dim3(512), 0, stream, a);
+}
+
 template <typename T>
 void forward(const came8_ffn* f, const void* x, const void* wg, const void* wu, const void* wd, void* y, float* g, float* u,
              const Layout& l, char* ws, hipStream_t stream) {
+  if (f->tokens <= kFewTokens) {
+    FewArgs a{};
+    a.x = x, a.ldx = f->ld_x;
+    a.w[0] = wg, a.w[1] = wu, a.ldw[0] = f->ld_gate, a.ldw[1] = f->ld_up;
+    a.M = int32_t(f->tokens), a.N = int32_t(f->hidden), a.K = int32_t(f->dim), a.act = f->activation;
+    a.out = ws + l.h, a.ldo = l.ldh;
+    a.g = g, a.u = u, a.ldg = f->hidden;
+    launch_few<T, true>(a, stream);
+    FewArgs d{};
+    d.x = ws + l.h, d.ldx = l.ldh;
+    d.w[0] = wd, d.ldw[0] = f->ld_down;
+    d.M = int32_t(f->tokens), d.N = int32_t(f->out), d.K = int32_t(f->hidden);
+    d.out = y, d.ldo = f->out;
+    launch_few<T, false>(d, stream);
+    return;
+  }
   GemmArgs a{};
   a.nseg = 1;
   a.act = f->activation;

@@ -178,6 +178,22 @@ def test_the_same_inputs_give_the_same_bits(T):
         assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(1030, 512, 1376, 512), (2048, 1024, 2752, 1024)], ids=lambda s: "x".join(map(str, s)))
+def test_many_steps_give_the_same_bits(shape, dtype):
+    """Wavefronts that run apart over many steps of a tile: results and gradients repeat bit for bit."""
+    from came_amd import gated_ffn
+    ops, dy = _operands(*shape, dtype, seed=10)
+    first = None
+    for _ in range(12):
+        leaves = [t.clone().requires_grad_() for t in ops]
+        y = gated_ffn(*leaves)
+        y.backward(dy)
+        got = [y.detach(), *(t.grad for t in leaves)]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
 def test_hidden_values_past_2_31():
     """More than 2^31 hidden values: the last tokens' rows and gradients (all others are zero)."""
     from came_amd import gated_ffn
