@@ -88,8 +88,9 @@ struct GemmArgs {
   int32_t nseg;
   int32_t M, N, K;  // K: of each segment
   int32_t tiles_m, tiles_n;
-  int32_t splits;   // workgroups that share a tile's sum (kStore, kBack)
-  float* part;      // splits > 1: their sums, [splits][M][N up to a multiple of 4], for k_ffn_join; else null
+  int32_t splits;   // workgroups that share a tile's sum
+  float* part;      // splits > 1: their sums, [splits][M][N up to a multiple of 4] (kGate: gate and up after each other in
+                    // a row), for k_ffn_join; else null
   int32_t act;
   void* out;        // kStore: C; kGate: h; kBack: dg
   int64_t ldo;
@@ -263,6 +264,20 @@ __device__ __forceinline__ void store_back(const GemmArgs& args, int64_t row, in
   if (args.out3) store4<T>(static_cast<S*>(args.out3) + row * args.ldo, n, ld, h);
 }
 
+// h of four values of g and u (zeros past N, where rows are padded), and g and u where they are kept
+template <typename T>
+__device__ __forceinline__ void store_gate(const GemmArgs& args, int64_t row, int n, const float (&g)[4], const float (&u)[4]) {
+  float h[4], none[4];
+  activate<false>(g, args.act, h, none);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] = n + e < args.N ? h[e] * u[e] : 0.0f;
+  store4<T>(static_cast<typename T::storage*>(args.out) + row * args.ldo, n, int(args.ldo), h);
+  if (args.g) {
+    store4<F32>(args.g + row * args.ldg, n, args.N, g);
+    store4<F32>(args.u + row * args.ldg, n, args.N, u);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------ product
 // Asks the scheduler to spread `count` instructions of the given kinds evenly among `products` matrix instructions, and to
 // move nothing past the end of the phase.
@@ -313,8 +328,11 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
   const int wm = wave & 1, wn = wave >> 1;
 
-  Stage<T, BM, NT, AROWS> sa;
-  Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0> sb;
+  // Steps loaded ahead; step t is in registers t % D.  Two where registers allow: 1021 tokens of 1024 and 2731 in fp32, tiles
+  // of 64 and 128, 516 us with one and 492 with two, 32 tokens of 4096 and 11008 in bf16 80 and 75 us.
+  constexpr int D = BM < 256 ? 2 : 1;
+  Stage<T, BM, NT, AROWS> sa[D];
+  Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0> sb[D];
   const int steps = (args.K + BK - 1) / BK;
   const int every = steps * args.nseg;
   int ahead = int(int64_t(every) * split / args.splits);  // the step that is fetched next
@@ -339,9 +357,10 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   int left = args.K - (ahead % steps) * BK;  // K less the next step's first k
   va.next(ahead % steps);
   vb.next(ahead % steps);
-  auto fetch = [&]() __attribute__((always_inline)) {
-    sa.fetch(va, va, left);
-    sb.fetch(vb, vb1, left);
+  if (EPI == kGate) vb1.next(ahead);
+  auto fetch = [&](int slot) __attribute__((always_inline)) {
+    sa[slot].fetch(va, va, left);
+    sb[slot].fetch(vb, vb1, left);
     va.next();
     vb.next();
     left -= BK;
@@ -360,10 +379,10 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
       left = turn ? args.K : left;
     }
   };
-  auto put = [&](int t) {
+  auto put = [&](int t, int slot) __attribute__((always_inline)) {
     char* to = lds + (t & 1) * kTileBytes;
-    sa.put(to);
-    sb.put(to + BM * kRowBytes);
+    sa[slot].put(to);
+    sb[slot].put(to + BM * kRowBytes);
   };
   // Fragment i of half s: row 16 i + lane % 16 of the wavefront's, chunk 4 s + lane / 16, at place
   // (lane / 16) ^ swz(the wavefront's first row + lane % 16) ^ 4 s ^ swz(16 i), one of four that differ by 2 v.
@@ -399,26 +418,27 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   // Step t + 2 is loaded as soon as step t + 1 has left the registers, a whole step before its use (8192 tokens forward and
   // backward 6555 us with loads half a step ahead, 6452 so); with columns, whose way to LDS takes registers, a quarter later.
   constexpr bool kEarly = AROWS && BROWS;
-  fetch();
-  put(0);
-  fetch();
+  fetch(0);
+  put(0, 0);
+#pragma unroll
+  for (int d = 1; d <= D; ++d) fetch(d % D);
   __syncthreads();
   read_a(lo, 0, 0, 0);
   read_b(0, 0, 0);
   read_b(0, 0, FN / 2);
-  for (int t = 0; t < total; ++t) {
+  auto step = [&](int t, int slot) __attribute__((always_inline)) {  // slot: of step t + 1
     read_a(hi, t, 0, FM / 2);
     read_b(t, 1, 0);
     read_b(t, 1, FN / 2);
     multiply(lo, 0, 0);
     interleave<kDsRead, FM / 2 + FN, kProducts>();
     read_a(lo, t, 1, 0);
-    put(t + 1);
-    if constexpr (kEarly) fetch();
+    put(t + 1, slot);
+    if constexpr (kEarly) fetch(slot);
     multiply(hi, 0, FM / 2);
     interleave<kDsRead | kDsWrite | kVmemRead, FM / 2 + FM + FN + (kEarly ? 8 : 0), kProducts>();
     read_a(hi, t, 1, FM / 2);
-    if constexpr (!kEarly) fetch();
+    if constexpr (!kEarly) fetch(slot);
     multiply(lo, 1, 0);
     interleave<kDsRead | kVmemRead, FM / 2 + (kEarly ? 0 : 8), kProducts>();
     // every wavefront has read its last of step t, whose place the next put takes, and written its part of step t + 1
@@ -429,7 +449,11 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     read_b(t + 1, 0, FN / 2);
     multiply(hi, 1, FM / 2);
     interleave<kDsRead, FM / 2 + FN, kProducts>();
-  }
+  };
+  for (int t = 0; t < total; t += D)
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (d == 0 || t + d < total) step(t + d, (d + 1) % D);
 
   // acc[i][j][e]: row 16 i + lane % 16 of the wavefront's, column 16 j + 4 (lane / 16) + e.  Up to 64 rows at a time go
   // through the wavefront's own part of LDS, so that lanes of successive columns read and write memory together; chunk c of
@@ -483,27 +507,22 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
         if (m + k * kRows >= args.M) continue;
         const int64_t row = m + k * kRows;
         const f32x4 c = *slot(r, cc);
-        if constexpr (EPI != kGate) {
-          if (args.part) {
-            const int pitch = (args.N + 3) & ~3;
-            store4<F32>(args.part + (int64_t(split) * args.M + row) * pitch, n, pitch, {c[0], c[1], c[2], c[3]});
-            continue;
+        if (args.part) {
+          const int pitch = (args.N + 3) & ~3;
+          float* to = args.part + (int64_t(split) * args.M + row) * pitch * (EPI == kGate ? 2 : 1);
+          store4<F32>(to, n, pitch, {c[0], c[1], c[2], c[3]});
+          if constexpr (EPI == kGate) {
+            const f32x4 d = *slot(r, cc + kChunks / 2);
+            store4<F32>(to + pitch, n, pitch, {d[0], d[1], d[2], d[3]});
           }
+          continue;
         }
         S* out = static_cast<S*>(args.out) + row * args.ldo;
         if constexpr (EPI == kStore) {
           store4<T>(out, n, args.N, {c[0], c[1], c[2], c[3]});
         } else if constexpr (EPI == kGate) {
           const f32x4 d = *slot(r, cc + kChunks / 2);
-          float h[4], none[4];
-          activate<false>({c[0], c[1], c[2], c[3]}, args.act, h, none);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) h[e] *= d[e];
-          store4<T>(out, n, int(args.ldo), h);  // zeros up to the padded end
-          if (args.g) {
-            store4<F32>(args.g + row * args.ldg, n, args.N, {c[0], c[1], c[2], c[3]});
-            store4<F32>(args.u + row * args.ldg, n, args.N, {d[0], d[1], d[2], d[3]});
-          }
+          store_gate<T>(args, row, n, {c[0], c[1], c[2], c[3]}, {d[0], d[1], d[2], d[3]});
         } else {
           store_back<T>(args, row, n, {c[0], c[1], c[2], c[3]}, g[k], u[k]);
         }
@@ -539,36 +558,57 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_grads(const Grad
 
 // The shares of tiles whose sums were split, added in order, and the epilogue.
 template <typename T, Epilogue EPI>
-__global__ __launch_bounds__(kThreads) void k_ffn_join(const GemmArgs args) {
+__device__ __forceinline__ void join(const GemmArgs& args) {
   const int pitch = (args.N + 3) & ~3, quads = pitch / 4;
-  const int64_t all = int64_t(args.M) * quads;
+  const int64_t width = int64_t(pitch) * (EPI == kGate ? 2 : 1), all = int64_t(args.M) * quads;
   for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < all; i += int64_t(gridDim.x) * kThreads) {
     const int64_t row = i / quads;
     const int n = int(i - row * quads) * 4;
-    f32x4 sum = {};
-    for (int s = 0; s < args.splits; ++s)
-      sum += *(const CAME8_GLOBAL f32x4*)(gbl(args.part) + (int64_t(s) * args.M + row) * pitch + n);
+    const CAME8_GLOBAL float* part = gbl(args.part) + row * width + n;
+    f32x4 sum = {}, sum1 = {};
+#pragma unroll 4
+    for (int s = 0; s < args.splits; ++s, part += args.M * width) {
+      sum += *(const CAME8_GLOBAL f32x4*)part;
+      if (EPI == kGate) sum1 += *(const CAME8_GLOBAL f32x4*)(part + pitch);
+    }
     const float x[4] = {sum[0], sum[1], sum[2], sum[3]};
+    const float none[4] = {};
+    // and the padded end of the row, where it is more than a quad past N
+    const int end = n + 4 == pitch ? int(args.ldo) : 0;
     if constexpr (EPI == kStore) {
       store4<T>(static_cast<typename T::storage*>(args.out) + row * args.ldo, n, args.N, x);
+    } else if constexpr (EPI == kGate) {
+      store_gate<T>(args, row, n, x, {sum1[0], sum1[1], sum1[2], sum1[3]});
+      for (int p = pitch; p < end; p += 4) store4<T>(static_cast<typename T::storage*>(args.out) + row * args.ldo, p, end, none);
     } else {
       float g[4], u[4];
       load4(args.g + row * args.ldg, n, args.N, g);
       load4(args.u + row * args.ldg, n, args.N, u);
       store_back<T>(args, row, n, x, g, u);
-      // the padded end of the row, where it is more than a quad past N
-      const float none[4] = {};
-      if (n + 4 == pitch)
-        for (int p = pitch; p < int(args.ldo); p += 4) store_back<T>(args, row, p, none, none, none);
+      for (int p = pitch; p < end; p += 4) store_back<T>(args, row, p, none, none, none);
     }
   }
 }
 
+template <typename T, Epilogue EPI>
+__global__ __launch_bounds__(kThreads) void k_ffn_join(const GemmArgs args) {
+  join<T, EPI>(args);
+}
+
+// Of dx and the weights' gradients, those that were split: blockIdx.y says which.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_ffn_join_grads(const GradArgs args) {
+  const GemmArgs& g = blockIdx.y == 0 ? args.dx : args.dw[blockIdx.y - 1];
+  if (g.part) join<T, kStore>(g);
+}
+
 // ------------------------------------------------------------------------------------------------- few rows of x
-// Up to 64 rows: the weights are read once and are all there is to wait for, so no tile goes through LDS.  A workgroup has
-// 16 rows of the weights (kGate: of both) and all rows of x; its NW wavefronts take steps of 128 bytes of k in turn, a lane
+// Up to 16 rows: the weights are read once and are all there is to wait for, so no tile goes through LDS.  A workgroup has
+// 16 rows of the weights (kGate: of both) and all rows of x; its 8 wavefronts take steps of 128 bytes of k in turn, a lane
 // two chunks of a row at once, whole lines of a row by four lanes, four steps in flight; their sums are added in order in
-// LDS.  Rows may start at any element.
+// LDS.  Rows may start at any element.  One token of 4096 and 11008 in bf16: 36.8 us for 180 MB of gate and up, 21.7 for the
+// 90 MB of down (4.9 and 4.2 TB/s), 58 together, 75 in tiles; 2 or 8 steps in flight and 16 wavefronts changed nothing.  With
+// 32 rows it took 89 us, tiles 75: x then costs more loads than the weights.
 struct FewArgs {
   const void* x;
   int64_t ldx;
@@ -581,6 +621,7 @@ struct FewArgs {
   float* u;
   int64_t ldg;
 };
+constexpr int kFewRows = 16;
 
 // a chunk at any address its type allows
 typedef uint32_t u32x4w __attribute__((ext_vector_type(4), aligned(4)));
@@ -592,8 +633,7 @@ template <typename T>
 __device__ __forceinline__ u32x4 load_chunk(const CAME8_GLOBAL typename T::storage* row, int k, int K) {
   using S = typename T::storage;
   constexpr int V = kChunkBytes / int(sizeof(S));
-  using raw = AnyChunk<T>;
-  if (k + V <= K) return *(const CAME8_GLOBAL raw*)(row + k);
+  if (k + V <= K) return *(const CAME8_GLOBAL AnyChunk<T>*)(row + k);
   u32x4 v = {};
 #pragma unroll
   for (int e = 0; e < V; ++e)
@@ -604,27 +644,25 @@ __device__ __forceinline__ u32x4 load_chunk(const CAME8_GLOBAL typename T::stora
   return v;
 }
 
-template <typename T, int MT, int NW, bool GATE>
-__global__ __launch_bounds__(NW * kWave) void k_ffn_few(const FewArgs args) {
+template <typename T, bool GATE>
+__global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
   using S = typename T::storage;
   using raw = AnyChunk<T>;
-  constexpr int V = kChunkBytes / int(sizeof(S)), BK = kRowBytes / int(sizeof(S)), G = GATE ? 2 : 1;
-  constexpr int U = MT == 4 ? 2 : 4;  // steps in flight
-  __shared__ f32x4 sums[NW][G * MT][kWave];
+  constexpr int V = kChunkBytes / int(sizeof(S)), BK = kRowBytes / int(sizeof(S)), G = GATE ? 2 : 1, NW = 8;
+  constexpr int U = 4;  // steps in flight
+  __shared__ f32x4 sums[NW][G][kWave];
   const int lane = int(threadIdx.x) % kWave, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int n0 = int(blockIdx.x) * 16, q = lane / 16 * 2 * V;
-  const CAME8_GLOBAL S *w[G], *x[MT];
+  const CAME8_GLOBAL S* w[G];  // rows past the end are not stored: any row will do
 #pragma unroll
-  for (int i = 0; i < G; ++i)  // rows past the end are not stored: any row will do
+  for (int i = 0; i < G; ++i)
     w[i] = gbl(static_cast<const S*>(args.w[i])) + int64_t(min(n0 + lane % 16, args.N - 1)) * args.ldw[i] + q;
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-    x[i] = gbl(static_cast<const S*>(args.x)) + int64_t(min(i * 16 + lane % 16, args.M - 1)) * args.ldx + q;
+  const CAME8_GLOBAL S* x = gbl(static_cast<const S*>(args.x)) + int64_t(min(lane % 16, args.M - 1)) * args.ldx + q;
 
-  f32x4 acc[G][MT] = {};
+  f32x4 acc[G] = {};
   const int full = args.K / BK;
   for (int s0 = wave; s0 < full; s0 += NW * U) {
-    u32x4 wv[U][G][2], xv[U][MT][2];
+    u32x4 wv[U][G][2], xv[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s0 + u * NW < full) {
@@ -633,8 +671,7 @@ __global__ __launch_bounds__(NW * kWave) void k_ffn_few(const FewArgs args) {
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int i = 0; i < G; ++i) wv[u][i][c] = __builtin_nontemporal_load((const CAME8_GLOBAL raw*)(w[i] + k + c * V));
-#pragma unroll
-          for (int i = 0; i < MT; ++i) xv[u][i][c] = *(const CAME8_GLOBAL raw*)(x[i] + k + c * V);
+          xv[u][c] = *(const CAME8_GLOBAL raw*)(x + k + c * V);
         }
       }
 #pragma unroll
@@ -643,33 +680,27 @@ __global__ __launch_bounds__(NW * kWave) void k_ffn_few(const FewArgs args) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[g][i] = mfma_chunk<T>(wv[u][g][c], xv[u][i][c], acc[g][i]);
+          for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(wv[u][g][c], xv[u][c], acc[g]);
   }
   if (full * BK < args.K && full % NW == wave) {
     const int k = full * BK, left = args.K - q;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c) {
+      const u32x4 xv = load_chunk<T>(x, k + c * V, left);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const u32x4 xv = load_chunk<T>(x[i], k + c * V, left);
-#pragma unroll
-        for (int g = 0; g < G; ++g) acc[g][i] = mfma_chunk<T>(load_chunk<T>(w[g], k + c * V, left), xv, acc[g][i]);
-      }
+      for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(load_chunk<T>(w[g], k + c * V, left), xv, acc[g]);
+    }
   }
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sums[wave][g * MT + i][lane] = acc[g][i];
+  for (int g = 0; g < G; ++g) sums[wave][g][lane] = acc[g];
   __syncthreads();
-  if (wave >= MT) return;
-  const int m = wave * 16 + lane % 16, n = n0 + lane / 16 * 4;
+  if (wave != 0) return;
+  const int m = lane % 16, n = n0 + lane / 16 * 4;
   f32x4 total[G] = {};
 #pragma unroll
   for (int i = 0; i < NW; ++i)
 #pragma unroll
-    for (int g = 0; g < G; ++g) total[g] += sums[i][g * MT + wave][lane];
+    for (int g = 0; g < G; ++g) total[g] += sums[i][g][lane];
   if (m >= args.M) return;
   S* out = static_cast<S*>(args.out) + int64_t(m) * args.ldo;
   const float a[4] = {total[0][0], total[0][1], total[0][2], total[0][3]};

@@ -60,10 +60,10 @@ Cut cut_of(const came8_ffn* f, const Size& z, bool gate) {
     const double us = f->dtype == CAME8_F32 ? v.full : v.half;
     if (us == 0.0) continue;
     const int64_t tiles = ceil_div(z.M, v.tile) * ceil_div(z.N, gate ? v.tile / 2 : v.tile), steps = steps_of(f, z);
-    for (int s = 1; s <= (gate ? 1 : kMaxSplits); ++s) {
+    for (int s = 1; s <= kMaxSplits; ++s) {
       if (s > 1 && steps / s < kSplitSteps) break;
       const double t = double(ceil_div(tiles * s, v.at_once)) * (double(ceil_div(steps, s)) + 3.0) * us +
-                       (s > 1 ? 4.0 + double(s) * double(z.M) * double(z.N) * 8.0 / kJoinBytes : 0.0);
+                       (s > 1 ? 4.0 + double(s) * double(z.M) * double(z.N) * (gate ? 16.0 : 8.0) / kJoinBytes : 0.0);
       if (t < least) {
         least = t;
         best.tile = v.tile;
@@ -91,8 +91,9 @@ void cut_together(const came8_ffn* f, const Size* z, int count, Cut* cuts) {
       const int64_t steps = steps_of(f, z[i]);
       splits[i] = int(std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, ceil_div(steps, share), steps / kSplitSteps})));
       longest = std::max(longest, ceil_div(steps, splits[i]) + 3);
-      if (splits[i] > 1) join += 4.0 + double(splits[i]) * double(z[i].M) * double(z[i].N) * 8.0 / kJoinBytes;
+      if (splits[i] > 1) join += double(splits[i]) * double(z[i].M) * double(z[i].N) * 8.0 / kJoinBytes;
     }
+    if (join > 0.0) join += 4.0;
     const double t = (std::max(work / v.at_once, double(longest)) + 0.5 * double(longest)) * us + join;
     if (t < least) {
       least = t;
@@ -100,12 +101,6 @@ void cut_together(const came8_ffn* f, const Size* z, int count, Cut* cuts) {
     }
   }
 }
-
-// Rows of x up to which the forward products read the weights straight into registers (k_ffn_few).
-#ifndef FEW
-#define FEW 64
-#endif
-constexpr int64_t kFewTokens = FEW;
 
 struct Cuts {
   Cut gate, down;          // forward
@@ -144,14 +139,14 @@ Layout layout_of(const came8_ffn* f, bool backward) {
     l.du = take(f->tokens, l.ldh);
     copy(l.dy, f->tokens, f->out, f->out);
   }
-  if (!backward && f->tokens <= kFewTokens) return l;
+  if (!backward && f->tokens <= kFewRows) return l;
   copy(l.x, f->tokens, f->dim, f->ld_x);
   copy(l.gate, f->hidden, f->dim, f->ld_gate);
   copy(l.up, f->hidden, f->dim, f->ld_up);
   copy(l.down, f->out, f->hidden, f->ld_down);
   // shares of split sums; dh's are joined before the others are written
   const Cuts c = cuts_of(f);
-  int64_t part = part_floats(c.down, f->tokens, f->out);
+  int64_t part = std::max(2 * part_floats(c.gate, f->tokens, f->hidden), part_floats(c.down, f->tokens, f->out));
   if (backward)
     part = std::max(part_floats(c.back, f->tokens, f->hidden),
                     part_floats(c.grads[0], f->tokens, f->dim) + part_floats(c.grads[1], f->hidden, f->dim) +
@@ -206,12 +201,8 @@ void tile(GemmArgs& a, const Cut& c, bool gate) {
   a.splits = c.splits;
 }
 
-template <typename T, Epilogue EPI>
-void join(const GemmArgs& a, hipStream_t stream) {
-  if (a.splits == 1) return;
-  const int64_t quads = int64_t(a.M) * ((a.N + 3) / 4);
-  hipLaunchKernelGGL((k_ffn_join<T, EPI>), dim3(unsigned(std::min<int64_t>(ceil_div(quads, kThreads), 1 << 16))), dim3(kThreads), 0,
-                     stream, a);
+unsigned join_groups(const GemmArgs& a) {
+  return unsigned(std::min<int64_t>(ceil_div(int64_t(a.M) * ((a.N + 3) / 4), kThreads), 1 << 14));
 }
 
 // One product over its tiles.  256 by 256 only for 16-bit types: fp32 products are bound by the matrix units at any size.
@@ -225,36 +216,31 @@ void launch(GemmArgs a, const Cut& c, float* part, hipStream_t stream) {
   }
   if (c.tile == 128) hipLaunchKernelGGL((k_ffn_gemm<T, 128, 2, true, BROWS, EPI>), grid, dim3(256), 0, stream, a);
   if (c.tile == 64) hipLaunchKernelGGL((k_ffn_gemm<T, 64, 2, true, BROWS, EPI>), grid, dim3(256), 0, stream, a);
-  if constexpr (EPI != kGate) join<T, EPI>(a, stream);
+  if (a.part) hipLaunchKernelGGL((k_ffn_join<T, EPI>), dim3(join_groups(a)), dim3(kThreads), 0, stream, a);
 }
 
-template <typename T, bool GATE>
-void launch_few(const FewArgs& a, hipStream_t stream) {
-  const unsigned groups = unsigned(ceil_div(a.N, 16));
-  if (a.M <= 16) hipLaunchKernelGGL((k_ffn_few<T, 1, 8, GATE>), dim3(groups), dim3(512), 0, stream, a);
-  else if (a.M <= 32) hipLaunchKernelGGL((k_ffn_few<T, 2, 8, GATE>), dim3(groups), dim3(512), 0, stream, a);
-  else hipLaunchKernelGGL((k_ffn_few<T, 4, 8, GATE>), dim3(groups), dim3(512), 0, stream, a);
+template <typename T>
+void forward_few(const came8_ffn* f, const void* x, const void* wg, const void* wu, const void* wd, void* y, float* g, float* u,
+                 const Layout& l, char* ws, hipStream_t stream) {
+  FewArgs a{};
+  a.x = x, a.ldx = f->ld_x;
+  a.w[0] = wg, a.w[1] = wu, a.ldw[0] = f->ld_gate, a.ldw[1] = f->ld_up;
+  a.M = int32_t(f->tokens), a.N = int32_t(f->hidden), a.K = int32_t(f->dim), a.act = f->activation;
+  a.out = ws + l.h, a.ldo = l.ldh;
+  a.g = g, a.u = u, a.ldg = f->hidden;
+  hipLaunchKernelGGL((k_ffn_few<T, true>), dim3(unsigned(ceil_div(a.N, 16))), dim3(512), 0, stream, a);
+  FewArgs d{};
+  d.x = ws + l.h, d.ldx = l.ldh;
+  d.w[0] = wd, d.ldw[0] = f->ld_down;
+  d.M = int32_t(f->tokens), d.N = int32_t(f->out), d.K = int32_t(f->hidden);
+  d.out = y, d.ldo = f->out;
+  hipLaunchKernelGGL((k_ffn_few<T, false>), dim3(unsigned(ceil_div(d.N, 16))), dim3(512), 0, stream, d);
 }
 
 template <typename T>
 void forward(const came8_ffn* f, const void* x, const void* wg, const void* wu, const void* wd, void* y, float* g, float* u,
              const Layout& l, char* ws, hipStream_t stream) {
-  if (f->tokens <= kFewTokens) {
-    FewArgs a{};
-    a.x = x, a.ldx = f->ld_x;
-    a.w[0] = wg, a.w[1] = wu, a.ldw[0] = f->ld_gate, a.ldw[1] = f->ld_up;
-    a.M = int32_t(f->tokens), a.N = int32_t(f->hidden), a.K = int32_t(f->dim), a.act = f->activation;
-    a.out = ws + l.h, a.ldo = l.ldh;
-    a.g = g, a.u = u, a.ldg = f->hidden;
-    launch_few<T, true>(a, stream);
-    FewArgs d{};
-    d.x = ws + l.h, d.ldx = l.ldh;
-    d.w[0] = wd, d.ldw[0] = f->ld_down;
-    d.M = int32_t(f->tokens), d.N = int32_t(f->out), d.K = int32_t(f->hidden);
-    d.out = y, d.ldo = f->out;
-    launch_few<T, false>(d, stream);
-    return;
-  }
+  if (f->tokens <= kFewRows) return forward_few<T>(f, x, wg, wu, wd, y, g, u, l, ws, stream);
   GemmArgs a{};
   a.nseg = 1;
   a.act = f->activation;
@@ -328,8 +314,10 @@ void backward(const came8_ffn* f, const void* x, const void* wg, const void* wu,
   }
   if (t == 128) hipLaunchKernelGGL((k_ffn_grads<T, 128, 2>), dim3(unsigned(groups)), dim3(256), 0, stream, r);
   if (t == 64) hipLaunchKernelGGL((k_ffn_grads<T, 64, 2>), dim3(unsigned(groups)), dim3(256), 0, stream, r);
-  if (dx) join<T, kStore>(r.dx, stream);
-  for (int k = 0; k < count; ++k) join<T, kStore>(r.dw[k], stream);
+  unsigned most = 0;
+  for (const GemmArgs* g : {&r.dx, &r.dw[0], &r.dw[1], &r.dw[2]})
+    if (g->part) most = std::max(most, join_groups(*g));
+  if (most > 0) hipLaunchKernelGGL(k_ffn_join_grads<T>, dim3(most, 4), dim3(kThreads), 0, stream, r);
 }
 
 }  // namespace
