@@ -245,9 +245,10 @@ def load(path: str | None = None) -> ctypes.CDLL:
 
 
 def host():
-    """The native descriptor gathering (csrc/came8_host.cpp), loaded once; RuntimeError if it is missing."""
+    """The native descriptor gathering and autograd node (csrc/came8_host.cpp), loaded once; RuntimeError if it is missing."""
     global _host
     if _host is None:
+        lib = load()
         with _lock:
             if _host is None:
                 if not os.path.exists(HOST_PATH):
@@ -257,6 +258,9 @@ def host():
                 spec = importlib.util.spec_from_file_location("came8_host", HOST_PATH)
                 mod = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(mod)
+                mod.bind(*(ctypes.cast(entry, ctypes.c_void_p).value for entry in (
+                    lib.came8_gated_ffn_workspace_size, lib.came8_gated_ffn_forward, lib.came8_gated_ffn_backward,
+                    lib.came8_last_error)))
                 _host = mod
     return _host
 
