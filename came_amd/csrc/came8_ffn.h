@@ -606,16 +606,19 @@ __global__ __launch_bounds__(kThreads) void k_ffn_join_grads(const GradArgs args
 // Up to 16 rows: the weights are read once and are all there is to wait for, so no tile goes through LDS.  A workgroup has
 // 16 rows of the weights (kGate: of both) and all rows of x; its 8 wavefronts take steps of 128 bytes of k in turn, a lane
 // two chunks of a row at once, whole lines of a row by four lanes, four steps in flight; their sums are added in order in
-// LDS.  Rows may start at any element.  One token of 4096 and 11008 in bf16: 36.8 us for 180 MB of gate and up, 21.7 for the
-// 90 MB of down (4.9 and 4.2 TB/s), 58 together, 75 in tiles; 2 or 8 steps in flight and 16 wavefronts changed nothing.  With
+// LDS.  Rows may start at any element.  One token of 4096 and 11008 in bf16: 36.8 us for 180 MB of gate and up, 22 for the
+// 90 MB of down (4.9 and 4.1 TB/s), 60 together, 75 in tiles; 2 or 8 steps in flight and 16 wavefronts changed nothing.  With
 // 32 rows it took 89 us, tiles 75: x then costs more loads than the weights.
+//
+// h between the two is kept in fp32: as an operand it is its rounding to the type and the rest's, two products, which the
+// weights' way hides, so that y is rounded once.
 struct FewArgs {
-  const void* x;
+  const void* x;     // down: h, float
   int64_t ldx;
   const void* w[2];  // kGate: gate and up
   int64_t ldw[2];
   int32_t M, N, K, act;
-  void* out;
+  void* out;         // gate and up: h, float
   int64_t ldo;
   float* g;
   float* u;
@@ -644,6 +647,22 @@ __device__ __forceinline__ u32x4 load_chunk(const CAME8_GLOBAL typename T::stora
   return v;
 }
 
+// 8 floats as two chunks of a 16-bit type: their roundings, and the roundings of the rest (none of what rounds to infinity)
+template <typename T>
+__device__ __forceinline__ void split_chunk(f32x4 a, f32x4 b, u32x4& high, u32x4& low) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+    const uint32_t hx = T::store(x), hy = T::store(y);
+    const uint32_t word = hx | hy << 16;
+    high[i] = word;
+    float rx = x - T::elem(&word, 0), ry = y - T::elem(&word, 1);
+    rx = fabsf(rx) <= 0x1p127f ? rx : 0.0f;
+    ry = fabsf(ry) <= 0x1p127f ? ry : 0.0f;
+    low[i] = uint32_t(T::store(rx)) | uint32_t(T::store(ry)) << 16;
+  }
+}
+
 template <typename T, bool GATE>
 __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
   using S = typename T::storage;
@@ -657,12 +676,15 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
 #pragma unroll
   for (int i = 0; i < G; ++i)
     w[i] = gbl(static_cast<const S*>(args.w[i])) + int64_t(min(n0 + lane % 16, args.N - 1)) * args.ldw[i] + q;
-  const CAME8_GLOBAL S* x = gbl(static_cast<const S*>(args.x)) + int64_t(min(lane % 16, args.M - 1)) * args.ldx + q;
+  constexpr bool kSplit = !GATE && sizeof(S) == 2;  // x is h in fp32, in two 16-bit parts
+  using X = typename std::conditional<GATE, S, float>::type;
+  constexpr int P = kSplit ? 2 : 1;
+  const CAME8_GLOBAL X* x = gbl(static_cast<const X*>(args.x)) + int64_t(min(lane % 16, args.M - 1)) * args.ldx + q;
 
   f32x4 acc[G] = {};
   const int full = args.K / BK;
   for (int s0 = wave; s0 < full; s0 += NW * U) {
-    u32x4 wv[U][G][2], xv[U][2];
+    u32x4 wv[U][G][2], xv[U][2][P];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s0 + u * NW < full) {
@@ -671,24 +693,45 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int i = 0; i < G; ++i) wv[u][i][c] = __builtin_nontemporal_load((const CAME8_GLOBAL raw*)(w[i] + k + c * V));
-          xv[u][c] = *(const CAME8_GLOBAL raw*)(x + k + c * V);
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            if constexpr (GATE) xv[u][c][p] = *(const CAME8_GLOBAL raw*)(x + k + c * V);
+            else xv[u][c][p] = __builtin_bit_cast(u32x4, *(const CAME8_GLOBAL f32x4*)(x + k + c * V + 4 * p));
+          }
         }
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s0 + u * NW < full)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) {
+          if constexpr (kSplit) {
+            u32x4 high, low;
+            split_chunk<T>(__builtin_bit_cast(f32x4, xv[u][c][0]), __builtin_bit_cast(f32x4, xv[u][c][1]), high, low);
+            acc[0] = mfma_chunk<T>(wv[u][0][c], high, acc[0]);
+            acc[0] = mfma_chunk<T>(wv[u][0][c], low, acc[0]);
+          } else {
 #pragma unroll
-          for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(wv[u][g][c], xv[u][c], acc[g]);
+            for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(wv[u][g][c], xv[u][c][0], acc[g]);
+          }
+        }
   }
   if (full * BK < args.K && full % NW == wave) {
     const int k = full * BK, left = args.K - q;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const u32x4 xv = load_chunk<T>(x, k + c * V, left);
+      if constexpr (kSplit) {
+        u32x4 high, low;
+        split_chunk<T>(__builtin_bit_cast(f32x4, load_chunk<F32>(x, k + c * V, left)),
+                       __builtin_bit_cast(f32x4, load_chunk<F32>(x, k + c * V + 4, left)), high, low);
+        const u32x4 wv = load_chunk<T>(w[0], k + c * V, left);
+        acc[0] = mfma_chunk<T>(wv, high, acc[0]);
+        acc[0] = mfma_chunk<T>(wv, low, acc[0]);
+      } else {
+        const u32x4 xv = load_chunk<T>(x, k + c * V, left);
 #pragma unroll
-      for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(load_chunk<T>(w[g], k + c * V, left), xv, acc[g]);
+        for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(load_chunk<T>(w[g], k + c * V, left), xv, acc[g]);
+      }
     }
   }
 #pragma unroll
@@ -702,7 +745,6 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
 #pragma unroll
     for (int g = 0; g < G; ++g) total[g] += sums[i][g][lane];
   if (m >= args.M) return;
-  S* out = static_cast<S*>(args.out) + int64_t(m) * args.ldo;
   const float a[4] = {total[0][0], total[0][1], total[0][2], total[0][3]};
   if constexpr (GATE) {
     const float b[4] = {total[1][0], total[1][1], total[1][2], total[1][3]};
@@ -710,13 +752,13 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
     activate<false>(a, args.act, h, none);
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] *= b[e];
-    store4<T>(out, n, args.N, h);
+    store4<F32>(static_cast<float*>(args.out) + int64_t(m) * args.ldo, n, args.N, h);
     if (args.g) {
       store4<F32>(args.g + int64_t(m) * args.ldg, n, args.N, a);
       store4<F32>(args.u + int64_t(m) * args.ldg, n, args.N, b);
     }
   } else {
-    store4<T>(out, n, args.N, a);
+    store4<T>(static_cast<S*>(args.out) + int64_t(m) * args.ldo, n, args.N, a);
   }
 }
 

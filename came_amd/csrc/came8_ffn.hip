@@ -133,13 +133,16 @@ Layout layout_of(const came8_ffn* f, bool backward) {
     c.at = take(rows, c.ld);
   };
   l.ldh = up(f->hidden, 16 / es);
+  if (!backward && f->tokens <= kFewRows) {  // h in fp32
+    l.h = take(f->tokens * 4 / es, l.ldh);
+    return l;
+  }
   l.h = take(f->tokens, l.ldh);
   if (backward) {
     l.dg = take(f->tokens, l.ldh);
     l.du = take(f->tokens, l.ldh);
     copy(l.dy, f->tokens, f->out, f->out);
   }
-  if (!backward && f->tokens <= kFewRows) return l;
   copy(l.x, f->tokens, f->dim, f->ld_x);
   copy(l.gate, f->hidden, f->dim, f->ld_gate);
   copy(l.up, f->hidden, f->dim, f->ld_up);
