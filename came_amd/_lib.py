@@ -259,8 +259,9 @@ def host():
                 mod = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(mod)
                 mod.bind(*(ctypes.cast(entry, ctypes.c_void_p).value for entry in (
-                    lib.came8_gated_ffn_workspace_size, lib.came8_gated_ffn_forward, lib.came8_gated_ffn_backward,
-                    lib.came8_last_error)))
+                    lib.came8_last_error, lib.came8_adamw_step, lib.came8_grad_norm_workspace_size, lib.came8_grad_norm,
+                    lib.came8_grad_clip, lib.came8_gated_ffn_workspace_size, lib.came8_gated_ffn_forward,
+                    lib.came8_gated_ffn_backward)))
                 _host = mod
     return _host
 

@@ -146,6 +146,19 @@ class _AdamWBase(torch.optim.Optimizer):
             _lib.check(_lib.load().came8_adamw_step(descs, n, ctypes.byref(hp), factor.data_ptr() if factor is not None else None,
                                                     torch.cuda.current_stream(device).cuda_stream), "came8_adamw_step")
 
+    def _step_native(self, group: dict, factor) -> bool:
+        """The group's step, descriptors and all, natively (csrc/came8_host.cpp); False: the Python has to take it."""
+        params = group["params"]
+        device = next((p.device for p in params if p.grad is not None), None)
+        if device is None:
+            return True
+        if type(params) is not list or device.type != "cuda":
+            return False
+        hp = self._hparams(group)
+        return bool(_lib.host().adamw_step(
+            params, self.state, hp.bits, hp.block_size, hp.seed, hp.lr, hp.beta1, hp.beta2, hp.eps, hp.weight_decay,
+            factor.data_ptr() if factor is not None else 0, torch.cuda.current_stream(device).cuda_stream))
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -162,13 +175,7 @@ class _AdamWBase(torch.optim.Optimizer):
                 return loss
             self.last_grad_norm, factor = found
         for group in self.param_groups:
-            params = group["params"]
-            descs = (_lib.Came8AdamwTensor * max(len(params), 1))()
-            used = _lib.host().gather_adamw(params, self.state, ctypes.addressof(descs), len(params), self._BITS,
-                                            self._block_size(group)) if type(params) is list else None
-            if used is not None:
-                if used:
-                    self._launch(used[0].device, descs, len(used), group, factor)
+            if self._step_native(group, factor):
                 continue
             lists, copyback = self._descriptors(group)
             for device, (descs, n, keep) in lists.items():

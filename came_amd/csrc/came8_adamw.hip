@@ -20,7 +20,12 @@ namespace {
 
 constexpr int kAdamTab = 64;    // tensors a launch: 60 bytes each of the 4 KB of arguments
 constexpr int kGradTab = 192;   // 20 bytes each
-constexpr int kAdamChunk = 8192;   // elements of a workgroup: 256 lanes x 4 rows x 8
+// Elements of a workgroup: 256 lanes by 8 by 4 rows; a launch that has fewer than kSmallLaunch of those takes single rows (or
+// as few as a block of 8-bit moments needs), since then only its latency counts: 192 adapters of 10 to 33 thousand elements,
+// three launches of 11.2 us in 4 rows and of 7.4 in single ones.
+constexpr int kAdamRow = 2048;
+constexpr int kAdamRows = 4;
+constexpr int kSmallLaunch = 512;
 constexpr int kGradChunk = 16384;
 constexpr int kNormGroups = 2048;  // workgroups of a norm launch: eight a CU, what is resident
 constexpr float kTinyBlock = 0x1p-100f;  // 8-bit blocks whose largest is below hold zeros (127/a and 1.875/a stay finite)
@@ -139,9 +144,9 @@ struct U8 {
 // 355 M fp32 parameters and the norm before it 1970 us (5.8 TB/s), 1.07 G bf16 ones 4281 us (5.5 TB/s); one round at a time
 // 2040 and 4420, eight elements a lane (two instructions an fp32 operand, each touching half of the lines) 2185 and 4650,
 // without the nontemporal hint 2181 and 4550.  The divide and square root are the IEEE ones: the memory hides them.
-template <typename P, typename G>
+template <typename P, typename G, int ROWS>
 __global__ __launch_bounds__(kThreads) void k_adamw32(const AdamTab tab) {
-  constexpr int V = 4, U = 4;
+  constexpr int V = 4, U = ROWS == 1 ? 2 : 4, kAdamChunk = kAdamRow * ROWS;
   const int t = find_tensor(tab.start, tab.count, int(blockIdx.x));
   const int64_t n = tab.n[t];
   const int64_t base = int64_t(int(blockIdx.x) - tab.start[t]) * kAdamChunk;
@@ -196,16 +201,17 @@ __device__ __forceinline__ uint32_t pair_hash(uint32_t pair, uint32_t key) {
   return x ^ (x >> 13);
 }
 
-// One wavefront takes 4 rows of 512 elements, 8 to a lane; a block is a part of a row, a row (K = 1), or K rows, so its
+// One wavefront takes 4 rows (or 1 or 2) of 512 elements, 8 to a lane; a block is a part of a row, a row (K = 1), or K rows, so its
 // largest is a reduction over lanes and no LDS is used.  Bound by memory: 1.07 G bf16 parameters 1913 us, 5.6 TB/s of their
 // 10 bytes each (1922 with one row loaded at a time), though some 60 operations an element come near what the vector units
 // issue meanwhile; an IEEE square root and division would be over it.
-template <typename P, typename G, int K>
+template <typename P, typename G, int K, int ROWS>
 __global__ __launch_bounds__(kThreads) void k_adamw8(const AdamTab tab) {
+  constexpr int kAdamChunk = kAdamRow * ROWS;
   const int t = find_tensor(tab.start, tab.count, int(blockIdx.x));
   const int64_t n = tab.n[t];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int64_t base = int64_t(int(blockIdx.x) - tab.start[t]) * kAdamChunk + wave * 2048 + lane * 8;
+  const int64_t base = int64_t(int(blockIdx.x) - tab.start[t]) * kAdamChunk + wave * (512 * ROWS) + lane * 8;
   auto* p = gbl(static_cast<typename P::storage*>(tab.p[t]));
   auto* g = gbl(static_cast<const typename G::storage*>(tab.g[t]));
   auto* mq = gbl(static_cast<uint8_t*>(tab.m[t]));
@@ -213,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw8(const AdamTab tab) {
   auto *ma = gbl(tab.ma[t]), *va = gbl(tab.va[t]);
   const float scale = tab.scale ? *tab.scale : 1.0f;
   const int lanes = K > 1 ? kWave : min(kWave, 1 << (tab.log2b - 3));  // of a block in a row
-  constexpr int L = 4;  // rows loaded together
+  constexpr int L = ROWS;  // loaded together
   Row<G, 8> gr[L];
   Row<P, 8> pr[L];
   Row<U8, 8> mc[L], vc[L];
@@ -438,19 +444,24 @@ constexpr int64_t kMaxGroups = int64_t(1) << 23;    // of a launch: its work ite
 
 using AdamFn = void (*)(AdamTab);
 
+// rows: in and out, how many a workgroup's wavefronts take; 1 asks for the fewest that the block size allows
 template <typename P, typename G>
-AdamFn adam_kernel(int bits, int block) {
-  if (bits == 32) return k_adamw32<P, G>;
-  return block <= 512 ? k_adamw8<P, G, 1> : block == 1024 ? k_adamw8<P, G, 2> : k_adamw8<P, G, 4>;
+AdamFn adam_kernel(int bits, int block, int& rows) {
+  if (bits == 32) return rows == 1 ? k_adamw32<P, G, 1> : k_adamw32<P, G, kAdamRows>;
+  if (block == 2048) rows = 4;
+  if (block == 1024 && rows == 1) rows = 2;
+  if (block == 2048) return k_adamw8<P, G, 4, 4>;
+  if (block == 1024) return rows == 2 ? k_adamw8<P, G, 2, 2> : k_adamw8<P, G, 2, 4>;
+  return rows == 1 ? k_adamw8<P, G, 1, 1> : k_adamw8<P, G, 1, 4>;
 }
 template <typename P>
-AdamFn adam_kernel_g(int gdt, int bits, int block) {
-  return gdt == CAME8_F32 ? adam_kernel<P, F32>(bits, block)
-         : gdt == CAME8_BF16 ? adam_kernel<P, BF16>(bits, block) : adam_kernel<P, F16>(bits, block);
+AdamFn adam_kernel_g(int gdt, int bits, int block, int& rows) {
+  return gdt == CAME8_F32 ? adam_kernel<P, F32>(bits, block, rows)
+         : gdt == CAME8_BF16 ? adam_kernel<P, BF16>(bits, block, rows) : adam_kernel<P, F16>(bits, block, rows);
 }
-AdamFn adam_kernel_of(int pdt, int gdt, int bits, int block) {
-  return pdt == CAME8_F32 ? adam_kernel_g<F32>(gdt, bits, block)
-         : pdt == CAME8_BF16 ? adam_kernel_g<BF16>(gdt, bits, block) : adam_kernel_g<F16>(gdt, bits, block);
+AdamFn adam_kernel_of(int pdt, int gdt, int bits, int block, int& rows) {
+  return pdt == CAME8_F32 ? adam_kernel_g<F32>(gdt, bits, block, rows)
+         : pdt == CAME8_BF16 ? adam_kernel_g<BF16>(gdt, bits, block, rows) : adam_kernel_g<F16>(gdt, bits, block, rows);
 }
 
 uint32_t mix(uint32_t x) {
@@ -459,15 +470,17 @@ uint32_t mix(uint32_t x) {
   return x ^ (x >> 13);
 }
 
+int refuse(const char* what, int32_t tensor, const char* why) {
+  return op_fail(CAME8_EINVAL, std::string(what) + ": tensor " + std::to_string(tensor) + ": " + why);
+}
+
 int check_grads(const char* what, const came8_grad_tensor* ts, int32_t n) {
   if (n < 0 || (n > 0 && ts == nullptr)) return op_fail(CAME8_EINVAL, std::string(what) + ": no tensors given");
   for (int32_t i = 0; i < n; ++i) {
     const came8_grad_tensor& t = ts[i];
-    const std::string at = std::string(what) + ": tensor " + std::to_string(i);
-    if (!type_ok(t.dtype)) return op_fail(CAME8_EINVAL, at + ": unknown dtype " + std::to_string(t.dtype));
-    if (t.numel < 0 || t.numel > kMaxElements) return op_fail(CAME8_EINVAL, at + ": bad numel " + std::to_string(t.numel));
-    if (t.numel > 0 && (t.data == nullptr || !aligned(t.data, size_of(t.dtype))))
-      return op_fail(CAME8_EINVAL, at + ": null or misaligned pointer");
+    if (!type_ok(t.dtype)) return refuse(what, i, "unknown dtype");
+    if (t.numel < 0 || t.numel > kMaxElements) return refuse(what, i, "bad numel");
+    if (t.numel > 0 && (t.data == nullptr || !aligned(t.data, size_of(t.dtype)))) return refuse(what, i, "null or misaligned pointer");
   }
   return CAME8_OK;
 }
@@ -569,18 +582,18 @@ int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const
     if (hp->flags != 0) return op_fail(CAME8_EINVAL, "came8_adamw_step: unknown flags");
     for (int32_t i = 0; i < n_tensors; ++i) {
       const came8_adamw_tensor& t = tensors[i];
-      const std::string at = "came8_adamw_step: tensor " + std::to_string(i);
-      if (!type_ok(t.param_dtype) || !type_ok(t.grad_dtype)) return op_fail(CAME8_EINVAL, at + ": unknown dtype");
-      if (t.numel < 0 || t.numel > kMaxElements) return op_fail(CAME8_EINVAL, at + ": bad numel");
-      if (t.step < 1) return op_fail(CAME8_EINVAL, at + ": step must be >= 1");
+      const char* what = "came8_adamw_step";
+      if (!type_ok(t.param_dtype) || !type_ok(t.grad_dtype)) return refuse(what, i, "unknown dtype");
+      if (t.numel < 0 || t.numel > kMaxElements) return refuse(what, i, "bad numel");
+      if (t.step < 1) return refuse(what, i, "step must be >= 1");
       if (t.numel == 0) continue;
       const size_t ms = hp->bits == 32 ? 4 : 1;
       if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || !aligned(t.param, size_of(t.param_dtype)) ||
           !aligned(t.grad, size_of(t.grad_dtype)) || !aligned(t.exp_avg, ms) || !aligned(t.exp_avg_sq, ms))
-        return op_fail(CAME8_EINVAL, at + ": null or misaligned pointer");
+        return refuse(what, i, "null or misaligned pointer");
       if (hp->bits == 8 && (!t.exp_avg_absmax || !t.exp_avg_sq_absmax || !aligned(t.exp_avg_absmax, 4) ||
                             !aligned(t.exp_avg_sq_absmax, 4)))
-        return op_fail(CAME8_EINVAL, at + ": null or misaligned absmax");
+        return refuse(what, i, "null or misaligned absmax");
     }
     // launches: tensors of one (types, step count) together, in the order given
     std::vector<char> done(size_t(n_tensors), 0);
@@ -600,11 +613,18 @@ int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const
       tab.key = mix(mix(hp->seed) ^ uint32_t(f.step));
       tab.log2b = hp->bits == 8 ? __builtin_ctz(unsigned(B)) : 0;
       tab.scale = grad_scale;
-      const AdamFn fn = adam_kernel_of(f.param_dtype, f.grad_dtype, hp->bits, B);
-      int64_t chunks = 0;
+      int64_t chunks = 0;  // of kAdamRows rows
       tab.count = 0;
       auto flush = [&]() {
-        if (tab.count > 0) hipLaunchKernelGGL(fn, dim3(unsigned(chunks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), tab);
+        if (tab.count == 0) return;
+        int rows = chunks < kSmallLaunch ? 1 : kAdamRows;
+        const AdamFn fn = adam_kernel_of(f.param_dtype, f.grad_dtype, hp->bits, B, rows);
+        int64_t groups = 0;
+        for (int k = 0; k < tab.count; ++k) {
+          tab.start[k] = int32_t(groups);
+          groups += chunks_of(tab.n[k], int64_t(kAdamRow) * rows);
+        }
+        hipLaunchKernelGGL(fn, dim3(unsigned(groups)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), tab);
         tab.count = 0;
         chunks = 0;
       };
@@ -613,7 +633,7 @@ int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const
         if (done[size_t(j)] || a.numel == 0 || a.step != f.step || a.param_dtype != f.param_dtype || a.grad_dtype != f.grad_dtype)
           continue;
         done[size_t(j)] = 1;
-        const int64_t c = chunks_of(a.numel, kAdamChunk);
+        const int64_t c = chunks_of(a.numel, int64_t(kAdamRow) * kAdamRows);
         if (tab.count == kAdamTab || chunks + c > kMaxGroups) flush();
         const int k = tab.count++;
         tab.p[k] = a.param;
@@ -623,7 +643,6 @@ int came8_adamw_step(const came8_adamw_tensor* tensors, int32_t n_tensors, const
         tab.ma[k] = a.exp_avg_absmax;
         tab.va[k] = a.exp_avg_sq_absmax;
         tab.n[k] = a.numel;
-        tab.start[k] = int32_t(chunks);
         chunks += c;
       }
       flush();

@@ -1,5 +1,5 @@
-// came8_host: descriptors of a param group's tensors for came8_step (and for came8_adamw_step and the gradient norm),
-// filled natively, and the gated feed-forward block as an autograd node.
+// came8_host: descriptors of a param group's tensors for came8_step, filled natively; AdamW's step and the gradient norm with
+// theirs; and the gated feed-forward block as an autograd node.
 //
 // gather() does what the optimizers' Python does for every parameter of a group before a step (the checks of
 // _prepare_param and _check_state, the fields of _descriptors and _fill_desc, the step counts) for the plain case:
@@ -40,6 +40,12 @@ int dtype_code(const at::Tensor& t) {
 const at::Tensor* tensor_of(PyObject* st, PyObject* name) {
   PyObject* o = PyDict_GetItemWithError(st, name);
   return o != nullptr && THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr;
+}
+
+// A parameter's state (borrowed), or null.  A tensor's hash is its address (torch.Tensor.__hash__, which the lookup would
+// call in Python for every parameter: CAME's gather of 192 tensors took 44 us so, and takes 30 without the calls).
+PyObject* state_of(PyObject* state, PyObject* param) {
+  return _PyDict_GetItem_KnownHash(state, param, Py_hash_t(reinterpret_cast<uintptr_t>(param)));
 }
 
 bool flag_off(PyObject* st, PyObject* name) {
@@ -198,7 +204,7 @@ PyObject* gather(PyObject*, PyObject* args) {
     counts.reserve(used.size());
     for (size_t i = 0; i < used.size(); ++i) {
       const at::Tensor& p = THPVariable_Unpack(used[i]);
-      PyObject* st = PyDict_GetItemWithError(state, used[i]);
+      PyObject* st = state_of(state, used[i]);
       long step = 0;
       if (st == nullptr || !PyDict_Check(st) || !describe(p, grads[i], st, kind, block, out[i], &step)) {
         PyErr_Clear();
@@ -213,6 +219,20 @@ PyObject* gather(PyObject*, PyObject* args) {
   }
 }
 
+// libcame8's entries, which Python has loaded
+struct Entries {
+  decltype(&came8_last_error) error = nullptr;
+  decltype(&came8_adamw_step) adamw = nullptr;
+  decltype(&came8_grad_norm_workspace_size) norm_size = nullptr;
+  decltype(&came8_grad_norm) norm = nullptr;
+  decltype(&came8_grad_clip) clip = nullptr;
+  decltype(&came8_gated_ffn_workspace_size) ffn_size = nullptr;
+  decltype(&came8_gated_ffn_forward) ffn_forward = nullptr;
+  decltype(&came8_gated_ffn_backward) ffn_backward = nullptr;
+} entries;
+
+void entry_check(int rc, const char* what) { TORCH_CHECK(rc == CAME8_OK, what, " failed (", rc, "): ", entries.error()); }
+
 // The buffer of a moment or its scales: contiguous, of the parameter's device; null otherwise.
 void* moment(PyObject* st, PyObject* name, const at::Tensor& p, at::ScalarType type, int64_t n) {
   const at::Tensor* t = tensor_of(st, name);
@@ -221,109 +241,113 @@ void* moment(PyObject* st, PyObject* name, const at::Tensor& p, at::ScalarType t
              : nullptr;
 }
 
-// gather_adamw(params: list, state: dict, address: int, capacity: int, bits: int, block_size: int)
-//   -> gather() for came8_adamw_tensor descriptors.
-PyObject* gather_adamw(PyObject*, PyObject* args) {
+// adamw_step(params: list, state: dict, bits, block_size, seed, lr, beta1, beta2, eps, weight_decay, grad_scale: int, stream:
+//   int) -> True: the group's parameters with a gradient are stepped (came8_adamw_step) and their step counts advanced;
+//   None: not the plain case, nothing changed.  As gather(), and the call with it: 4 tensors 17 us of host time a step
+//   instead of 19 with the descriptors handed back.
+PyObject* adamw_step(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
   PyObject *params, *state;
-  unsigned long long addr;
-  long long cap, block;
-  int bits;
-  if (!PyArg_ParseTuple(args, "O!O!KLiL", &PyList_Type, &params, &PyDict_Type, &state, &addr, &cap, &bits, &block))
+  unsigned long long scale, stream;
+  came8_adamw_hparams hp{};
+  if (!PyArg_ParseTuple(args, "O!O!iiIdddddKK", &PyList_Type, &params, &PyDict_Type, &state, &hp.bits, &hp.block_size, &hp.seed,
+                        &hp.lr, &hp.beta1, &hp.beta2, &hp.eps, &hp.weight_decay, &scale, &stream))
     return nullptr;
-  if (block < 1) Py_RETURN_NONE;
+  if (hp.block_size < 1) Py_RETURN_NONE;
   static PyObject *k_step = key("step"), *k_m = key("exp_avg"), *k_v = key("exp_avg_sq"), *k_mq = key("exp_avg_q"),
                   *k_vq = key("exp_avg_sq_q"), *k_ma = key("exp_avg_absmax"), *k_va = key("exp_avg_sq_absmax");
-  try {
-    came8_adamw_tensor* out = reinterpret_cast<came8_adamw_tensor*>(static_cast<uintptr_t>(addr));
-    std::vector<PyObject*> used;
-    std::vector<at::Tensor> grads;
-    if (!collect(params, cap, used, grads)) Py_RETURN_NONE;
-    std::vector<std::pair<PyObject*, long>> counts;
-    counts.reserve(used.size());
-    for (size_t i = 0; i < used.size(); ++i) {
-      const at::Tensor& p = THPVariable_Unpack(used[i]);
-      PyObject* st = PyDict_GetItemWithError(state, used[i]);
-      PyObject* so = st != nullptr && PyDict_Check(st) ? PyDict_GetItemWithError(st, k_step) : nullptr;
-      int over = 0;
-      const long step = so != nullptr && PyLong_CheckExact(so) ? PyLong_AsLongAndOverflow(so, &over) : -1;
-      if (step < 0 || over != 0) {
-        PyErr_Clear();
-        Py_RETURN_NONE;
-      }
-      came8_adamw_tensor& d = out[i];
-      d = came8_adamw_tensor{};
-      d.param = p.data_ptr();
-      d.grad = grads[i].data_ptr();
-      d.numel = p.numel();
-      d.step = step + 1;
-      d.param_dtype = dtype_code(p);
-      d.grad_dtype = dtype_code(grads[i]);
-      if (bits == 32) {
-        d.exp_avg = moment(st, k_m, p, at::kFloat, d.numel);
-        d.exp_avg_sq = moment(st, k_v, p, at::kFloat, d.numel);
-      } else {
-        d.exp_avg = moment(st, k_mq, p, at::kChar, d.numel);
-        d.exp_avg_sq = moment(st, k_vq, p, at::kByte, d.numel);
-        d.exp_avg_absmax = static_cast<float*>(moment(st, k_ma, p, at::kFloat, num_blocks(d.numel, block)));
-        d.exp_avg_sq_absmax = static_cast<float*>(moment(st, k_va, p, at::kFloat, num_blocks(d.numel, block)));
-      }
-      if (d.exp_avg == nullptr || d.exp_avg_sq == nullptr ||
-          (bits != 32 && (d.exp_avg_absmax == nullptr || d.exp_avg_sq_absmax == nullptr))) {
-        PyErr_Clear();
-        Py_RETURN_NONE;
-      }
-      counts.emplace_back(st, step);
+  std::vector<PyObject*> used;
+  std::vector<at::Tensor> grads;
+  if (!collect(params, PyList_GET_SIZE(params), used, grads)) Py_RETURN_NONE;
+  if (used.empty()) Py_RETURN_TRUE;
+  std::vector<came8_adamw_tensor> descs(used.size());
+  std::vector<std::pair<PyObject*, long>> counts;
+  counts.reserve(used.size());
+  for (size_t i = 0; i < used.size(); ++i) {
+    const at::Tensor& p = THPVariable_Unpack(used[i]);
+    PyObject* st = state_of(state, used[i]);
+    PyObject* so = st != nullptr && PyDict_Check(st) ? PyDict_GetItemWithError(st, k_step) : nullptr;
+    int over = 0;
+    const long step = so != nullptr && PyLong_CheckExact(so) ? PyLong_AsLongAndOverflow(so, &over) : -1;
+    if (step < 0 || over != 0) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
     }
-    return advanced(used, counts);
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+    came8_adamw_tensor& d = descs[i];
+    d.param = p.data_ptr();
+    d.grad = grads[i].data_ptr();
+    d.numel = p.numel();
+    d.step = step + 1;
+    d.param_dtype = dtype_code(p);
+    d.grad_dtype = dtype_code(grads[i]);
+    if (hp.bits == 32) {
+      d.exp_avg = moment(st, k_m, p, at::kFloat, d.numel);
+      d.exp_avg_sq = moment(st, k_v, p, at::kFloat, d.numel);
+    } else {
+      d.exp_avg = moment(st, k_mq, p, at::kChar, d.numel);
+      d.exp_avg_sq = moment(st, k_vq, p, at::kByte, d.numel);
+      d.exp_avg_absmax = static_cast<float*>(moment(st, k_ma, p, at::kFloat, num_blocks(d.numel, hp.block_size)));
+      d.exp_avg_sq_absmax = static_cast<float*>(moment(st, k_va, p, at::kFloat, num_blocks(d.numel, hp.block_size)));
+    }
+    if (d.exp_avg == nullptr || d.exp_avg_sq == nullptr ||
+        (hp.bits != 32 && (d.exp_avg_absmax == nullptr || d.exp_avg_sq_absmax == nullptr))) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    counts.emplace_back(st, step);
   }
+  c10::OptionalDeviceGuard guard(grads[0].device());
+  entry_check(entries.adamw(descs.data(), int32_t(descs.size()), &hp, reinterpret_cast<const float*>(scale),
+                            reinterpret_cast<void*>(stream)),
+              "came8_adamw_step");
+  PyObject* list = advanced(used, counts);
+  if (list == nullptr) return nullptr;
+  Py_DECREF(list);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
 }
 
-// gather_grads(tensors: list, address: int, capacity: int, of_parameters: bool) -> the number of came8_grad_tensor
-//   descriptors now at `address`, one for each tensor (or for the gradient of each parameter that has one); None: some
-//   tensor is not a plain contiguous one of the first's device.  192 gradients: 12 us less than a list of them in Python.
-PyObject* gather_grads(PyObject*, PyObject* args) {
+// grad_norm(tensors: list, of_parameters: bool, max_norm: float, scale: bool, stream: int) -> (norm, factor), device scalars of
+//   the tensors (or of the parameters' gradients, of those that have one); with scale they are multiplied in place.  False:
+//   no tensors; None: some tensor is not a plain contiguous one of the first's device.
+PyObject* grad_norm(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
   PyObject* tensors;
-  unsigned long long addr;
-  long long cap;
-  int of_parameters;
-  if (!PyArg_ParseTuple(args, "O!KLp", &PyList_Type, &tensors, &addr, &cap, &of_parameters)) return nullptr;
-  try {
-    came8_grad_tensor* out = reinterpret_cast<came8_grad_tensor*>(static_cast<uintptr_t>(addr));
-    long long n = 0;
-    c10::optional<at::Device> device;
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
-      PyObject* o = PyList_GET_ITEM(tensors, i);
-      if (!THPVariable_CheckExact(o) && !(of_parameters && THPVariable_Check(o))) Py_RETURN_NONE;
-      const at::Tensor& t = of_parameters ? THPVariable_Unpack(o).grad() : THPVariable_Unpack(o);
-      if (of_parameters && !t.defined()) continue;
-      if (!device) device = t.device();
-      if (n >= cap || t.key_set().has(c10::DispatchKey::Python) || !t.is_cuda() || t.device() != *device ||
-          t.layout() != at::kStrided || !t.is_contiguous() || dtype_code(t) < 0)
-        Py_RETURN_NONE;
-      out[n++] = came8_grad_tensor{t.numel() > 0 ? t.data_ptr() : nullptr, t.numel(), dtype_code(t), 0};
-    }
-    return PyLong_FromLongLong(n);
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+  int of_parameters, scale;
+  double max_norm;
+  unsigned long long stream;
+  if (!PyArg_ParseTuple(args, "O!pdpK", &PyList_Type, &tensors, &of_parameters, &max_norm, &scale, &stream)) return nullptr;
+  std::vector<came8_grad_tensor> descs;
+  descs.reserve(size_t(PyList_GET_SIZE(tensors)));
+  at::Tensor first;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
+    PyObject* o = PyList_GET_ITEM(tensors, i);
+    if (!THPVariable_CheckExact(o) && !(of_parameters && THPVariable_Check(o))) Py_RETURN_NONE;
+    const at::Tensor& t = of_parameters ? THPVariable_Unpack(o).grad() : THPVariable_Unpack(o);
+    if (of_parameters && !t.defined()) continue;
+    if (!first.defined()) first = t;
+    if (t.key_set().has(c10::DispatchKey::Python) || !t.is_cuda() || t.device() != first.device() || t.layout() != at::kStrided ||
+        !t.is_contiguous() || dtype_code(t) < 0)
+      Py_RETURN_NONE;
+    descs.push_back(came8_grad_tensor{t.numel() > 0 ? t.data_ptr() : nullptr, t.numel(), dtype_code(t), 0});
   }
+  if (descs.empty()) Py_RETURN_FALSE;
+  c10::OptionalDeviceGuard guard(first.device());
+  const int32_t n = int32_t(descs.size());
+  const size_t bytes = entries.norm_size(n);
+  const at::Tensor ws = at::empty({int64_t(bytes / 4) + 2}, first.options().dtype(at::kFloat).requires_grad(false));
+  float* out = ws.data_ptr<float>() + bytes / 4;  // the two scalars
+  entry_check((scale ? entries.clip : entries.norm)(descs.data(), n, max_norm, out, out + 1, ws.data_ptr(), bytes,
+                                                    reinterpret_cast<void*>(stream)),
+              scale ? "came8_grad_clip" : "came8_grad_norm");
+  const int64_t at = int64_t(bytes / 4);
+  return Py_BuildValue("NN", THPVariable_Wrap(ws.select(0, at)), THPVariable_Wrap(ws.narrow(0, at + 1, 1)));
+  END_HANDLE_TH_ERRORS
 }
 
 // ------------------------------------------------------------------------------------------- gated feed-forward block
 // The block as an autograd node.  In Python its backward pass, which runs on a thread of the engine's, waits for the
 // interpreter's lock twice: 198 us of host time for 4 tokens of 256 and 512 forward and backward, 81 natively.
-struct FfnEntries {
-  decltype(&came8_gated_ffn_workspace_size) size = nullptr;
-  decltype(&came8_gated_ffn_forward) forward = nullptr;
-  decltype(&came8_gated_ffn_backward) backward = nullptr;
-  decltype(&came8_last_error) error = nullptr;
-} ffn;
-
-void ffn_check(int rc, const char* what) { TORCH_CHECK(rc == CAME8_OK, what, " failed (", rc, "): ", ffn.error()); }
-
 std::string dtype_name(const at::Tensor& t) {
   const char* known[3] = {"torch.float32", "torch.bfloat16", "torch.float16"};
   const int code = dtype_code(t);
@@ -353,7 +377,7 @@ FfnOperands ffn_operands(const at::Tensor& x, const at::Tensor& gate, const at::
 }
 
 at::Tensor ffn_workspace(const came8_ffn& f, bool backward, const at::Tensor& like, size_t* bytes) {
-  ffn_check(ffn.size(&f, backward ? 1 : 0, bytes), "came8_gated_ffn_workspace_size");
+  entry_check(entries.ffn_size(&f, backward ? 1 : 0, bytes), "came8_gated_ffn_workspace_size");
   return at::empty({int64_t(*bytes)}, like.options().dtype(at::kByte));
 }
 
@@ -369,7 +393,7 @@ std::pair<at::Tensor, at::Tensor> ffn_forward(const at::Tensor& x, const at::Ten
     size_t bytes = 0;
     const at::Tensor ws = ffn_workspace(o.f, false, x, &bytes);
     float* g = keep ? gu.data_ptr<float>() : nullptr;
-    ffn_check(ffn.forward(&o.f, o.x.data_ptr(), o.gate.data_ptr(), o.up.data_ptr(), o.down.data_ptr(), y.data_ptr(), g,
+    entry_check(entries.ffn_forward(&o.f, o.x.data_ptr(), o.gate.data_ptr(), o.up.data_ptr(), o.down.data_ptr(), y.data_ptr(), g,
                           keep ? g + T * F : nullptr, ws.data_ptr(), bytes, reinterpret_cast<void*>(stream)),
               "came8_gated_ffn_forward");
   }
@@ -405,7 +429,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
       const at::Tensor ws = ffn_workspace(o.f, true, dy, &bytes);
       const float* g = saved[4].data_ptr<float>();
       auto out = [&](size_t i) { return grads[i].defined() ? grads[i].data_ptr() : nullptr; };
-      ffn_check(ffn.backward(&o.f, o.x.data_ptr(), o.gate.data_ptr(), o.up.data_ptr(), o.down.data_ptr(), dy.data_ptr(), g, g + T * F,
+      entry_check(entries.ffn_backward(&o.f, o.x.data_ptr(), o.gate.data_ptr(), o.up.data_ptr(), o.down.data_ptr(), dy.data_ptr(), g, g + T * F,
                              out(0), out(1), out(2), out(3), ws.data_ptr(), bytes,
                              reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
                 "came8_gated_ffn_backward");
@@ -424,14 +448,19 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   }
 };
 
-// bind(size, forward, backward, last_error): the addresses of libcame8's entries
+// bind(*addresses): of libcame8's entries, in the order of Entries
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[4];
-  if (!PyArg_ParseTuple(args, "KKKK", &a[0], &a[1], &a[2], &a[3])) return nullptr;
-  ffn.size = reinterpret_cast<decltype(ffn.size)>(a[0]);
-  ffn.forward = reinterpret_cast<decltype(ffn.forward)>(a[1]);
-  ffn.backward = reinterpret_cast<decltype(ffn.backward)>(a[2]);
-  ffn.error = reinterpret_cast<decltype(ffn.error)>(a[3]);
+  unsigned long long a[8];
+  if (!PyArg_ParseTuple(args, "KKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7])) return nullptr;
+  auto take = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(a[i]); };
+  take(entries.error, 0);
+  take(entries.adamw, 1);
+  take(entries.norm_size, 2);
+  take(entries.norm, 3);
+  take(entries.clip, 4);
+  take(entries.ffn_size, 5);
+  take(entries.ffn_forward, 6);
+  take(entries.ffn_backward, 7);
   Py_RETURN_NONE;
 }
 
@@ -458,7 +487,6 @@ PyObject* gated_ffn(PyObject*, PyObject* args) {
                     gate.sizes(), ", ", up.sizes(), ", ", down.sizes());
   TORCH_CHECK_VALUE(x.size(-1) == gate.size(1) && down.size(1) == gate.size(0) && gate.numel() > 0 && down.numel() > 0,
                     "gated_ffn: widths do not match or are empty: ", x.sizes(), ", ", gate.sizes(), ", ", down.sizes());
-  TORCH_CHECK(ffn.forward != nullptr, "came8_host: bind() first");
   pybind11::gil_scoped_release no_gil;
   const int64_t tokens = x.numel() / x.size(-1);
   const at::Tensor rows = x.dim() == 2 ? x : x.reshape({tokens, x.size(-1)});
@@ -478,9 +506,9 @@ PyObject* gated_ffn(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "descriptors of a param group's tensors"},
-                         {"gather_adamw", gather_adamw, METH_VARARGS, "AdamW descriptors of a param group's tensors"},
-                         {"gather_grads", gather_grads, METH_VARARGS, "descriptors of a list of gradients"},
-                         {"bind", bind, METH_VARARGS, "the library's entries for gated_ffn"},
+                         {"adamw_step", adamw_step, METH_VARARGS, "one AdamW step of a param group"},
+                         {"grad_norm", grad_norm, METH_VARARGS, "the norm of gradients, and the clip by it"},
+                         {"bind", bind, METH_VARARGS, "libcame8's entries"},
                          {"gated_ffn", gated_ffn, METH_VARARGS, "the gated feed-forward block"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "came8_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -6,8 +6,6 @@ in place.  No host synchronisation: the norm is a device tensor.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -41,30 +39,20 @@ def _contiguous(tensors: list, what: str):
 def _reduce(tensors: list, max_norm: float | None, scale: bool, what: str, of_parameters: bool = False):
     """(norm, factor): device scalars of one call over the tensors, or the parameters' gradients; with `scale` those are
     multiplied in place.  None where no parameter has a gradient."""
-    lib = _lib.load()
-    descs = (_lib.Came8GradTensor * max(len(tensors), 1))()
-    copies = []
-    n = _lib.host().gather_grads(tensors, ctypes.addressof(descs), len(tensors), of_parameters)
-    if n is None:
+    device = next((t.device for t in tensors if not of_parameters or t.grad is not None), None)
+    if device is None:
+        return None
+    stream = torch.cuda.current_stream(device).cuda_stream if device.type == "cuda" else 0
+    host = _lib.host()
+    found = host.grad_norm(tensors, of_parameters, float(max_norm or 0.0), scale, stream)
+    if found is None:  # strided tensors, or ones that are refused
         if of_parameters:
             tensors = [g for g in [p.grad for p in tensors] if g is not None]
         tensors, copies = _contiguous(tensors, what)
-        n = len(tensors)
-        for d, t in zip(descs, tensors):
-            d.data, d.numel, d.dtype = (t.data_ptr() if t.numel() else None), t.numel(), _DTYPE_CODE[t.dtype]
-    if n == 0:
-        return None
-    device = tensors[0].device if copies or not of_parameters else next(p.grad for p in tensors if p.grad is not None).device
-    with torch.cuda.device(device):
-        size = lib.came8_grad_norm_workspace_size(n)
-        ws = torch.empty(size // 4 + 2, dtype=torch.float32, device=device)  # and the two scalars
-        at = ws.data_ptr()
-        _lib.check((lib.came8_grad_clip if scale else lib.came8_grad_norm)(
-            descs, n, float(max_norm or 0.0), at + size, at + size + 4, at, size,
-            torch.cuda.current_stream(device).cuda_stream), "came8_grad_clip" if scale else "came8_grad_norm")
+        found = host.grad_norm([t.detach() for t in tensors], False, float(max_norm or 0.0), scale, stream)
         for t, c in copies if scale else ():
             t.copy_(c)
-    return ws[-2], ws[-1:]
+    return found
 
 
 @torch.no_grad()
