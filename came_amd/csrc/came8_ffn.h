@@ -137,14 +137,19 @@ __host__ __device__ constexpr int swz(int r) { return (r >> 3 & 1) | ((r ^ r >> 
 // Rows: a thread loads chunk t % 8 of every NT / 8-th row from row t / 8 on; a chunk at or past k = K lies nowhere and gives
 // zeros (a chunk that K cuts holds zeros in memory).  Columns: a thread loads kLoads successive k of kVec rows, and k past K
 // lie past the end.  HALF > 0: rows taken in turns of HALF from two matrices (the gate's and the up projection's weights);
-// loads i of a thread go to the one and the other in turn.
-template <typename T, int R, int NT, bool ROWS, int HALF = 0>
+// loads i of a thread go to the one and the other in turn.  ODD: 16-bit rows an odd number of elements apart, every other
+// one of which starts in the middle of a word: the words that hold a chunk are loaded, five of them, and shifted on their way
+// to LDS, where a chunk that K cuts loses what is of the next row.
+template <typename T, int R, int NT, bool ROWS, int HALF = 0, bool ODD = false>
 struct Stage {
   static constexpr int kElem = int(sizeof(typename T::storage));
   static constexpr int kVec = kChunkBytes / kElem;        // elements of a chunk
   static constexpr int kLoads = R * 8 / NT;               // 16-byte loads a thread
   static constexpr int kStep = NT / 8;                    // rows: from a load's to the next
+  static_assert(!ODD || (ROWS && HALF == 0 && kElem == 2 && kStep % 2 == 0), "");
   u32x4 v[kLoads];
+  uint32_t fifth[ODD ? kLoads : 1], shift;  // ODD: 2 where the thread's rows start in the middle of a word
+  int odd_left;
 
   // left: K less the view's first k
   __device__ __forceinline__ void fetch(const View& a, const View& a1, int left) {
@@ -158,7 +163,15 @@ struct Stage {
       const bool out = int(t & 7) * kVec >= left;
       const Buffer buf = a.buffer();
       const uint32_t off = out ? kNowhere : (t >> 3) * a.ld + (t & 7) * kChunkBytes;
-      if constexpr (HALF == 0) {
+      if constexpr (ODD) {
+        shift = off & 2;
+        odd_left = left;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          v[i] = __builtin_amdgcn_raw_buffer_load_b128(buf, off - shift + i * kStep * a.ld, 0, 0);
+          fifth[i] = __builtin_amdgcn_raw_buffer_load_b32(buf, off - shift + i * kStep * a.ld + 16, 0, 0);
+        }
+      } else if constexpr (HALF == 0) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(buf, off + i * kStep * a.ld, 0, 0);
       } else {
@@ -180,6 +193,20 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = HALF == 0 ? i * kStep : i / 2 * 2 * kStep + (i & 1) * HALF;
+        if constexpr (ODD) {
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_alignbyte(e < 3 ? v[i][e + 1] : fifth[i], v[i][e], shift);
+          if (odd_left < (c + 1) * kVec) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = c * kVec + 2 * e;
+              w[e] = k + 1 < odd_left ? w[e] : k < odd_left ? w[e] & 0xffffu : 0u;
+            }
+          }
+          *reinterpret_cast<u32x4*>(lds + (r * kRowBytes + ((c ^ swz(r)) ^ swz(row)) * kChunkBytes) + row * kRowBytes) = w;
+          continue;
+        }
         *reinterpret_cast<u32x4*>(lds + (r * kRowBytes + ((c ^ swz(r)) ^ swz(row)) * kChunkBytes) + row * kRowBytes) = v[i];
       }
     } else if constexpr (kElem == 4) {
@@ -301,7 +328,7 @@ __device__ __forceinline__ void interleave() {
 // the operands of step t + 1 go from registers to the other LDS buffer, and those of step t + 2 are loaded.  The step's one
 // barrier stands before the last phase, whose reads are the first of step t + 1.  So neither LDS reads nor global loads are
 // waited for at the barrier.  Steps past the end load zeros.
-template <typename T, int BM, int BN, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
+template <typename T, int BM, int BN, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD = false>
 __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) {
   using S = typename T::storage;
   constexpr int kElem = int(sizeof(S));
@@ -332,7 +359,7 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   // of 64 and 128, 516 us with one and 492 with two, 32 tokens of 4096 and 11008 in bf16 80 and 75 us.
   constexpr int D = BM < 256 ? 2 : 1;
   Stage<T, BM, NT, AROWS> sa[D];
-  Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0> sb[D];
+  Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0, ODD> sb[D];
   const int steps = (args.K + BK - 1) / BK;
   const int every = steps * args.nseg;
   int ahead = int(int64_t(every) * split / args.splits);  // the step that is fetched next
@@ -531,10 +558,10 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   }
 }
 
-template <typename T, int B, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI>
+template <typename T, int B, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD>
 __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmArgs args) {
   __shared__ __attribute__((aligned(16))) char lds[4 * B * kRowBytes];
-  product<T, B, B, WAVES_N, AROWS, BROWS, EPI>(args, int(blockIdx.x), lds);
+  product<T, B, B, WAVES_N, AROWS, BROWS, EPI, ODD>(args, int(blockIdx.x), lds);
 }
 
 // The products that only wait for dg, du and h: dx and the weights' gradients, one launch, the longest sums first.  The last
