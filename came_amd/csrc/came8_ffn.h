@@ -241,6 +241,65 @@ struct Stage {
   }
 };
 
+// fp32 values as three bf16 ones, each the rounding of what the ones before leave: their sum is the value to 2^-24 of it.
+// (Infinities and NaN, and what rounds to infinity, are in the first alone.)
+struct Parts {
+  uint32_t w[3];  // of two values, packed
+};
+__device__ __forceinline__ Parts parts_of(float x, float y) {
+  Parts p;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    p.w[i] = uint32_t(BF16::store(x)) | uint32_t(BF16::store(y)) << 16;
+    x -= BF16::elem(&p.w[i], 0);
+    y -= BF16::elem(&p.w[i], 1);
+    x = fabsf(x) <= 0x1p127f ? x : 0.0f;
+    y = fabsf(y) <= 0x1p127f ? y : 0.0f;
+  }
+  return p;
+}
+
+// Rows of three parts in LDS: 64 bytes each, 32 values of k.  Chunk c of row r lies at c ^ part_swz(r), so that the lanes of a
+// read (see swz) touch all banks once.
+constexpr int kPartBytes = 64, kPartRow = 3 * kPartBytes;
+__host__ __device__ constexpr int part_swz(int r) { return (4 - (r >> 2 & 3)) & 3; }
+
+// Stage::put for rows of parts
+template <int R, int NT, bool ROWS, int HALF>
+__device__ __forceinline__ void put_parts(const Stage<F32, R, NT, ROWS, HALF>& s, char* lds) {
+  using St = Stage<F32, R, NT, ROWS, HALF>;
+  const int t = int(threadIdx.x);
+  if constexpr (ROWS) {
+    constexpr int H = HALF == 0 ? St::kStep : HALF;
+    const int c = t & 7, r = HALF == 0 ? t >> 3 : (t >> 3) / H * 2 * H + (t >> 3) % H;
+#pragma unroll
+    for (int i = 0; i < St::kLoads; ++i) {
+      const int row = r + (HALF == 0 ? i * St::kStep : i / 2 * 2 * St::kStep + (i & 1) * HALF);
+      const Parts a = parts_of(__uint_as_float(s.v[i][0]), __uint_as_float(s.v[i][1]));
+      const Parts b = parts_of(__uint_as_float(s.v[i][2]), __uint_as_float(s.v[i][3]));
+      char* at = lds + row * kPartRow + ((c >> 1) ^ part_swz(row)) * kChunkBytes + (c & 1) * 8;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(at + p * kPartBytes) = u32x2{a.w[p], b.w[p]};
+    }
+  } else {
+    const int r = (t % (R / 4)) * 4, k = (t / (R / 4)) * St::kLoads;  // first row, first k
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      char* at = lds + (r + e) * kPartRow + ((k >> 3) ^ part_swz(r + e)) * kChunkBytes + (k & 7) * 2;
+      const Parts a = parts_of(__uint_as_float(s.v[0][e]), __uint_as_float(s.v[1][e]));
+      if constexpr (St::kLoads == 4) {
+        const Parts b = parts_of(__uint_as_float(s.v[2][e]), __uint_as_float(s.v[3][e]));
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(at + p * kPartBytes) = u32x2{a.w[p], b.w[p]};
+      } else {
+        static_assert(St::kLoads == 2, "");
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t*>(at + p * kPartBytes) = a.w[p];
+      }
+    }
+  }
+}
+
 // V consecutive values to a row of N elements at any address, those past N left out (unless the row is padded past it)
 template <typename T>
 __device__ __forceinline__ void store4(void* row, int n, int N, const float (&x)[4]) {
@@ -320,6 +379,14 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
+// The tiles: B by B on 2 by WAVES_N wavefronts, and for fp32 at B = 256 ("parts") 256 by 128 on 4 by 2.
+template <typename T, int B, int WAVES_N>
+struct Tile {
+  static constexpr bool kParts = std::is_same<T, F32>::value && B == 256;
+  static constexpr int kWavesM = kParts ? 4 : 2, kWidth = kParts ? 128 : B, kGroup = kWavesM * WAVES_N * kWave;
+  static constexpr int kBytes = (B + kWidth) * (kParts ? kPartRow : kRowBytes);  // of a step's operands
+};
+
 // Workgroups of 2 by WAVES_N wavefronts on a tile of BM by BN; an accumulator lane holds 4 consecutive columns of a row.
 // kGate: the tile's BN rows of weights are, in turns of half a wavefront's, gate and up projection, so that a wavefront
 // holds both values of its columns of h.
@@ -328,14 +395,20 @@ __device__ __forceinline__ void interleave() {
 // the operands of step t + 1 go from registers to the other LDS buffer, and those of step t + 2 are loaded.  The step's one
 // barrier stands before the last phase, whose reads are the first of step t + 1.  So neither LDS reads nor global loads are
 // waited for at the barrier.  Steps past the end load zeros.
-template <typename T, int BM, int BN, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD = false>
+//
+// fp32 at BM = 256: the matrix instructions of fp32 run at a sixteenth of bf16's rate.  The operands are taken apart into three
+// bf16 parts on their way to LDS, and the six products of parts down to 2^-16 of the largest, summed in fp32, are a product
+// of fp32's accuracy at a sixth of bf16's rate: 2048 tokens of 4096 and 11008 forward and backward 9.8 ms (170
+// TFLOP/s) against 12.4.
+template <typename T, int BM, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD = false>
 __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) {
   using S = typename T::storage;
+  using Shape = Tile<T, BM, WAVES_N>;
   constexpr int kElem = int(sizeof(S));
   constexpr int BK = kRowBytes / kElem;
-  constexpr int NT = 2 * WAVES_N * kWave;
-  constexpr int WM = BM / 2, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
-  constexpr int kTileBytes = (BM + BN) * kRowBytes;
+  constexpr int BN = Shape::kWidth, WAVES_M = Shape::kWavesM, NT = Shape::kGroup;
+  constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 16, FN = WN / 16;
+  constexpr int kTileBytes = Shape::kBytes;
 
   // Workgroups go to the 8 XCDs in turn: each XCD gets a run of successive tiles, 8 tiles of rows by the columns.
   int tm, tn, split;
@@ -353,7 +426,7 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   }
   const int m0 = tm * BM, n0 = tn * (EPI == kGate ? BN / 2 : BN);
   const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave % WAVES_M, wn = wave / WAVES_M;
 
   // Steps loaded ahead; step t is in registers t % D.  Two where registers allow: 1021 tokens of 1024 and 2731 in fp32, tiles
   // of 64 and 128, 516 us with one and 492 with two, 32 tokens of 4096 and 11008 in bf16 80 and 75 us.
@@ -406,88 +479,119 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
       left = turn ? args.K : left;
     }
   };
-  auto put = [&](int t, int slot) __attribute__((always_inline)) {
-    char* to = lds + (t & 1) * kTileBytes;
-    sa[slot].put(to);
-    sb[slot].put(to + BM * kRowBytes);
-  };
-  // Fragment i of half s: row 16 i + lane % 16 of the wavefront's, chunk 4 s + lane / 16, at place
-  // (lane / 16) ^ swz(the wavefront's first row + lane % 16) ^ 4 s ^ swz(16 i), one of four that differ by 2 v.
-  const int fr = lane % 16;
-  uint32_t pa[4], pb[4];
-#pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    pa[v] = uint32_t((wm * WM + fr) * kRowBytes + (lane / 16 ^ swz(wm * (WM % 64) + fr) ^ (2 * v)) * kChunkBytes);
-    pb[v] = uint32_t((BM + wn * WN + fr) * kRowBytes + (lane / 16 ^ swz(wn * (WN % 64) + fr) ^ (2 * v)) * kChunkBytes);
-  }
-  u32x4 lo[FM / 2], hi[FM / 2], fb[2][FN];
-  auto read_a = [&](u32x4(&f)[FM / 2], int t, int s, int i0) __attribute__((always_inline)) {
-    const char* a = lds + (t & 1) * kTileBytes;
-#pragma unroll
-    for (int i = 0; i < FM / 2; ++i)
-      f[i] = *reinterpret_cast<const u32x4*>(a + pa[(4 * s ^ swz(16 * (i0 + i))) / 2] + (i0 + i) * 16 * kRowBytes);
-  };
-  auto read_b = [&](int t, int s, int j0) __attribute__((always_inline)) {
-    const char* b = lds + (t & 1) * kTileBytes;
-#pragma unroll
-    for (int j = j0; j < j0 + FN / 2; ++j)
-      fb[s][j] = *reinterpret_cast<const u32x4*>(b + pb[(4 * s ^ swz(16 * j)) / 2] + j * 16 * kRowBytes);
-  };
-
   f32x4 acc[FM][FN] = {};
-  auto multiply = [&](const u32x4(&f)[FM / 2], int s, int i0) __attribute__((always_inline)) {
+  if constexpr (Shape::kParts) {
+    fetch(0);
+    for (int t = 0; t < total; ++t) {
+      char* at = lds + (t & 1) * kTileBytes;
+      put_parts(sa[0], at);
+      put_parts(sb[0], at + BM * kPartRow);
+      fetch(0);
+      __syncthreads();  // the other buffer's last reads are behind every wavefront that has come here
+      const int r = lane % 16, place = r * kPartRow + (lane / 16 ^ part_swz(r)) * kChunkBytes;
+      const char* pa = at + wm * WM * kPartRow + place;
+      const char* pb = at + (BM + wn * WN) * kPartRow + place;
+      u32x4 fb[3][FN];
 #pragma unroll
-    for (int i = 0; i < FM / 2; ++i)
+      for (int p = 0; p < 3; ++p)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i0 + i][j] = mfma_chunk<T>(fb[s][j], f[i], acc[i0 + i][j]);
-  };
-  constexpr int kProducts = FM / 2 * FN * (kElem == 4 ? 4 : 1);  // of a phase
-  // Step t + 2 is loaded as soon as step t + 1 has left the registers, a whole step before its use (8192 tokens forward and
-  // backward 6555 us with loads half a step ahead, 6452 so); with columns, whose way to LDS takes registers, a quarter later.
-  constexpr bool kEarly = AROWS && BROWS;
-  fetch(0);
-  put(0, 0);
+        for (int j = 0; j < FN; ++j) fb[p][j] = *reinterpret_cast<const u32x4*>(pb + j * 16 * kPartRow + p * kPartBytes);
 #pragma unroll
-  for (int d = 1; d <= D; ++d) fetch(d % D);
-  __syncthreads();
-  read_a(lo, 0, 0, 0);
-  read_b(0, 0, 0);
-  read_b(0, 0, FN / 2);
-  auto step = [&](int t, int slot) __attribute__((always_inline)) {  // slot: of step t + 1
-    read_a(hi, t, 0, FM / 2);
-    read_b(t, 1, 0);
-    read_b(t, 1, FN / 2);
-    multiply(lo, 0, 0);
-    interleave<kDsRead, FM / 2 + FN, kProducts>();
-    read_a(lo, t, 1, 0);
-    put(t + 1, slot);
-    if constexpr (kEarly) fetch(slot);
-    multiply(hi, 0, FM / 2);
-    interleave<kDsRead | kDsWrite | kVmemRead, FM / 2 + FM + FN + (kEarly ? 8 : 0), kProducts>();
-    read_a(hi, t, 1, FM / 2);
-    if constexpr (!kEarly) fetch(slot);
-    multiply(lo, 1, 0);
-    interleave<kDsRead | kVmemRead, FM / 2 + (kEarly ? 0 : 8), kProducts>();
-    // every wavefront has read its last of step t, whose place the next put takes, and written its part of step t + 1
+      for (int i = 0; i < FM; ++i) {
+        u32x4 fa[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) fa[p] = *reinterpret_cast<const u32x4*>(pa + i * 16 * kPartRow + p * kPartBytes);
+#pragma unroll
+        for (int p = 2; p >= 0; --p)  // the smallest products first
+#pragma unroll
+          for (int q = 2 - p; q >= 0; --q)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma_chunk<BF16>(fb[q][j], fa[p], acc[i][j]);
+      }
+    }
+  } else {
+    auto put = [&](int t, int slot) __attribute__((always_inline)) {
+      char* to = lds + (t & 1) * kTileBytes;
+      sa[slot].put(to);
+      sb[slot].put(to + BM * kRowBytes);
+    };
+    // Fragment i of half s: row 16 i + lane % 16 of the wavefront's, chunk 4 s + lane / 16, at place
+    // (lane / 16) ^ swz(the wavefront's first row + lane % 16) ^ 4 s ^ swz(16 i), one of four that differ by 2 v.
+    const int fr = lane % 16;
+    uint32_t pa[4], pb[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      pa[v] = uint32_t((wm * WM + fr) * kRowBytes + (lane / 16 ^ swz(wm * (WM % 64) + fr) ^ (2 * v)) * kChunkBytes);
+      pb[v] = uint32_t((BM + wn * WN + fr) * kRowBytes + (lane / 16 ^ swz(wn * (WN % 64) + fr) ^ (2 * v)) * kChunkBytes);
+    }
+    u32x4 lo[FM / 2], hi[FM / 2], fb[2][FN];
+    auto read_a = [&](u32x4(&f)[FM / 2], int t, int s, int i0) __attribute__((always_inline)) {
+      const char* a = lds + (t & 1) * kTileBytes;
+#pragma unroll
+      for (int i = 0; i < FM / 2; ++i)
+        f[i] = *reinterpret_cast<const u32x4*>(a + pa[(4 * s ^ swz(16 * (i0 + i))) / 2] + (i0 + i) * 16 * kRowBytes);
+    };
+    auto read_b = [&](int t, int s, int j0) __attribute__((always_inline)) {
+      const char* b = lds + (t & 1) * kTileBytes;
+#pragma unroll
+      for (int j = j0; j < j0 + FN / 2; ++j)
+        fb[s][j] = *reinterpret_cast<const u32x4*>(b + pb[(4 * s ^ swz(16 * j)) / 2] + j * 16 * kRowBytes);
+    };
+
+    auto multiply = [&](const u32x4(&f)[FM / 2], int s, int i0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < FM / 2; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i0 + i][j] = mfma_chunk<T>(fb[s][j], f[i], acc[i0 + i][j]);
+    };
+    constexpr int kProducts = FM / 2 * FN * (kElem == 4 ? 4 : 1);  // of a phase
+    // Step t + 2 is loaded as soon as step t + 1 has left the registers, a whole step before its use (8192 tokens forward and
+    // backward 6555 us with loads half a step ahead, 6452 so); with columns, whose way to LDS takes registers, a quarter later.
+    constexpr bool kEarly = AROWS && BROWS;
+    fetch(0);
+    put(0, 0);
+#pragma unroll
+    for (int d = 1; d <= D; ++d) fetch(d % D);
     __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-    read_a(lo, t + 1, 0, 0);
-    read_b(t + 1, 0, 0);
-    read_b(t + 1, 0, FN / 2);
-    multiply(hi, 1, FM / 2);
-    interleave<kDsRead, FM / 2 + FN, kProducts>();
-  };
-  for (int t = 0; t < total; t += D)
+    read_a(lo, 0, 0, 0);
+    read_b(0, 0, 0);
+    read_b(0, 0, FN / 2);
+    auto step = [&](int t, int slot) __attribute__((always_inline)) {  // slot: of step t + 1
+      read_a(hi, t, 0, FM / 2);
+      read_b(t, 1, 0);
+      read_b(t, 1, FN / 2);
+      multiply(lo, 0, 0);
+      interleave<kDsRead, FM / 2 + FN, kProducts>();
+      read_a(lo, t, 1, 0);
+      put(t + 1, slot);
+      if constexpr (kEarly) fetch(slot);
+      multiply(hi, 0, FM / 2);
+      interleave<kDsRead | kDsWrite | kVmemRead, FM / 2 + FM + FN + (kEarly ? 8 : 0), kProducts>();
+      read_a(hi, t, 1, FM / 2);
+      if constexpr (!kEarly) fetch(slot);
+      multiply(lo, 1, 0);
+      interleave<kDsRead | kVmemRead, FM / 2 + (kEarly ? 0 : 8), kProducts>();
+      // every wavefront has read its last of step t, whose place the next put takes, and written its part of step t + 1
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      read_a(lo, t + 1, 0, 0);
+      read_b(t + 1, 0, 0);
+      read_b(t + 1, 0, FN / 2);
+      multiply(hi, 1, FM / 2);
+      interleave<kDsRead, FM / 2 + FN, kProducts>();
+    };
+    for (int t = 0; t < total; t += D)
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-      if (d == 0 || t + d < total) step(t + d, (d + 1) % D);
+      for (int d = 0; d < D; ++d)
+        if (d == 0 || t + d < total) step(t + d, (d + 1) % D);
+  }
 
   // acc[i][j][e]: row 16 i + lane % 16 of the wavefront's, column 16 j + 4 (lane / 16) + e.  Up to 64 rows at a time go
   // through the wavefront's own part of LDS, so that lanes of successive columns read and write memory together; chunk c of
   // row r lies at c ^ r.  Several rounds' reads of g and u are in flight before the first is used.
   constexpr int kPart = FM < 4 ? FM : 4;
   constexpr int kChunks = WN / 4;
-  static_assert(2 * WAVES_N * kPart * 16 * WN * 4 <= 2 * kTileBytes, "");
+  static_assert(WAVES_M * WAVES_N * kPart * 16 * WN * 4 <= 2 * kTileBytes, "");
   char* mine = lds + wave * (kPart * 16 * WN * 4);
   constexpr int kCols = EPI == kGate ? WN / 2 : WN;  // of the output
   constexpr int kLanes = kCols / 4, kRows = kWave / kLanes, kRounds = kPart * 16 / kRows;
@@ -559,9 +663,9 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
 }
 
 template <typename T, int B, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD>
-__global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_gemm(const GemmArgs args) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * B * kRowBytes];
-  product<T, B, B, WAVES_N, AROWS, BROWS, EPI, ODD>(args, int(blockIdx.x), lds);
+__global__ __launch_bounds__((Tile<T, B, WAVES_N>::kGroup), 2) void k_ffn_gemm(const GemmArgs args) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * Tile<T, B, WAVES_N>::kBytes];
+  product<T, B, WAVES_N, AROWS, BROWS, EPI, ODD>(args, int(blockIdx.x), lds);
 }
 
 // The products that only wait for dg, du and h: dx and the weights' gradients, one launch, the longest sums first.  The last
@@ -572,14 +676,14 @@ struct GradArgs {
   int32_t first[4];  // workgroups before each dw, and all
 };
 template <typename T, int B, int WAVES_N>
-__global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_ffn_grads(const GradArgs args) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * B * kRowBytes];
+__global__ __launch_bounds__((Tile<T, B, WAVES_N>::kGroup), 2) void k_ffn_grads(const GradArgs args) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * Tile<T, B, WAVES_N>::kBytes];
   const int b = int(blockIdx.x);
   if (b < args.first[0]) {
-    product<T, B, B, WAVES_N, true, false, kStore>(args.dx, b, lds);
+    product<T, B, WAVES_N, true, false, kStore>(args.dx, b, lds);
   } else {
     const int k = (b >= args.first[1]) + (b >= args.first[2]);
-    product<T, B, B, WAVES_N, false, false, kStore>(args.dw[k], b - args.first[k], lds);
+    product<T, B, WAVES_N, false, false, kStore>(args.dw[k], b - args.first[k], lds);
   }
 }
 

@@ -29,7 +29,8 @@ bool ragged(const came8_ffn* f, int64_t cols, int64_t ld) {
   return f->dtype == CAME8_F32 ? cols % 4 != 0 : cols % 8 != 0 || ld % 2 != 0;
 }
 
-// How a product is cut: tiles of `tile` by `tile` (gate and up: half as many columns of h), `splits` workgroups a tile.
+// How a product is cut: tiles of `tile` by `tile` (fp32 at 256: 128 wide; gate and up: half as many columns of h), `splits`
+// workgroups a tile.
 struct Cut {
   int tile = 0, splits = 1;
 };
@@ -38,13 +39,14 @@ struct Size {
   int nseg;
 };
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int width_of(bool fp32, int tile) { return fp32 && tile == 256 ? 128 : tile; }
 
 // What a tile size runs at: workgroups at once on the GPU, and a step of k (128 bytes) of one, microseconds.
 struct Speed {
   int tile, at_once;
   double half, full;  // 16-bit types, fp32
 };
-constexpr Speed kSpeeds[] = {{256, 256, 1.87, 0.0}, {128, 512, 1.22, 3.8}, {64, 1024, 1.19, 1.9}};
+constexpr Speed kSpeeds[] = {{256, 256, 1.87, 3.3}, {128, 512, 1.22, 3.8}, {64, 1024, 1.19, 1.9}};
 constexpr int kSplitSteps = 4;   // a share of a sum has at least these steps
 constexpr int kMaxSplits = 16;
 constexpr double kJoinBytes = 4e6;  // a microsecond of k_ffn_join: shares written and read
@@ -58,8 +60,8 @@ Cut cut_of(const came8_ffn* f, const Size& z, bool gate) {
   double least = 1e300;
   for (const Speed& v : kSpeeds) {
     const double us = f->dtype == CAME8_F32 ? v.full : v.half;
-    if (us == 0.0) continue;
-    const int64_t tiles = ceil_div(z.M, v.tile) * ceil_div(z.N, gate ? v.tile / 2 : v.tile), steps = steps_of(f, z);
+    const int width = width_of(f->dtype == CAME8_F32, v.tile);
+    const int64_t tiles = ceil_div(z.M, v.tile) * ceil_div(z.N, gate ? width / 2 : width), steps = steps_of(f, z);
     for (int s = 1; s <= kMaxSplits; ++s) {
       if (s > 1 && steps / s < kSplitSteps) break;
       const double t = double(ceil_div(tiles * s, v.at_once)) * (double(ceil_div(steps, s)) + 3.0) * us +
@@ -80,11 +82,11 @@ void cut_together(const came8_ffn* f, const Size* z, int count, Cut* cuts) {
   double least = 1e300;
   for (const Speed& v : kSpeeds) {
     const double us = f->dtype == CAME8_F32 ? v.full : v.half;
-    if (us == 0.0) continue;
+    const int width = width_of(f->dtype == CAME8_F32, v.tile);
     double work = 0.0, join = 0.0;
     int64_t longest = 0;
     for (int i = 0; i < count; ++i)
-      work += double(ceil_div(z[i].M, v.tile) * ceil_div(z[i].N, v.tile)) * (double(steps_of(f, z[i])) + 3.0);
+      work += double(ceil_div(z[i].M, v.tile) * ceil_div(z[i].N, width)) * (double(steps_of(f, z[i])) + 3.0);
     const int64_t share = std::max<int64_t>(2 * kSplitSteps, int64_t(work / v.at_once));
     int splits[4];
     for (int i = 0; i < count; ++i) {
@@ -204,8 +206,9 @@ int check_pointers(const char* what, std::initializer_list<const void*> ps) {
   return CAME8_OK;
 }
 
+template <typename T>
 void tile(GemmArgs& a, const Cut& c, bool gate) {
-  const int cols = gate ? c.tile / 2 : c.tile;
+  const int width = width_of(std::is_same<T, F32>::value, c.tile), cols = gate ? width / 2 : width;
   a.tiles_m = int32_t(ceil_div(a.M, c.tile));
   a.tiles_n = int32_t(ceil_div(a.N, cols));
   a.splits = c.splits;
@@ -215,15 +218,15 @@ unsigned join_groups(const GemmArgs& a) {
   return unsigned(std::min<int64_t>(ceil_div(int64_t(a.M) * ((a.N + 3) / 4), kThreads), 1 << 14));
 }
 
-// One product over its tiles.  256 by 256 only for 16-bit types: fp32 products are bound by the matrix units at any size.
-// odd: the second operand's rows are an odd number of elements apart (shifted_in_place).
+// One product over its tiles.  odd: the second operand's rows are an odd number of elements apart (shifted_in_place).
 template <typename T, bool BROWS, Epilogue EPI>
 void launch(GemmArgs a, const Cut& c, float* part, hipStream_t stream, bool odd = false) {
-  tile(a, c, EPI == kGate);
+  tile<T>(a, c, EPI == kGate);
   a.part = c.splits > 1 ? part : nullptr;
   const dim3 grid(unsigned(a.tiles_m) * unsigned(a.tiles_n) * unsigned(a.splits));
+  constexpr int kWide = std::is_same<T, F32>::value ? 2 : 4;
+  if (c.tile == 256) hipLaunchKernelGGL((k_ffn_gemm<T, 256, kWide, true, BROWS, EPI, false>), grid, dim3(512), 0, stream, a);
   if constexpr (!std::is_same<T, F32>::value) {
-    if (c.tile == 256) hipLaunchKernelGGL((k_ffn_gemm<T, 256, 4, true, BROWS, EPI, false>), grid, dim3(512), 0, stream, a);
     if constexpr (BROWS && EPI == kStore) {
       if (c.tile == 128 && odd) hipLaunchKernelGGL((k_ffn_gemm<T, 128, 2, true, true, kStore, true>), grid, dim3(256), 0, stream, a);
       if (c.tile == 64 && odd) hipLaunchKernelGGL((k_ffn_gemm<T, 64, 2, true, true, kStore, true>), grid, dim3(256), 0, stream, a);
@@ -298,7 +301,7 @@ void backward(const came8_ffn* f, const void* x, const void* wg, const void* wu,
     g.nseg = std::max(g.nseg, 1);
     g.M = int32_t(M), g.N = int32_t(N), g.K = int32_t(K);
     g.out = out, g.ldo = N;
-    tile(g, cut, false);
+    tile<T>(g, cut, false);
     if (cut.splits > 1) {
       g.part = part;
       part += part_floats(cut, M, N);
@@ -324,9 +327,8 @@ void backward(const came8_ffn* f, const void* x, const void* wg, const void* wu,
   for (int k = count; k < 4; ++k) r.first[k] = groups;
   if (groups == 0) return;
   const int t = c.grads[0].tile;
-  if constexpr (!std::is_same<T, F32>::value) {
-    if (t == 256) hipLaunchKernelGGL((k_ffn_grads<T, 256, 4>), dim3(unsigned(groups)), dim3(512), 0, stream, r);
-  }
+  constexpr int kWide = std::is_same<T, F32>::value ? 2 : 4;
+  if (t == 256) hipLaunchKernelGGL((k_ffn_grads<T, 256, kWide>), dim3(unsigned(groups)), dim3(512), 0, stream, r);
   if (t == 128) hipLaunchKernelGGL((k_ffn_grads<T, 128, 2>), dim3(unsigned(groups)), dim3(256), 0, stream, r);
   if (t == 64) hipLaunchKernelGGL((k_ffn_grads<T, 64, 2>), dim3(unsigned(groups)), dim3(256), 0, stream, r);
   unsigned most = 0;

@@ -83,6 +83,25 @@ def test_several_tiles(shape, dtype):
     _check_all(ops, dy, "silu")
 
 
+def test_large_fp32_products_keep_fp32_accuracy():
+    """fp32 products of many tiles take their operands apart: rows of magnitudes from 1e-8 to 1e8 each keep float32's accuracy
+    against their own, and a row's infinity, NaN or near-largest value stays in that row."""
+    from came_amd import gated_ffn
+    ops, dy = _operands(2100, 520, 1500, 600, F32, seed=12)
+    ops[0] = ops[0] * torch.pow(10.0, torch.linspace(-8, 8, 2100, device="cuda"))[:, None]
+    dy = dy * torch.pow(10.0, torch.linspace(8, -8, 2100, device="cuda"))[:, None]
+    _check_all(ops, dy, "gelu_tanh")
+    ops, dy = _operands(2100, 520, 1500, 600, F32, seed=13)
+    with torch.no_grad():
+        want = gated_ffn(*ops)
+        bad = ops[0].clone()
+        bad[5, 519], bad[700, 3], bad[2099, 0] = float("inf"), float("nan"), 3.4e38
+        got = gated_ffn(bad, *ops[1:])
+    rows = torch.ones(2100, dtype=torch.bool, device="cuda")
+    rows[[5, 700, 2099]] = False
+    assert torch.equal(got[rows], want[rows]) and not torch.isfinite(got[[5, 700]]).any()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("T", [1, 9, 140])
 def test_operands_where_they_lie(T, dtype):
