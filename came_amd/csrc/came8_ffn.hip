@@ -48,7 +48,7 @@ struct Speed {
 };
 constexpr Speed kSpeeds[] = {{256, 256, 1.87, 3.3}, {128, 512, 1.22, 3.8}, {64, 1024, 1.19, 1.9}};
 constexpr int kSplitSteps = 4;   // a share of a sum has at least these steps
-constexpr int kMaxSplits = 16;
+constexpr int kMaxSplits = 8;    // 32 tokens of 4096 and 11008 68.4 us with 16, 65.8 with 8, 70.5 with 4; 64 tokens 82.1, 77.8, 81.5
 constexpr double kJoinBytes = 4e6;  // a microsecond of k_ffn_join: shares written and read
 
 int64_t steps_of(const came8_ffn* f, const Size& z) { return ceil_div(z.K, f->dtype == CAME8_F32 ? 32 : 64) * z.nseg; }
