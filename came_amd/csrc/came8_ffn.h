@@ -241,21 +241,24 @@ struct Stage {
   }
 };
 
-// fp32 values as three bf16 ones, each the rounding of what the ones before leave: their sum is the value to 2^-24 of it.
-// (Infinities and NaN, and what rounds to infinity, are in the first alone.)
+// fp32 values as three bf16 ones, each the rounding of what the ones before leave: their sum is the value to 2^-24 of it.  The
+// first two are bounded by bf16's largest value, so that one that would round to infinity leaves a rest, and infinities and NaN
+// get to the third, which meets the other operand's first alone: infinity times a number has the number's sign, and no part of
+// it cancels another.
 struct Parts {
   uint32_t w[3];  // of two values, packed
 };
 __device__ __forceinline__ Parts parts_of(float x, float y) {
+  constexpr float kLargest = 0x1.fep127f;
   Parts p;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    p.w[i] = uint32_t(BF16::store(x)) | uint32_t(BF16::store(y)) << 16;
+  for (int i = 0; i < 2; ++i) {
+    p.w[i] = uint32_t(BF16::store(__builtin_amdgcn_fmed3f(x, -kLargest, kLargest))) |
+             uint32_t(BF16::store(__builtin_amdgcn_fmed3f(y, -kLargest, kLargest))) << 16;
     x -= BF16::elem(&p.w[i], 0);
     y -= BF16::elem(&p.w[i], 1);
-    x = fabsf(x) <= 0x1p127f ? x : 0.0f;
-    y = fabsf(y) <= 0x1p127f ? y : 0.0f;
   }
+  p.w[2] = uint32_t(BF16::store(x)) | uint32_t(BF16::store(y)) << 16;
   return p;
 }
 
@@ -398,7 +401,7 @@ struct Tile {
 //
 // fp32 at BM = 256: the matrix instructions of fp32 run at a sixteenth of bf16's rate.  The operands are taken apart into three
 // bf16 parts on their way to LDS, and the six products of parts down to 2^-16 of the largest, summed in fp32, are a product
-// of fp32's accuracy at a sixth of bf16's rate: 2048 tokens of 4096 and 11008 forward and backward 9.8 ms (170
+// of fp32's accuracy at a sixth of bf16's rate: 2048 tokens of 4096 and 11008 forward and backward 9.6 ms (173
 // TFLOP/s) against 12.4.
 template <typename T, int BM, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD = false>
 __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) {
@@ -429,7 +432,8 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
   const int wm = wave % WAVES_M, wn = wave / WAVES_M;
 
   // Steps loaded ahead; step t is in registers t % D.  Two where registers allow: 1021 tokens of 1024 and 2731 in fp32, tiles
-  // of 64 and 128, 516 us with one and 492 with two, 32 tokens of 4096 and 11008 in bf16 80 and 75 us.
+  // of 64 and 128, 516 us with one and 492 with two, 32 tokens of 4096 and 11008 in bf16 80 and 75 us (with sums in
+  // up to 16 shares).
   constexpr int D = BM < 256 ? 2 : 1;
   Stage<T, BM, NT, AROWS> sa[D];
   Stage<T, BN, NT, BROWS, EPI == kGate ? WN / 2 : 0, ODD> sb[D];
@@ -739,7 +743,7 @@ __global__ __launch_bounds__(kThreads) void k_ffn_join_grads(const GradArgs args
 // two chunks of a row at once, whole lines of a row by four lanes, four steps in flight; their sums are added in order in
 // LDS.  Rows may start at any element.  One token of 4096 and 11008 in bf16: 36.8 us for 180 MB of gate and up, 22 for the
 // 90 MB of down (4.9 and 4.1 TB/s), 60 together, 75 in tiles; 2 or 8 steps in flight and 16 wavefronts changed nothing.  With
-// 32 rows it took 89 us, tiles 75: x then costs more loads than the weights.
+// 32 rows it took 89 us, tiles 66: x then costs more loads than the weights.
 //
 // h between the two is kept in fp32: as an operand it is its rounding to the type and the rest's, two products, which the
 // weights' way hides, so that y is rounded once.

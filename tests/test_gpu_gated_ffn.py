@@ -102,6 +102,25 @@ def test_large_fp32_products_keep_fp32_accuracy():
     assert torch.equal(got[rows], want[rows]) and not torch.isfinite(got[[5, 700]]).any()
 
 
+@pytest.mark.parametrize("T", [3, 140, 2100])
+def test_fp32_values_next_to_the_largest_and_infinity(T):
+    """A row with a value that would round to infinity in a shorter type keeps float32's accuracy, and infinity times positive
+    weights is infinity, in every kernel."""
+    from came_amd import gated_ffn
+    ops, _ = _operands(T, 520, 1500, 600, F32, seed=14)
+    ops = [t.abs() for t in ops]
+    ops[1][:, 0] *= 2.0**-100
+    ops[2][:, 0] *= 2.0**-100
+    ops[0][T - 1, 0] = torch.finfo(F32).max
+    with torch.no_grad():
+        want, bound, _ = orc.forward(*ops, "silu", F32)
+        _check(gated_ffn(*ops), want, bound, "next to the largest")
+        rows = ops[0].clone()
+        rows[1, 519] = float("inf")
+        got = gated_ffn(rows, *ops[1:])
+    assert torch.isinf(got[1]).all() and torch.isfinite(got[[0, T - 1]]).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("T", [1, 9, 140])
 def test_operands_where_they_lie(T, dtype):
