@@ -64,7 +64,7 @@ def train(steps: int = 200, tokens: int = 512, dim: int = 256, hidden: int = 704
         opt.step()
         opt.zero_grad()
         if step % 10 == 0 or step == steps - 1:
-            losses.append(float(loss))
+            losses.append(float(loss.detach()))
             log(f"step {step:4d}  loss {losses[-1]:.5f}")
     return losses
 
