@@ -322,7 +322,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   at::Tensor first;
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
     PyObject* o = PyList_GET_ITEM(tensors, i);
-    if (!THPVariable_CheckExact(o) && !(of_parameters && THPVariable_Check(o))) Py_RETURN_NONE;
+    if (!THPVariable_Check(o)) Py_RETURN_NONE;
     const at::Tensor& t = of_parameters ? THPVariable_Unpack(o).grad() : THPVariable_Unpack(o);
     if (of_parameters && !t.defined()) continue;
     if (!first.defined()) first = t;

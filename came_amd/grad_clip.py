@@ -14,7 +14,7 @@ _DTYPE_CODE = {torch.float32: _lib.CAME8_F32, torch.bfloat16: _lib.CAME8_BF16, t
 
 
 def _check(t: torch.Tensor, what: str, device) -> None:
-    if t.is_sparse:
+    if t.layout != torch.strided:
         raise RuntimeError(f"{what}: sparse gradients are not supported")
     if not t.is_cuda:
         raise RuntimeError(f"{what}: came_amd runs on the GPU; got a {t.device} tensor")
@@ -50,6 +50,8 @@ def _reduce(tensors: list, max_norm: float | None, scale: bool, what: str, of_pa
             tensors = [g for g in [p.grad for p in tensors] if g is not None]
         tensors, copies = _contiguous(tensors, what)
         found = host.grad_norm([t.detach() for t in tensors], False, float(max_norm or 0.0), scale, stream)
+        if found is None:  # nothing else is left that it refuses
+            raise RuntimeError(f"{what}: tensor subclasses that dispatch in Python are not supported: their values may lie elsewhere")
         for t, c in copies if scale else ():
             t.copy_(c)
     return found

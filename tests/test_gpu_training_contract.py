@@ -1,0 +1,35 @@
+"""What programs count on around AdamW, the clip and the gated feed-forward block beside their formulas."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _needs_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+class Named(torch.Tensor):
+    """A subclass without dispatch of its own: its values are its storage's."""
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_gradients_of_a_simple_subclass(strided):
+    import came_amd
+    g = torch.randn(40, 50, device="cuda")
+    g = g.t() if strided else g
+    want = float(g.double().norm())
+    p = torch.nn.Parameter(torch.zeros(g.shape, device="cuda"))
+    p.grad = g.clone(memory_format=torch.preserve_format).as_subclass(Named)
+    assert abs(float(came_amd.grad_norm([p.grad])) / want - 1) < 1e-6
+    assert abs(float(came_amd.clip_grad_norm_([p], 1.0)) / want - 1) < 1e-6
+    assert abs(float(p.grad.as_subclass(torch.Tensor).double().norm()) - 1) < 1e-5
+    q = torch.nn.Parameter(torch.zeros(g.shape, device="cuda"))
+    q.grad = p.grad.as_subclass(torch.Tensor).clone()
+    a, b = came_amd.AdamW([p], max_grad_norm=0.5), came_amd.AdamW([q], max_grad_norm=0.5)
+    a.step()
+    b.step()
+    assert a.state[p]["step"] == 1 and torch.equal(p, q) and torch.equal(a.last_grad_norm, b.last_grad_norm)

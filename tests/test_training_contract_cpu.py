@@ -1,0 +1,53 @@
+"""What programs count on around AdamW and the gradient clip, on the host: nothing is left out in silence, copies and
+checkpoints keep what a step goes by."""
+import types
+
+import pytest
+import torch
+from torch.utils._pytree import tree_map
+
+import came_amd
+
+
+class Elsewhere(torch.Tensor):
+    """A subclass that says it is on the GPU and keeps its values in a tensor of its own, as distributed tensors do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        t = torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device="cuda:0")
+        t.inner = inner
+        return t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        bare = lambda x: x.inner if isinstance(x, Elsewhere) else x  # noqa: E731
+        out = func(*tree_map(bare, args), **tree_map(bare, kwargs or {}))
+        return tree_map(lambda x: Elsewhere(x) if isinstance(x, torch.Tensor) else x, out)
+
+
+@pytest.fixture
+def elsewhere(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+    p = torch.nn.Parameter(Elsewhere(torch.zeros(4)))
+    p.grad = Elsewhere(torch.full((4,), 100.0))
+    return p
+
+
+def test_a_clip_that_cannot_be_taken_raises(elsewhere):
+    with pytest.raises(RuntimeError, match="clip_grad_norm_: tensor subclasses"):
+        came_amd.clip_grad_norm_([elsewhere], 1.0)
+    with pytest.raises(RuntimeError, match="grad_norm: tensor subclasses"):
+        came_amd.grad_norm([elsewhere.grad])
+
+
+@pytest.mark.parametrize("cls", [came_amd.AdamW, came_amd.AdamW8bit])
+def test_a_step_whose_clip_cannot_be_taken_raises(cls, elsewhere):
+    with pytest.raises(RuntimeError, match="tensor subclasses"):
+        cls([elsewhere], max_grad_norm=1.0).step()
+
+
+def test_compressed_sparse_gradients_are_refused():
+    p = torch.nn.Parameter(torch.eye(3))
+    g = torch.eye(3).to_sparse_csr()
+    with pytest.raises(RuntimeError, match="sparse"):
+        came_amd.grad_norm([g])
