@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "came8_device.h"
+#include "came8_view.h"
 
 namespace came8 {
 
@@ -101,8 +102,7 @@ struct GemmArgs {
   int64_t ldg;
 };
 
-// A tile's view of an operand from its next k on: reads past the matrix's end give zeros, whatever the tile.  The hardware
-// checks words, and rows start on words (k_ffn_pack), so the last word may count whole: it holds a byte of the matrix.
+// A tile's view of an operand from its next k on: reads past the matrix's end give zeros, whatever the tile.
 typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every view's end (offsets within one stay below 2^31)
 struct View {
@@ -112,8 +112,7 @@ struct View {
   int32_t ld;    // bytes from a row (or k) to the next
 
   __device__ __forceinline__ Buffer buffer() const {
-    const int64_t bytes = left <= 0 ? 0 : left > 0x7ffffffcll ? 0x7ffffffcll : (left + 3) & ~int64_t(3);
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, int32_t(bytes), 0x00027000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, buffer_bytes(left), 0x00027000);
   }
   __device__ __forceinline__ void next(int64_t steps = 1) {
     p += step * steps;
@@ -445,7 +444,7 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     const int64_t ld = o.ld * kElem;
     View v;
     v.p = static_cast<const char*>(o.p) + (rows ? at * ld : int64_t(at) * kElem);
-    v.left = rows ? (extent - at) * ld : (args.K - 1) * ld + int64_t(extent - at) * kElem;
+    v.left = view_bytes(rows, extent - at, args.K, ld, kElem);
     v.step = rows ? kRowBytes : BK * ld;
     v.ld = int32_t(ld);
     return v;
