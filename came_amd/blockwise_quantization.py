@@ -50,6 +50,14 @@ def _require_cuda(t: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what}: came_amd runs on the GPU; got a {t.device} tensor")
 
 
+def _require_absmax(q: torch.Tensor, absmax: torch.Tensor, block_size: int, what: str) -> None:
+    """The kernels read it on the codes' GPU: a host address, or another GPU's, faults there."""
+    if absmax.device != q.device:
+        raise RuntimeError(f"{what}: codes on {q.device}, absmax on {absmax.device}")
+    if absmax.numel() < num_blocks(q.numel(), block_size):
+        raise ValueError("absmax has fewer entries than the number of blocks")
+
+
 def quantize_blockwise(tensor: torch.Tensor, *, signed: bool, block_size: int):
     """Return ``(codes shaped like tensor, absmax[num_blocks])`` computed by libcame8."""
     _require_cuda(tensor, "quantize_blockwise")
@@ -72,11 +80,10 @@ def dequantize_blockwise(q: torch.Tensor, absmax: torch.Tensor, *, signed: bool,
                          dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``q * (absmax / Q)`` per element, shaped like ``q``."""
     _require_cuda(q, "dequantize_blockwise")
+    _require_absmax(q, absmax, block_size, "dequantize_blockwise")
     lib = _lib.load()
     qc = q.contiguous()
     ac = absmax.to(torch.float32).contiguous()
-    if ac.numel() < num_blocks(qc.numel(), block_size):
-        raise ValueError("absmax has fewer entries than the number of blocks")
     out = torch.empty(qc.shape, device=qc.device, dtype=torch.float32)
     with torch.cuda.device(qc.device):
         stream = torch.cuda.current_stream(qc.device).cuda_stream
@@ -95,11 +102,10 @@ def dequantize_second_moment(q: torch.Tensor, absmax: torch.Tensor, *, block_siz
     _require_cuda(q, "dequantize_second_moment")
     if q.dtype != torch.uint8:
         raise ValueError(f"dequantize_second_moment: codes are uint8, got {q.dtype}")
+    _require_absmax(q, absmax, block_size, "dequantize_second_moment")
     lib = _lib.load()
     qc = q.contiguous()
     ac = absmax.to(torch.float32).contiguous()
-    if ac.numel() < num_blocks(qc.numel(), block_size):
-        raise ValueError("absmax has fewer entries than the number of blocks")
     out = torch.empty(qc.shape, device=qc.device, dtype=torch.float32)
     with torch.cuda.device(qc.device):
         stream = torch.cuda.current_stream(qc.device).cuda_stream

@@ -51,3 +51,14 @@ def test_compressed_sparse_gradients_are_refused():
     g = torch.eye(3).to_sparse_csr()
     with pytest.raises(RuntimeError, match="sparse"):
         came_amd.grad_norm([g])
+
+
+def test_absmax_of_another_device_is_refused():
+    from came_amd import blockwise_quantization as bq
+    for dtype, call in ((torch.uint8, lambda q, a: bq.dequantize_second_moment(q, a, block_size=64)),
+                        (torch.int8, lambda q, a: bq.dequantize_blockwise(q, a, signed=True, block_size=64))):
+        q = Elsewhere(torch.zeros(100, dtype=dtype))
+        with pytest.raises(RuntimeError, match="codes on cuda:0, absmax on cpu"):
+            call(q, torch.ones(2))
+        with pytest.raises(ValueError, match="fewer entries"):
+            call(q, Elsewhere(torch.ones(1)))
