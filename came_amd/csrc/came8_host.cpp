@@ -475,6 +475,8 @@ PyObject* gated_ffn(PyObject*, PyObject* args) {
   for (int i = 0; i < 4; ++i) {
     TORCH_CHECK(THPVariable_Check(po[i]), "gated_ffn: came_amd runs on the GPU; ", names[i], " is ", Py_TYPE(po[i])->tp_name);
     t[i] = THPVariable_Unpack(po[i]);
+    // without an operand that needs a gradient no autograd node would refuse it, and the result would have no tangent
+    TORCH_CHECK(!t[i]._fw_grad(0).defined(), "gated_ffn: no forward-mode derivatives; ", names[i], " has a tangent");
     TORCH_CHECK(t[i].is_cuda(), "gated_ffn: came_amd runs on the GPU; ", names[i], " is a ", t[i].device(), " tensor");
     TORCH_CHECK(t[i].layout() == at::kStrided && dtype_code(t[i]) >= 0, "gated_ffn: unsupported dtype ", dtype_name(t[i]), " of ",
                 names[i], " (float32, bfloat16 and float16 are supported)");

@@ -20,8 +20,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` over the last dimension of ``x``.
 
     x [..., dim]; w_gate, w_up [hidden, dim]; w_down [out, hidden]: one type (float32, bfloat16 or float16), one GPU.
-    activation: "silu", "gelu" (by erf) or "gelu_tanh".  Differentiable once in every operand.  Operands whose rows are
-    contiguous are read where they are, with the row strides they have; others are copied.
+    activation: "silu", "gelu" (by erf) or "gelu_tanh".  Differentiable once in every operand, in
+    reverse mode (an operand with a forward-mode tangent is refused).  Operands whose rows are contiguous are read where they
+    are, with the row strides they have; others are copied.
     """
     act = ACTIVATIONS.get(activation)
     if act is None:

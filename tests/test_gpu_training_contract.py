@@ -1,7 +1,7 @@
 """What programs count on around AdamW, the clip and the gated feed-forward block beside their formulas."""
-
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,31 @@ def test_gradients_of_a_simple_subclass(strided):
     a.step()
     b.step()
     assert a.state[p]["step"] == 1 and torch.equal(p, q) and torch.equal(a.last_grad_norm, b.last_grad_norm)
+
+
+@pytest.mark.parametrize("dual", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_raise(dual, grad):
+    """There are none: without an error they would read as zero."""
+    import came_amd
+    ops = [torch.randn(*s, device="cuda") for s in ((5, 16), (24, 16), (24, 16), (16, 24))]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        ops[dual] = forward_ad.make_dual(ops[dual], torch.ones_like(ops[dual]))
+        with pytest.raises(RuntimeError, match="forward-mode|forward mode|forward AD|jvp"):
+            came_amd.gated_ffn(*ops)
+
+
+@pytest.mark.parametrize("transform", ["jvp", "vmap", "grad", "jacfwd"])
+def test_function_transforms_raise(transform):
+    import came_amd
+    ops = [torch.randn(*s, device="cuda") for s in ((5, 16), (24, 16), (24, 16), (16, 24))]
+
+    def fn(x):
+        y = came_amd.gated_ffn(x, *ops[1:])
+        return y.sum() if transform == "grad" else y
+
+    func = torch.func
+    call = dict(jvp=lambda: func.jvp(fn, (ops[0],), (torch.ones_like(ops[0]),)), vmap=lambda: func.vmap(fn)(ops[0][None]),
+                grad=lambda: func.grad(fn)(ops[0]), jacfwd=lambda: func.jacfwd(fn)(ops[0]))[transform]
+    with pytest.raises(RuntimeError):
+        call()

@@ -4,6 +4,7 @@ import types
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils._pytree import tree_map
 
 import came_amd
@@ -62,3 +63,12 @@ def test_absmax_of_another_device_is_refused():
             call(q, torch.ones(2))
         with pytest.raises(ValueError, match="fewer entries"):
             call(q, Elsewhere(torch.ones(1)))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_tangent_of_the_feed_forward_block_is_refused(grad):
+    w = torch.zeros(24, 16)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.zeros(5, 16), torch.ones(5, 16))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            came_amd.gated_ffn(x, w, w, w.t())
