@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
@@ -470,6 +471,7 @@ PyObject* gated_ffn(PyObject*, PyObject* args) {
   PyObject* po[4];
   long long act, stream;
   if (!PyArg_ParseTuple(args, "OOOOLL", &po[0], &po[1], &po[2], &po[3], &act, &stream)) return nullptr;
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), "gated_ffn: cannot be traced; a trace would hold the result's allocation alone");
   const char* names[4] = {"x", "w_gate", "w_up", "w_down"};
   at::Tensor t[4];
   for (int i = 0; i < 4; ++i) {

@@ -61,3 +61,12 @@ def test_function_transforms_raise(transform):
                 grad=lambda: func.grad(fn)(ops[0]), jacfwd=lambda: func.jacfwd(fn)(ops[0]))[transform]
     with pytest.raises(RuntimeError):
         call()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_traces_raise(grad):
+    """A trace would hold the result's allocation and not what fills it."""
+    import came_amd
+    ops = [torch.randn(*s, device="cuda") for s in ((5, 16), (24, 16), (24, 16), (16, 24))]
+    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="gated_ffn.*trace"):
+        torch.jit.trace(lambda x: came_amd.gated_ffn(x, *ops[1:]), (ops[0],), check_trace=False)

@@ -72,3 +72,9 @@ def test_a_tangent_of_the_feed_forward_block_is_refused(grad):
         x = forward_ad.make_dual(torch.zeros(5, 16), torch.ones(5, 16))
         with pytest.raises(RuntimeError, match="forward-mode"):
             came_amd.gated_ffn(x, w, w, w.t())
+
+
+def test_a_trace_of_the_feed_forward_block_is_refused():
+    w = torch.zeros(24, 16)
+    with pytest.raises(RuntimeError, match="gated_ffn: cannot be traced"):
+        torch.jit.trace(lambda x: came_amd.gated_ffn(x, w, w, w.t()), (torch.zeros(5, 16),), check_trace=False)
