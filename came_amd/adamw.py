@@ -5,9 +5,10 @@
     ``exp_avg_sq_q``, ``exp_avg_sq_absmax``)
 
 The update is that of ``torch.optim.AdamW`` (decoupled weight decay).  ``max_grad_norm`` clips by the norm over all
-gradients of the optimizer inside the step: the gradients are scaled as they are read and are not changed.  Parameters
-must live on the GPU.  The step count is a host number that enters the bias corrections, so a step cannot be captured in
-a HIP graph and replayed.
+gradients of the optimizer inside the step: the gradients are scaled as they are read and are not changed.  A step counts
+as a write to the parameters: a backward pass through a node that saved them before it raises.  Parameters must live on the
+GPU.  The step count is a host number that enters the bias corrections, so a step cannot be captured in a HIP graph and
+replayed.
 """
 from __future__ import annotations
 
@@ -182,6 +183,7 @@ class _AdamWBase(torch.optim.Optimizer):
                 self._launch(device, descs, n, group, factor)
             for p, pd in copyback:
                 p.data.copy_(pd)
+            torch.autograd.graph.increment_version([p for p in group["params"] if p.grad is not None])
         return loss
 
 

@@ -234,6 +234,12 @@ struct Entries {
 
 void entry_check(int rc, const char* what) { TORCH_CHECK(rc == CAME8_OK, what, " failed (", rc, "): ", entries.error()); }
 
+// A tensor that a kernel has written, for the nodes that have saved it (gated_ffn its weights); inference tensors have no
+// version.
+void written(c10::TensorImpl* t) {
+  if (!t->is_inference()) t->bump_version();
+}
+
 // The buffer of a moment or its scales: contiguous, of the parameter's device; null otherwise.
 void* moment(PyObject* st, PyObject* name, const at::Tensor& p, at::ScalarType type, int64_t n) {
   const at::Tensor* t = tensor_of(st, name);
@@ -301,6 +307,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   entry_check(entries.adamw(descs.data(), int32_t(descs.size()), &hp, reinterpret_cast<const float*>(scale),
                             reinterpret_cast<void*>(stream)),
               "came8_adamw_step");
+  for (PyObject* po : used) written(THPVariable_Unpack(po).unsafeGetTensorImpl());
   PyObject* list = advanced(used, counts);
   if (list == nullptr) return nullptr;
   Py_DECREF(list);
@@ -319,7 +326,9 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   unsigned long long stream;
   if (!PyArg_ParseTuple(args, "O!pdpK", &PyList_Type, &tensors, &of_parameters, &max_norm, &scale, &stream)) return nullptr;
   std::vector<came8_grad_tensor> descs;
+  std::vector<c10::TensorImpl*> scaled;
   descs.reserve(size_t(PyList_GET_SIZE(tensors)));
+  scaled.reserve(size_t(PyList_GET_SIZE(tensors)));
   at::Tensor first;
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i) {
     PyObject* o = PyList_GET_ITEM(tensors, i);
@@ -331,6 +340,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
         !t.is_contiguous() || dtype_code(t) < 0)
       Py_RETURN_NONE;
     descs.push_back(came8_grad_tensor{t.numel() > 0 ? t.data_ptr() : nullptr, t.numel(), dtype_code(t), 0});
+    if (scale) scaled.push_back(t.unsafeGetTensorImpl());
   }
   if (descs.empty()) Py_RETURN_FALSE;
   c10::OptionalDeviceGuard guard(first.device());
@@ -341,6 +351,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   entry_check((scale ? entries.clip : entries.norm)(descs.data(), n, max_norm, out, out + 1, ws.data_ptr(), bytes,
                                                     reinterpret_cast<void*>(stream)),
               scale ? "came8_grad_clip" : "came8_grad_norm");
+  for (c10::TensorImpl* t : scaled) written(t);
   const int64_t at = int64_t(bytes / 4);
   return Py_BuildValue("NN", THPVariable_Wrap(ws.select(0, at)), THPVariable_Wrap(ws.narrow(0, at + 1, 1)));
   END_HANDLE_TH_ERRORS

@@ -12,6 +12,11 @@ def _needs_gpu():
         pytest.skip("no GPU")
 
 
+def _classes():
+    import came_amd
+    return came_amd.AdamW, came_amd.AdamW8bit
+
+
 class Named(torch.Tensor):
     """A subclass without dispatch of its own: its values are its storage's."""
 
@@ -33,6 +38,47 @@ def test_gradients_of_a_simple_subclass(strided):
     a.step()
     b.step()
     assert a.state[p]["step"] == 1 and torch.equal(p, q) and torch.equal(a.last_grad_norm, b.last_grad_norm)
+
+
+@pytest.mark.parametrize("cls", range(2))
+@pytest.mark.parametrize("transposed", [False, True])
+def test_a_step_between_forward_and_backward_is_seen(cls, transposed):
+    """The block's backward pass uses the weights of the forward one: where a step has changed them it raises."""
+    import came_amd
+    w = [torch.randn(*s, device="cuda") * 0.1 for s in ((72, 64), (72, 64), (64, 72))]
+    w = [torch.nn.Parameter(t.t().contiguous().t() if transposed else t) for t in w]
+    opt = _classes()[cls](w)
+    y = came_amd.gated_ffn(torch.randn(20, 64, device="cuda"), *w)
+    y.backward(torch.ones_like(y), retain_graph=True)
+    before = [p._version for p in w]
+    opt.step()
+    assert all(p._version > b for p, b in zip(w, before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(torch.ones_like(y))
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+def test_a_clip_advances_the_gradients_versions(transposed):
+    import came_amd
+    p = torch.nn.Parameter(torch.zeros(30, 20, device="cuda"))
+    p.grad = torch.randn(20, 30, device="cuda").t() if transposed else torch.randn(30, 20, device="cuda")
+    before = p.grad._version
+    came_amd.grad_norm([p.grad])
+    assert p.grad._version == before
+    came_amd.clip_grad_norm_([p], 0.5)
+    assert p.grad._version > before
+
+
+def test_inference_tensors_are_stepped_and_clipped():
+    """They have no version; a step and a clip write them as others."""
+    import came_amd
+    with torch.inference_mode():
+        p = torch.nn.Parameter(torch.ones(100, device="cuda"), requires_grad=False)
+        p.grad = torch.ones(100, device="cuda")
+    assert abs(float(came_amd.clip_grad_norm_([p], 1.0)) - 10) < 1e-4
+    opt = came_amd.AdamW([p], lr=0.1, weight_decay=0.0)
+    opt.step()
+    assert (p - 0.9).abs().max() < 1e-4
 
 
 @pytest.mark.parametrize("dual", range(4))
