@@ -43,6 +43,14 @@ class _AdamWBase(torch.optim.Optimizer):
         self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None  # of the last step with max_grad_norm: a device scalar, before the clip
 
+    def __getstate__(self) -> dict:  # of copies and pickles
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
+
+    def __setstate__(self, state: dict) -> None:  # also torch's loading of a state_dict, without the bound
+        super().__setstate__(state)
+        self.__dict__.setdefault("max_grad_norm", None)
+        self.last_grad_norm = None
+
     # ------------------------------------------------------------------ state
     def _init_state(self, state: dict, p: torch.Tensor, group: dict) -> None:
         raise NotImplementedError

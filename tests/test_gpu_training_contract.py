@@ -1,4 +1,6 @@
 """What programs count on around AdamW, the clip and the gated feed-forward block beside their formulas."""
+import copy
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -116,3 +118,17 @@ def test_traces_raise(grad):
     ops = [torch.randn(*s, device="cuda") for s in ((5, 16), (24, 16), (24, 16), (16, 24))]
     with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="gated_ffn.*trace"):
         torch.jit.trace(lambda x: came_amd.gated_ffn(x, *ops[1:]), (ops[0],), check_trace=False)
+
+
+def test_copies_of_an_optimizer_clip_as_it_does():
+    for cls in _classes():
+        p = torch.nn.Parameter(torch.ones(100, device="cuda"))
+        p.grad = torch.ones(100, device="cuda")
+        opt = cls([p], max_grad_norm=1e-3)
+        opt.step()
+        two = copy.deepcopy(opt)
+        q = two.param_groups[0]["params"][0]
+        q.grad = p.grad.clone()
+        opt.step()
+        two.step()
+        assert torch.equal(p, q) and torch.equal(opt.last_grad_norm, two.last_grad_norm)

@@ -1,5 +1,7 @@
 """What programs count on around AdamW and the gradient clip, on the host: nothing is left out in silence, copies and
 checkpoints keep what a step goes by."""
+import copy
+import pickle
 import types
 
 import pytest
@@ -78,3 +80,15 @@ def test_a_trace_of_the_feed_forward_block_is_refused():
     w = torch.zeros(24, 16)
     with pytest.raises(RuntimeError, match="gated_ffn: cannot be traced"):
         torch.jit.trace(lambda x: came_amd.gated_ffn(x, w, w, w.t()), (torch.zeros(5, 16),), check_trace=False)
+
+
+@pytest.mark.parametrize("cls", [came_amd.AdamW, came_amd.AdamW8bit])
+@pytest.mark.parametrize("bound", [None, 0.0, 2.5])
+@pytest.mark.parametrize("way", [copy.deepcopy, lambda opt: pickle.loads(pickle.dumps(opt))], ids=["deepcopy", "pickle"])
+def test_copies_keep_the_clip_bound(cls, bound, way):
+    opt = cls([torch.nn.Parameter(torch.zeros(3))], max_grad_norm=bound)
+    two = way(opt)
+    assert two.max_grad_norm == bound and two.last_grad_norm is None
+    two.step()  # no gradient: nothing to do
+    two.load_state_dict(opt.state_dict())
+    assert two.max_grad_norm == bound
