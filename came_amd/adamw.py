@@ -23,6 +23,13 @@ from .blockwise_quantization import init_qstate, num_blocks
 from .grad_clip import _DTYPE_CODE, _reduce
 
 
+def _refuse_options(group: dict) -> None:
+    """Options of torch.optim.AdamW that change its update and that the step here does not have."""
+    for option in ("amsgrad", "maximize"):
+        if group.get(option):
+            raise ValueError(f"param group with {option}=True: AdamW (came_amd) does not have this option")
+
+
 class _AdamWBase(torch.optim.Optimizer):
     _BITS = 32
     _KEYS: dict = {}  # state tensors and their types
@@ -51,6 +58,11 @@ class _AdamWBase(torch.optim.Optimizer):
         self.__dict__.setdefault("max_grad_norm", None)
         self.last_grad_norm = None
 
+    def add_param_group(self, param_group: dict) -> None:
+        if isinstance(param_group, dict):  # torch refuses others
+            _refuse_options(param_group)
+        super().add_param_group(param_group)
+
     # ------------------------------------------------------------------ state
     def _init_state(self, state: dict, p: torch.Tensor, group: dict) -> None:
         raise NotImplementedError
@@ -77,6 +89,8 @@ class _AdamWBase(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Loads every state tensor in the type it was saved in (torch's loader casts them to the parameter's)."""
         groups, saved = state_dict["param_groups"], state_dict["state"]
+        for g in groups:
+            _refuse_options(g)
         super().load_state_dict(state_dict)
         ids = dict(zip(chain.from_iterable(g["params"] for g in groups),
                        chain.from_iterable(g["params"] for g in self.param_groups)))

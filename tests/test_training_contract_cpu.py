@@ -92,3 +92,29 @@ def test_copies_keep_the_clip_bound(cls, bound, way):
     two.step()  # no gradient: nothing to do
     two.load_state_dict(opt.state_dict())
     assert two.max_grad_norm == bound
+
+
+def _stepped(p, **kw):
+    """A torch.optim.AdamW over p after a step."""
+    opt = torch.optim.AdamW([p], **kw)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    return opt
+
+
+@pytest.mark.parametrize("option", ["amsgrad", "maximize"])
+def test_options_that_the_step_does_not_have_are_refused(option):
+    p = torch.nn.Parameter(torch.zeros(5))
+    opt = came_amd.AdamW([p], lr=0.5)
+    with pytest.raises(ValueError, match=option):
+        opt.load_state_dict(_stepped(p, **{option: True}).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5 and not opt.param_groups[0].get(option) and not opt.state
+    opt.load_state_dict(_stepped(p, lr=0.25).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.state[p]["step"] == 1
+    with pytest.raises(ValueError, match=option):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2))], option: True})
+    assert len(opt.param_groups) == 1
+    for cls in (came_amd.AdamW, came_amd.AdamW8bit):
+        with pytest.raises(ValueError, match=option):
+            cls([{"params": [p], option: True}])
+        cls([{"params": [p], option: False}])
