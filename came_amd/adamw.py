@@ -87,7 +87,8 @@ class _AdamWBase(torch.optim.Optimizer):
         return int(group.get("block_size", 256))
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """Loads every state tensor in the type it was saved in (torch's loader casts them to the parameter's)."""
+        """Loads every state tensor in the type it was saved in (torch's loader casts them to the parameter's), contiguous (torch
+        keeps the moments of a transposed or channels-last parameter in its order)."""
         groups, saved = state_dict["param_groups"], state_dict["state"]
         for g in groups:
             _refuse_options(g)
@@ -102,7 +103,7 @@ class _AdamWBase(torch.optim.Optimizer):
                 if key == "step":  # torch.optim keeps a tensor
                     self.state[p][key] = int(v)
                 elif isinstance(v, torch.Tensor):
-                    self.state[p][key] = v.detach().to(device=p.device).clone()
+                    self.state[p][key] = v.detach().to(device=p.device, copy=True, memory_format=torch.contiguous_format)
         for g in self.param_groups:
             for p in g["params"]:
                 if self.state.get(p):

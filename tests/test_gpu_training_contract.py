@@ -132,3 +132,24 @@ def test_copies_of_an_optimizer_clip_as_it_does():
         opt.step()
         two.step()
         assert torch.equal(p, q) and torch.equal(opt.last_grad_norm, two.last_grad_norm)
+
+
+def test_a_checkpoint_of_a_transposed_parameter_continues():
+    """torch keeps its moments in the parameter's order; the next steps agree within float32 rounding (three roundings of the
+    parameter and of an update of at most a few lr a step)."""
+    import came_amd
+    u, lr = 2.0**-24, 1e-2
+    gen = torch.Generator().manual_seed(4)
+    p = torch.nn.Parameter(torch.randn(60, 50, generator=gen).cuda().t())
+    ref = torch.optim.AdamW([p], lr=lr, weight_decay=0.1, foreach=False)
+    p.grad = torch.randn(50, 60, generator=gen).cuda()
+    ref.step()
+    q = torch.nn.Parameter(p.detach().clone())
+    opt = came_amd.AdamW([q], lr=lr, weight_decay=0.1)
+    opt.load_state_dict(ref.state_dict())
+    for _ in range(3):
+        p.grad = torch.randn(50, 60, generator=gen).cuda()
+        q.grad = p.grad.clone()
+        ref.step()
+        opt.step()
+    assert ((p - q).abs() <= 3 * (8 * u * p.abs() + 64 * u * lr)).all()

@@ -118,3 +118,19 @@ def test_options_that_the_step_does_not_have_are_refused(option):
         with pytest.raises(ValueError, match=option):
             cls([{"params": [p], option: True}])
         cls([{"params": [p], option: False}])
+
+
+@pytest.mark.parametrize("p", [torch.randn(6, 4).t(), torch.randn(2, 3, 4, 5).to(memory_format=torch.channels_last)],
+                         ids=["transposed", "channels_last"])
+def test_moments_in_the_order_of_a_strided_parameter_are_taken(p):
+    p = torch.nn.Parameter(p)
+    ref = torch.optim.AdamW([p])
+    p.grad = torch.randn(p.shape).contiguous()
+    ref.step()
+    assert not ref.state[p]["exp_avg"].is_contiguous()
+    opt = came_amd.AdamW([p])
+    opt.load_state_dict(ref.state_dict())
+    for key in ("exp_avg", "exp_avg_sq"):
+        got = opt.state[p][key]
+        assert got.is_contiguous() and torch.equal(got, ref.state[p][key])
+        assert got.data_ptr() != ref.state[p][key].data_ptr()
