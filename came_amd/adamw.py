@@ -88,26 +88,27 @@ class _AdamWBase(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Loads every state tensor in the type it was saved in (torch's loader casts them to the parameter's), contiguous (torch
-        keeps the moments of a transposed or channels-last parameter in its order)."""
+        keeps the moments of a transposed or channels-last parameter in its order).  What is refused leaves the optimizer as it
+        was."""
         groups, saved = state_dict["param_groups"], state_dict["state"]
         for g in groups:
             _refuse_options(g)
+        loaded = {}  # all of it looked over before anything changes
+        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:  # torch's loader raises else
+            for g, own in zip(groups, self.param_groups):
+                for k, p in zip(g["params"], own["params"]):
+                    if not saved.get(k):
+                        continue
+                    st = loaded[p] = {}
+                    for key, v in saved[k].items():
+                        if key == "step":  # torch.optim keeps a tensor
+                            st[key] = int(v)
+                        elif isinstance(v, torch.Tensor):
+                            st[key] = v.detach().to(device=p.device, copy=True, memory_format=torch.contiguous_format)
+                    self._moments(st, p, g)
         super().load_state_dict(state_dict)
-        ids = dict(zip(chain.from_iterable(g["params"] for g in groups),
-                       chain.from_iterable(g["params"] for g in self.param_groups)))
-        for k, st in saved.items():
-            p = ids.get(k)
-            if p is None:
-                continue
-            for key, v in st.items():
-                if key == "step":  # torch.optim keeps a tensor
-                    self.state[p][key] = int(v)
-                elif isinstance(v, torch.Tensor):
-                    self.state[p][key] = v.detach().to(device=p.device, copy=True, memory_format=torch.contiguous_format)
-        for g in self.param_groups:
-            for p in g["params"]:
-                if self.state.get(p):
-                    self._moments(self.state[p], p, g)
+        for p, st in loaded.items():
+            self.state[p].update(st)
 
     # ------------------------------------------------------------------- step
     def _hparams(self, group: dict) -> _lib.Came8AdamwHParams:

@@ -134,3 +134,38 @@ def test_moments_in_the_order_of_a_strided_parameter_are_taken(p):
         got = opt.state[p][key]
         assert got.is_contiguous() and torch.equal(got, ref.state[p][key])
         assert got.data_ptr() != ref.state[p][key].data_ptr()
+
+
+@pytest.mark.parametrize("wrong", ["type", "size", "missing", "groups"])
+def test_a_refused_load_leaves_the_optimizer_as_it_was(wrong):
+    p, q = torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(7))
+    opt = came_amd.AdamW([p, q], lr=0.5)
+    opt.load_state_dict(_two(p, q).state_dict())
+    opt.param_groups[0]["lr"] = 0.5
+    kept = copy.deepcopy(opt.state_dict())
+    saved = _two(p, q, lr=0.25).state_dict()
+    st = saved["state"][1]  # of the second parameter: the first one's is fine
+    if wrong == "type":
+        st["exp_avg"] = st["exp_avg"].half()
+    elif wrong == "size":
+        st["exp_avg_sq"] = torch.zeros(6)
+    elif wrong == "missing":
+        del st["exp_avg"]
+    else:
+        saved["param_groups"][0]["params"].append(2)
+    with pytest.raises((RuntimeError, ValueError)):
+        opt.load_state_dict(saved)
+    now = opt.state_dict()
+    assert now["param_groups"] == kept["param_groups"]
+    for k, st in kept["state"].items():
+        for key, v in st.items():
+            w = now["state"][k][key]
+            assert torch.equal(v, w) if isinstance(v, torch.Tensor) else v == w
+
+
+def _two(p, q, **kw):
+    """A torch.optim.AdamW over both after a step."""
+    opt = torch.optim.AdamW([p, q], **kw)
+    p.grad, q.grad = torch.randn(5), torch.randn(7)
+    opt.step()
+    return opt
