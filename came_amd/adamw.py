@@ -118,10 +118,9 @@ class _AdamWBase(torch.optim.Optimizer):
                                       int(group.get("seed", 0)) & 0xFFFFFFFF, 0)
 
     def _descriptors(self, group: dict):
-        """{device: (descriptors, how many, tensors to keep alive)} of the group's parameters with gradients, and
-        (parameter, contiguous copy) pairs to write back."""
+        """{device: (descriptors, how many, [(parameter, contiguous copy or None, gradient, state)])} of the group's parameters with
+        gradients: the copies are to be written back, and the states' steps to be counted, once the step is launched."""
         lists: dict = {}
-        copyback = []
         for p in group["params"]:
             g = p.grad
             if g is None:
@@ -143,25 +142,22 @@ class _AdamWBase(torch.optim.Optimizer):
             lists.setdefault(p.device, []).append((p, g, state, moments))
         out = {}
         for device, items in lists.items():
-            descs, keep, k = (_lib.Came8AdamwTensor * len(items))(), [], 0
+            descs, used, k = (_lib.Came8AdamwTensor * len(items))(), [], 0
             for p, g, state, moments in items:
-                state["step"] += 1
+                copy = None if p.data.is_contiguous() else p.data.contiguous()
+                g = g.contiguous()
+                used.append((p, copy, g, state))
                 if p.numel() == 0:
                     continue
-                pd = p.data
-                if not pd.is_contiguous():
-                    pd = pd.contiguous()
-                    copyback.append((p, pd))
-                g = g.contiguous()
-                keep.append((pd, g))
                 d = descs[k]
                 k += 1
-                d.param, d.grad, d.numel, d.step = pd.data_ptr(), g.data_ptr(), p.numel(), state["step"]
+                d.param, d.grad = (p.data if copy is None else copy).data_ptr(), g.data_ptr()
+                d.numel, d.step = p.numel(), state["step"] + 1
                 d.param_dtype, d.grad_dtype = _DTYPE_CODE[p.dtype], _DTYPE_CODE[g.dtype]
                 for (name, _), t in zip(self._KEYS.items(), moments):
                     setattr(d, name.removesuffix("_q"), t.data_ptr())
-            out[device] = (descs, k, keep)
-        return out, copyback
+            out[device] = (descs, k, used)
+        return out
 
     def _launch(self, device, descs, n: int, group: dict, factor) -> None:
         if n == 0:
@@ -202,12 +198,13 @@ class _AdamWBase(torch.optim.Optimizer):
         for group in self.param_groups:
             if self._step_native(group, factor):
                 continue
-            lists, copyback = self._descriptors(group)
-            for device, (descs, n, keep) in lists.items():
+            for device, (descs, n, used) in self._descriptors(group).items():
                 self._launch(device, descs, n, group, factor)
-            for p, pd in copyback:
-                p.data.copy_(pd)
-            torch.autograd.graph.increment_version([p for p in group["params"] if p.grad is not None])
+                for p, copy, _, state in used:
+                    state["step"] += 1
+                    if copy is not None:
+                        p.data.copy_(copy)
+                torch.autograd.graph.increment_version([p for p, *_ in used])
         return loss
 
 

@@ -120,6 +120,23 @@ def test_traces_raise(grad):
         torch.jit.trace(lambda x: came_amd.gated_ffn(x, *ops[1:]), (ops[0],), check_trace=False)
 
 
+@pytest.mark.parametrize("cls", range(2))
+@pytest.mark.parametrize("transposed", [False, True])
+def test_a_refused_step_is_not_counted(cls, transposed):
+    p = torch.randn(30, 20, device="cuda")
+    p = torch.nn.Parameter(p.t() if transposed else p)
+    p.grad = torch.randn(p.shape, device="cuda")
+    before = p.detach().clone()
+    opt = _classes()[cls]([p], lr=1e-2)
+    opt.param_groups[0]["lr"] = -1.0
+    with pytest.raises(RuntimeError, match="lr"):
+        opt.step()
+    assert torch.equal(p, before) and opt.state[p].get("step", 0) == 0
+    opt.param_groups[0]["lr"] = 1e-2
+    opt.step()
+    assert opt.state[p]["step"] == 1 and not torch.equal(p, before)
+
+
 def test_copies_of_an_optimizer_clip_as_it_does():
     for cls in _classes():
         p = torch.nn.Parameter(torch.ones(100, device="cuda"))
