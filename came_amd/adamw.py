@@ -145,7 +145,7 @@ class _AdamWBase(torch.optim.Optimizer):
             descs, used, k = (_lib.Came8AdamwTensor * len(items))(), [], 0
             for p, g, state, moments in items:
                 copy = None if p.data.is_contiguous() else p.data.contiguous()
-                g = g.contiguous()
+                g = g.resolve_neg().contiguous()
                 used.append((p, copy, g, state))
                 if p.numel() == 0:
                     continue

@@ -276,7 +276,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     PyObject* so = st != nullptr && PyDict_Check(st) ? PyDict_GetItemWithError(st, k_step) : nullptr;
     int over = 0;
     const long step = so != nullptr && PyLong_CheckExact(so) ? PyLong_AsLongAndOverflow(so, &over) : -1;
-    if (step < 0 || over != 0) {
+    if (step < 0 || over != 0 || grads[i].is_neg()) {
       PyErr_Clear();
       Py_RETURN_NONE;
     }
@@ -435,7 +435,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
       if (ctx->needs_input_grad(i))
         grads[i] = T > 0 ? at::empty(ops[i]->sizes(), ops[i]->options()) : at::zeros(ops[i]->sizes(), ops[i]->options());
     if (T > 0 && dys[0].defined()) {
-      at::Tensor dy = dys[0].contiguous();
+      at::Tensor dy = dys[0].resolve_neg().contiguous();
       if (reinterpret_cast<uintptr_t>(dy.data_ptr()) % 4 != 0) dy = dy.clone(at::MemoryFormat::Contiguous);
       size_t bytes = 0;
       const at::Tensor ws = ffn_workspace(o.f, true, dy, &bytes);

@@ -137,6 +137,25 @@ def test_a_refused_step_is_not_counted(cls, transposed):
     assert opt.state[p]["step"] == 1 and not torch.equal(p, before)
 
 
+def test_gradients_that_are_negative_views():
+    import came_amd
+    ops = [torch.randn(*s, device="cuda") for s in ((5, 16), (24, 16), (24, 16), (16, 24))]
+    dy = torch.randn(5, 16, device="cuda")
+    a, b = ([t.clone().requires_grad_() for t in ops] for _ in range(2))
+    came_amd.gated_ffn(*a).backward(torch._neg_view(dy))
+    came_amd.gated_ffn(*b).backward(-dy)
+    assert all(torch.equal(s.grad, t.grad) for s, t in zip(a, b))
+    for cls in _classes():
+        p, q = (torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(2))
+        g = torch.randn(300, device="cuda")
+        p.grad, q.grad = torch._neg_view(g), -g
+        a, b = cls([p], lr=0.1), cls([q], lr=0.1)
+        for _ in range(2):  # the second with the states that the first has made
+            a.step()
+            b.step()
+            assert torch.equal(p, q)
+
+
 def test_copies_of_an_optimizer_clip_as_it_does():
     for cls in _classes():
         p = torch.nn.Parameter(torch.ones(100, device="cuda"))
