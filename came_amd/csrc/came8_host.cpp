@@ -346,14 +346,15 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   c10::OptionalDeviceGuard guard(first.device());
   const int32_t n = int32_t(descs.size());
   const size_t bytes = entries.norm_size(n);
-  const at::Tensor ws = at::empty({int64_t(bytes / 4) + 2}, first.options().dtype(at::kFloat).requires_grad(false));
-  float* out = ws.data_ptr<float>() + bytes / 4;  // the two scalars
-  entry_check((scale ? entries.clip : entries.norm)(descs.data(), n, max_norm, out, out + 1, ws.data_ptr(), bytes,
+  const at::TensorOptions options = first.options().dtype(at::kFloat).requires_grad(false);
+  const at::Tensor ws = at::empty({int64_t(bytes / 4)}, options);
+  const at::Tensor out = at::empty({2}, options);  // not in the workspace: a program may keep every step's norm
+  float* norm = out.data_ptr<float>();
+  entry_check((scale ? entries.clip : entries.norm)(descs.data(), n, max_norm, norm, norm + 1, ws.data_ptr(), bytes,
                                                     reinterpret_cast<void*>(stream)),
               scale ? "came8_grad_clip" : "came8_grad_norm");
   for (c10::TensorImpl* t : scaled) written(t);
-  const int64_t at = int64_t(bytes / 4);
-  return Py_BuildValue("NN", THPVariable_Wrap(ws.select(0, at)), THPVariable_Wrap(ws.narrow(0, at + 1, 1)));
+  return Py_BuildValue("NN", THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out.narrow(0, 1, 1)));
   END_HANDLE_TH_ERRORS
 }
 

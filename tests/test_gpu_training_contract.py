@@ -156,6 +156,17 @@ def test_gradients_that_are_negative_views():
             assert torch.equal(p, q)
 
 
+def test_a_kept_norm_keeps_no_workspace():
+    """A program that keeps every step's norm keeps a few bytes a step."""
+    import came_amd
+    p = torch.nn.Parameter(torch.zeros(100, device="cuda"))
+    p.grad = torch.ones(100, device="cuda")
+    opt = came_amd.AdamW([p], max_grad_norm=1.0)
+    opt.step()
+    for norm in (came_amd.grad_norm([p.grad]), came_amd.clip_grad_norm_([p], 1.0), opt.last_grad_norm):
+        assert norm.untyped_storage().nbytes() <= 8
+
+
 def test_copies_of_an_optimizer_clip_as_it_does():
     for cls in _classes():
         p = torch.nn.Parameter(torch.ones(100, device="cuda"))
