@@ -73,6 +73,8 @@ def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = Fals
     and leaves them as they were (and waits for the GPU to know)."""
     if not float(max_norm) >= 0.0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if not isinstance(error_if_nonfinite, (bool, int)) or error_if_nonfinite not in (0, 1):  # torch's third argument is norm_type
+        raise TypeError(f"error_if_nonfinite must be a bool, got {error_if_nonfinite!r}; the norm is always the 2-norm")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     parameters = list(parameters)

@@ -169,3 +169,12 @@ def _two(p, q, **kw):
     p.grad, q.grad = torch.randn(5), torch.randn(7)
     opt.step()
     return opt
+
+
+@pytest.mark.parametrize("norm_type", [2.0, 1.0, 2, float("inf"), "inf"])
+def test_a_norm_type_in_torchs_place_is_refused(norm_type):
+    p = torch.nn.Parameter(torch.zeros(3))
+    with pytest.raises(TypeError, match="always the 2-norm"):
+        came_amd.clip_grad_norm_([p], 1.0, norm_type)
+    for flag in (True, False):
+        assert float(came_amd.clip_grad_norm_([p], 1.0, flag)) == 0.0
