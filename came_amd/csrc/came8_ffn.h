@@ -240,25 +240,44 @@ struct Stage {
   }
 };
 
-// fp32 values as three bf16 ones, each the rounding of what the ones before leave: their sum is the value to 2^-24 of it.  The
-// first two are bounded by bf16's largest value, so that one that would round to infinity leaves a rest, and infinities and NaN
-// get to the third, which meets the other operand's first alone: infinity times a number has the number's sign, and no part of
-// it cancels another.
+// fp32 values as three bf16 ones, each the rounding of what the ones before leave: their sum is the value to 2^-24 of it.
+//
+// LARGE: for values of any size.  The first part is bounded by bf16's largest value, so that a value that would round to infinity
+// leaves a rest.  An infinity is its sign, zero and itself: the third part meets the other operand's first alone, which has the
+// other's sign and is zero where that is (and below 2^-134), and the sign meets what is finite where the other operand is, so no
+// part of it cancels the infinity.  NaN gets to the third part as well.  Without LARGE no part is bounded: a thread looks
+// over its loads once (2048 tokens of 4096 and 11008 forward and backward 8.98 ms, 9.97 with every value bounded).
+constexpr float kLargestBf16 = 0x1.fep127f;
 struct Parts {
   uint32_t w[3];  // of two values, packed
 };
+template <bool LARGE>
 __device__ __forceinline__ Parts parts_of(float x, float y) {
-  constexpr float kLargest = 0x1.fep127f;
+  auto first = [](float v) {
+    if (!LARGE) return v;
+    const float most = __builtin_isinf(v) ? 1.0f : kLargestBf16;
+    return __builtin_amdgcn_fmed3f(v, -most, most);
+  };
+  auto second = [](float v) { return LARGE && __builtin_isinf(v) ? 0.0f : v; };
   Parts p;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    p.w[i] = uint32_t(BF16::store(__builtin_amdgcn_fmed3f(x, -kLargest, kLargest))) |
-             uint32_t(BF16::store(__builtin_amdgcn_fmed3f(y, -kLargest, kLargest))) << 16;
-    x -= BF16::elem(&p.w[i], 0);
-    y -= BF16::elem(&p.w[i], 1);
-  }
+  p.w[0] = uint32_t(BF16::store(first(x))) | uint32_t(BF16::store(first(y))) << 16;
+  x -= BF16::elem(&p.w[0], 0);
+  y -= BF16::elem(&p.w[0], 1);
+  p.w[1] = uint32_t(BF16::store(second(x))) | uint32_t(BF16::store(second(y))) << 16;
+  x -= BF16::elem(&p.w[1], 0);
+  y -= BF16::elem(&p.w[1], 1);
   p.w[2] = uint32_t(BF16::store(x)) | uint32_t(BF16::store(y)) << 16;
   return p;
+}
+
+// the largest magnitude of a thread's loads and `top`; NaN if there is one
+template <int R, int NT, bool ROWS, int HALF>
+__device__ __forceinline__ float largest(const Stage<F32, R, NT, ROWS, HALF>& s, float top) {
+#pragma unroll
+  for (int i = 0; i < Stage<F32, R, NT, ROWS, HALF>::kLoads; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, __builtin_fabsf(__uint_as_float(s.v[i][e])));
+  return top;
 }
 
 // Rows of three parts in LDS: 64 bytes each, 32 values of k.  Chunk c of row r lies at c ^ part_swz(r), so that the lanes of a
@@ -267,7 +286,7 @@ constexpr int kPartBytes = 64, kPartRow = 3 * kPartBytes;
 __host__ __device__ constexpr int part_swz(int r) { return (4 - (r >> 2 & 3)) & 3; }
 
 // Stage::put for rows of parts
-template <int R, int NT, bool ROWS, int HALF>
+template <bool LARGE, int R, int NT, bool ROWS, int HALF>
 __device__ __forceinline__ void put_parts(const Stage<F32, R, NT, ROWS, HALF>& s, char* lds) {
   using St = Stage<F32, R, NT, ROWS, HALF>;
   const int t = int(threadIdx.x);
@@ -277,8 +296,8 @@ __device__ __forceinline__ void put_parts(const Stage<F32, R, NT, ROWS, HALF>& s
 #pragma unroll
     for (int i = 0; i < St::kLoads; ++i) {
       const int row = r + (HALF == 0 ? i * St::kStep : i / 2 * 2 * St::kStep + (i & 1) * HALF);
-      const Parts a = parts_of(__uint_as_float(s.v[i][0]), __uint_as_float(s.v[i][1]));
-      const Parts b = parts_of(__uint_as_float(s.v[i][2]), __uint_as_float(s.v[i][3]));
+      const Parts a = parts_of<LARGE>(__uint_as_float(s.v[i][0]), __uint_as_float(s.v[i][1]));
+      const Parts b = parts_of<LARGE>(__uint_as_float(s.v[i][2]), __uint_as_float(s.v[i][3]));
       char* at = lds + row * kPartRow + ((c >> 1) ^ part_swz(row)) * kChunkBytes + (c & 1) * 8;
 #pragma unroll
       for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(at + p * kPartBytes) = u32x2{a.w[p], b.w[p]};
@@ -288,9 +307,9 @@ __device__ __forceinline__ void put_parts(const Stage<F32, R, NT, ROWS, HALF>& s
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       char* at = lds + (r + e) * kPartRow + ((k >> 3) ^ part_swz(r + e)) * kChunkBytes + (k & 7) * 2;
-      const Parts a = parts_of(__uint_as_float(s.v[0][e]), __uint_as_float(s.v[1][e]));
+      const Parts a = parts_of<LARGE>(__uint_as_float(s.v[0][e]), __uint_as_float(s.v[1][e]));
       if constexpr (St::kLoads == 4) {
-        const Parts b = parts_of(__uint_as_float(s.v[2][e]), __uint_as_float(s.v[3][e]));
+        const Parts b = parts_of<LARGE>(__uint_as_float(s.v[2][e]), __uint_as_float(s.v[3][e]));
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(at + p * kPartBytes) = u32x2{a.w[p], b.w[p]};
       } else {
@@ -400,7 +419,7 @@ struct Tile {
 //
 // fp32 at BM = 256: the matrix instructions of fp32 run at a sixteenth of bf16's rate.  The operands are taken apart into three
 // bf16 parts on their way to LDS, and the six products of parts down to 2^-16 of the largest, summed in fp32, are a product
-// of fp32's accuracy at a sixth of bf16's rate: 2048 tokens of 4096 and 11008 forward and backward 9.6 ms (173
+// of fp32's accuracy at a sixth of bf16's rate: 2048 tokens of 4096 and 11008 forward and backward 9.0 ms (185
 // TFLOP/s) against 12.4.
 template <typename T, int BM, int WAVES_N, bool AROWS, bool BROWS, Epilogue EPI, bool ODD = false>
 __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) {
@@ -487,8 +506,14 @@ __device__ __forceinline__ void product(const GemmArgs& args, int b, char* lds) 
     fetch(0);
     for (int t = 0; t < total; ++t) {
       char* at = lds + (t & 1) * kTileBytes;
-      put_parts(sa[0], at);
-      put_parts(sb[0], at + BM * kPartRow);
+      const bool large = !(largest(sb[0], largest(sa[0], 0.0f)) <= kLargestBf16);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(large) == 0, 1)) {
+        put_parts<false>(sa[0], at);
+        put_parts<false>(sb[0], at + BM * kPartRow);
+      } else {
+        put_parts<true>(sa[0], at);
+        put_parts<true>(sb[0], at + BM * kPartRow);
+      }
       fetch(0);
       __syncthreads();  // the other buffer's last reads are behind every wavefront that has come here
       const int r = lane % 16, place = r * kPartRow + (lane / 16 ^ part_swz(r)) * kChunkBytes;
