@@ -769,8 +769,8 @@ __global__ __launch_bounds__(kThreads) void k_ffn_join_grads(const GradArgs args
 // 90 MB of down (4.9 and 4.1 TB/s), 60 together, 75 in tiles; 2 or 8 steps in flight and 16 wavefronts changed nothing.  With
 // 32 rows it took 89 us, tiles 66: x then costs more loads than the weights.
 //
-// h between the two is kept in fp32: as an operand it is its rounding to the type and the rest's, two products, which the
-// weights' way hides, so that y is rounded once.
+// h between the two is kept in fp32: as an operand it is its rounding to the type and the rest's, two products with sums of
+// their own, which the weights' way hides, so that y is rounded once.  What the type rounds to infinity is infinite there too.
 struct FewArgs {
   const void* x;     // down: h, float
   int64_t ldx;
@@ -828,19 +828,20 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
   using raw = AnyChunk<T>;
   constexpr int V = kChunkBytes / int(sizeof(S)), BK = kRowBytes / int(sizeof(S)), G = GATE ? 2 : 1, NW = 8;
   constexpr int U = 4;  // steps in flight
-  __shared__ f32x4 sums[NW][G][kWave];
+  constexpr bool kSplit = !GATE && sizeof(S) == 2;  // x is h in fp32, in two 16-bit parts
+  constexpr int A = kSplit ? 2 : G;                 // kSplit: sums of h's rounding and of its rest
+  __shared__ f32x4 sums[NW][A][kWave];
   const int lane = int(threadIdx.x) % kWave, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int n0 = int(blockIdx.x) * 16, q = lane / 16 * 2 * V;
   const CAME8_GLOBAL S* w[G];  // rows past the end are not stored: any row will do
 #pragma unroll
   for (int i = 0; i < G; ++i)
     w[i] = gbl(static_cast<const S*>(args.w[i])) + int64_t(min(n0 + lane % 16, args.N - 1)) * args.ldw[i] + q;
-  constexpr bool kSplit = !GATE && sizeof(S) == 2;  // x is h in fp32, in two 16-bit parts
   using X = typename std::conditional<GATE, S, float>::type;
   constexpr int P = kSplit ? 2 : 1;
   const CAME8_GLOBAL X* x = gbl(static_cast<const X*>(args.x)) + int64_t(min(lane % 16, args.M - 1)) * args.ldx + q;
 
-  f32x4 acc[G] = {};
+  f32x4 acc[A] = {};
   const int full = args.K / BK;
   for (int s0 = wave; s0 < full; s0 += NW * U) {
     u32x4 wv[U][G][2], xv[U][2][P];
@@ -868,7 +869,7 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
             u32x4 high, low;
             split_chunk<T>(__builtin_bit_cast(f32x4, xv[u][c][0]), __builtin_bit_cast(f32x4, xv[u][c][1]), high, low);
             acc[0] = mfma_chunk<T>(wv[u][0][c], high, acc[0]);
-            acc[0] = mfma_chunk<T>(wv[u][0][c], low, acc[0]);
+            acc[1] = mfma_chunk<T>(wv[u][0][c], low, acc[1]);
           } else {
 #pragma unroll
             for (int g = 0; g < G; ++g) acc[g] = mfma_chunk<T>(wv[u][g][c], xv[u][c][0], acc[g]);
@@ -885,7 +886,7 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
                        __builtin_bit_cast(f32x4, load_chunk<F32>(x, k + c * V + 4, left)), high, low);
         const u32x4 wv = load_chunk<T>(w[0], k + c * V, left);
         acc[0] = mfma_chunk<T>(wv, high, acc[0]);
-        acc[0] = mfma_chunk<T>(wv, low, acc[0]);
+        acc[1] = mfma_chunk<T>(wv, low, acc[1]);
       } else {
         const u32x4 xv = load_chunk<T>(x, k + c * V, left);
 #pragma unroll
@@ -894,17 +895,22 @@ __global__ __launch_bounds__(512) void k_ffn_few(const FewArgs args) {
     }
   }
 #pragma unroll
-  for (int g = 0; g < G; ++g) sums[wave][g][lane] = acc[g];
+  for (int g = 0; g < A; ++g) sums[wave][g][lane] = acc[g];
   __syncthreads();
   if (wave != 0) return;
   const int m = lane % 16, n = n0 + lane / 16 * 4;
-  f32x4 total[G] = {};
+  f32x4 total[A] = {};
 #pragma unroll
   for (int i = 0; i < NW; ++i)
 #pragma unroll
-    for (int g = 0; g < G; ++g) total[g] += sums[i][g][lane];
+    for (int g = 0; g < A; ++g) total[g] += sums[i][g][lane];
   if (m >= args.M) return;
-  const float a[4] = {total[0][0], total[0][1], total[0][2], total[0][3]};
+  float a[4] = {total[0][0], total[0][1], total[0][2], total[0][3]};
+  if constexpr (kSplit) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // of an infinite weight the rest, zero or of either sign, says nothing
+      if (__builtin_isfinite(a[e])) a[e] += total[1][e];
+  }
   if constexpr (GATE) {
     const float b[4] = {total[1][0], total[1][1], total[1][2], total[1][3]};
     float h[4], none[4];

@@ -6,7 +6,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-F32 = torch.float32
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
 @pytest.fixture(autouse=True)
@@ -52,6 +52,24 @@ def test_fp32_infinity_times_infinity(T):
     with torch.no_grad():
         y = gated_ffn(*ops)
     assert (y == float("inf")).all()  # every other row: a positive number times infinity
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T", [1, 16, 17])
+def test_an_infinite_down_weight(T, dtype):
+    """An infinity in a row of w_down is an infinity, of h's sign, in that column of y, and in no other."""
+    from came_amd import gated_ffn
+    gen = torch.Generator().manual_seed(22)
+    x, wg, wu, wd = (torch.rand(*s, generator=gen).to(dtype).cuda() for s in ((T, 72), (100, 72), (100, 72), (40, 100)))
+    wu[7] = -wu[7]  # h of column 7 is negative
+    with torch.no_grad():
+        want = gated_ffn(x, wg, wu, wd)
+        bad = wd.clone()
+        bad[3, 7], bad[5, 99] = float("inf"), float("inf")
+        y = gated_ffn(x, wg, wu, bad)
+    assert (y[:, 3] == -float("inf")).all() and (y[:, 5] == float("inf")).all()
+    rest = [e for e in range(40) if e not in (3, 5)]
+    assert torch.equal(y[:, rest], want[:, rest])
 
 
 def test_large_fp32_products_of_small_values():
