@@ -315,7 +315,8 @@ size_t came8_grad_norm_workspace_size(int32_t n_tensors);
 int came8_grad_norm(const came8_grad_tensor* tensors, int32_t n_tensors, double max_norm, float* norm, float* factor,
                     void* workspace, size_t workspace_bytes, void* stream);
 
-/* came8_grad_norm, then every tensor times the factor, in place (nothing is written where the factor is 1). */
+/* came8_grad_norm, then every tensor times the factor, in place (nothing is written where the factor is 1); tensors that
+ * have memory in common one after another. */
 int came8_grad_clip(const came8_grad_tensor* tensors, int32_t n_tensors, double max_norm, float* norm, float* factor,
                     void* workspace, size_t workspace_bytes, void* stream);
 

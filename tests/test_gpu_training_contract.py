@@ -200,3 +200,23 @@ def test_a_checkpoint_of_a_transposed_parameter_continues():
         ref.step()
         opt.step()
     assert ((p - q).abs() <= 3 * (8 * u * p.abs() + 64 * u * lr)).all()
+
+
+@pytest.mark.parametrize("kind", ["again", "overlapping"])
+def test_gradients_that_share_memory_are_scaled_one_after_another(kind):
+    """As in torch, a gradient counts in the norm and is scaled as often as it is listed, and so is what two have in common."""
+    import came_amd
+    n = 40_000_000
+    buf = torch.randn(n + 1000, device="cuda")
+    views = {"again": [buf, buf, buf], "overlapping": [buf[1000:], buf[:n], buf[500:700]]}[kind]
+    before, times = buf.double(), torch.zeros(n + 1000, device="cuda", dtype=torch.float64)
+    want = float(torch.stack([v.double().square().sum() for v in views]).sum().sqrt())
+    params = []
+    for v in views:
+        params.append(torch.nn.Parameter(torch.empty_like(v)))
+        params[-1].grad = v
+        times[v.storage_offset() : v.storage_offset() + v.numel()] += 1
+    norm = came_amd.clip_grad_norm_(params, 0.5 * want)
+    assert abs(float(norm) / want - 1) < 1e-6
+    x = before * (0.5 * want / (want + 1e-6)) ** times
+    assert ((buf.double() - x).abs() <= x.abs() * (3 * 10 * 2.0**-24)).all()  # a factor and a product each time
