@@ -61,6 +61,12 @@ class _AdamWBase(torch.optim.Optimizer):
     def add_param_group(self, param_group: dict) -> None:
         if isinstance(param_group, dict):  # torch refuses others
             _refuse_options(param_group)
+            params = param_group.get("params")
+            if not isinstance(params, (torch.Tensor, set, type(None))):
+                params = param_group["params"] = list(params)
+                each = [p[1] if isinstance(p, tuple) else p for p in params]  # named ones are pairs
+                if len({id(p) for p in each}) != len(each):  # torch warns
+                    raise ValueError("a parameter appears twice in a param group: one launch would step it twice at the same time")
         super().add_param_group(param_group)
 
     # ------------------------------------------------------------------ state

@@ -178,3 +178,14 @@ def test_a_norm_type_in_torchs_place_is_refused(norm_type):
         came_amd.clip_grad_norm_([p], 1.0, norm_type)
     for flag in (True, False):
         assert float(came_amd.clip_grad_norm_([p], 1.0, flag)) == 0.0
+
+
+@pytest.mark.parametrize("cls", [came_amd.AdamW, came_amd.AdamW8bit])
+def test_a_parameter_that_appears_twice_is_refused(cls):
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    for params in ([p, q, p], iter([p, p]), [{"params": [q]}, {"params": (p, p)}], [{"params": iter([q, q])}],
+                   [("first", p), ("second", p)]):
+        with pytest.raises(ValueError, match="appears twice"):
+            cls(params)
+    for params in ([p, q], iter([p, q]), [{"params": iter([p])}, {"params": q}], [("first", p), ("second", q)]):
+        assert sum(len(g["params"]) for g in cls(params).param_groups) == 2
