@@ -96,25 +96,33 @@ class _AdamWBase(torch.optim.Optimizer):
         """Loads every state tensor in the type it was saved in (torch's loader casts them to the parameter's), contiguous (torch
         keeps the moments of a transposed or channels-last parameter in its order).  What is refused leaves the optimizer as it
         was."""
+        loaded: dict = {}
+        handle = self.register_load_state_dict_pre_hook(lambda _, given: self._look_over(given, loaded))  # after the user's
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            handle.remove()
+        for p, st in loaded.items():
+            self.state[p].update(st)
+
+    def _look_over(self, state_dict: dict, loaded: dict) -> None:
+        """What a state_dict holds for each parameter, checked before anything changes."""
         groups, saved = state_dict["param_groups"], state_dict["state"]
         for g in groups:
             _refuse_options(g)
-        loaded = {}  # all of it looked over before anything changes
-        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:  # torch's loader raises else
-            for g, own in zip(groups, self.param_groups):
-                for k, p in zip(g["params"], own["params"]):
-                    if not saved.get(k):
-                        continue
-                    st = loaded[p] = {}
-                    for key, v in saved[k].items():
-                        if key == "step":  # torch.optim keeps a tensor
-                            st[key] = int(v)
-                        elif isinstance(v, torch.Tensor):
-                            st[key] = v.detach().to(device=p.device, copy=True, memory_format=torch.contiguous_format)
-                    self._moments(st, p, g)
-        super().load_state_dict(state_dict)
-        for p, st in loaded.items():
-            self.state[p].update(st)
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            return  # torch's loader raises
+        for g, own in zip(groups, self.param_groups):
+            for k, p in zip(g["params"], own["params"]):
+                if not saved.get(k):
+                    continue
+                st = loaded[p] = {}
+                for key, v in saved[k].items():
+                    if key == "step":  # torch.optim keeps a tensor
+                        st[key] = int(v)
+                    elif isinstance(v, torch.Tensor):
+                        st[key] = v.detach().to(device=p.device, copy=True, memory_format=torch.contiguous_format)
+                self._moments(st, p, g)
 
     # ------------------------------------------------------------------- step
     def _hparams(self, group: dict) -> _lib.Came8AdamwHParams:

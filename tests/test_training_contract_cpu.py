@@ -189,3 +189,18 @@ def test_a_parameter_that_appears_twice_is_refused(cls):
             cls(params)
     for params in ([p, q], iter([p, q]), [{"params": iter([p])}, {"params": q}], [("first", p), ("second", q)]):
         assert sum(len(g["params"]) for g in cls(params).param_groups) == 2
+
+
+def test_hooks_of_a_load_are_heard():
+    p = torch.nn.Parameter(torch.zeros(5, dtype=torch.bfloat16))
+    saved = _stepped(torch.nn.Parameter(torch.zeros(5))).state_dict()
+    opt = came_amd.AdamW([p])
+
+    def hook(_, given):
+        state = {k: {key: v if key == "step" else v + 1 / 3 for key, v in st.items()} for k, st in given["state"].items()}
+        return {**given, "state": state}
+
+    opt.register_load_state_dict_pre_hook(hook)
+    opt.load_state_dict(saved)
+    for key in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(opt.state[p][key], saved["state"][0][key] + 1 / 3)
