@@ -11,6 +11,7 @@ with Q = 127 (signed) or uint8 codes with Q = 255 (unsigned),
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -50,6 +51,11 @@ def _require_cuda(t: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what}: came_amd runs on the GPU; got a {t.device} tensor")
 
 
+def _on(device: torch.device):
+    """torch.cuda.device where another device is current: it takes a microsecond of host time."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _require_absmax(q: torch.Tensor, absmax: torch.Tensor, block_size: int, what: str) -> None:
     """The kernels read it on the codes' GPU: a host address, or another GPU's, faults there."""
     if absmax.device != q.device:
@@ -85,7 +91,7 @@ def dequantize_blockwise(q: torch.Tensor, absmax: torch.Tensor, *, signed: bool,
     qc = q.contiguous()
     ac = absmax.to(torch.float32).contiguous()
     out = torch.empty(qc.shape, device=qc.device, dtype=torch.float32)
-    with torch.cuda.device(qc.device):
+    with _on(qc.device):
         stream = torch.cuda.current_stream(qc.device).cuda_stream
         _lib.check(
             lib.came8_dequantize_blockwise(qc.data_ptr(), ac.data_ptr(), qc.numel(), int(bool(signed)),
@@ -107,7 +113,7 @@ def dequantize_second_moment(q: torch.Tensor, absmax: torch.Tensor, *, block_siz
     qc = q.contiguous()
     ac = absmax.to(torch.float32).contiguous()
     out = torch.empty(qc.shape, device=qc.device, dtype=torch.float32)
-    with torch.cuda.device(qc.device):
+    with _on(qc.device):
         stream = torch.cuda.current_stream(qc.device).cuda_stream
         _lib.check(
             lib.came8_dequantize_second_moment(qc.data_ptr(), ac.data_ptr(), qc.numel(), int(block_size), out.data_ptr(),

@@ -38,7 +38,7 @@ def _contiguous(tensors: list, what: str):
 
 def _reduce(tensors: list, max_norm: float | None, scale: bool, what: str, of_parameters: bool = False):
     """(norm, factor): device scalars of one call over the tensors, or the parameters' gradients; with `scale` those are
-    multiplied in place.  None where no parameter has a gradient."""
+    multiplied in place, and factor is None.  None where no parameter has a gradient."""
     device = next((t.device for t in tensors if not of_parameters or t.grad is not None), None)
     if device is None:
         return None
