@@ -20,7 +20,7 @@ namespace came8 {
 namespace {
 
 constexpr int kAdamTab = 64;    // tensors a launch: 60 bytes each of the 4 KB of arguments
-constexpr int kGradTab = 192;   // 20 bytes each
+constexpr int kGradTab = 192;   // 18 bytes each; a multiple of a wavefront's lanes (find_tensor)
 // Elements of a workgroup: 256 lanes by 8 by 4 rows; a launch that has fewer than kSmallLaunch of those takes single rows (or
 // as few as a block of 8-bit moments needs), since then only its latency counts: 192 adapters of 10 to 33 thousand elements,
 // three launches of 11.2 us in 4 rows and of 7.4 in single ones.

@@ -127,6 +127,8 @@ constexpr int kRowBytes = 128;  // of a tile in LDS: 8 chunks, 64 (fp32: 32) val
 // 12-15, 20-23 and 24-27 go together (and 4-11, 16-19, 28-31).  With a fragment's lanes, row l % 16 and chunk l / 16, these
 // are 16 different places of two rows' length, all 64 banks once; eight lanes that write a chunk of rows 8 apart (columns on
 // their way in) touch eight places.  (With places that only 8 lanes in order tell apart, every read took twice its time.)
+// By the counters, launches of rows alone have conflicts in 0 to 1% of their LDS cycles, those with columns, whose writes are 8
+// bytes a lane in tiles of 256, in 24% (the gradients) and 16% (dy Wd): 8192 tokens of 4096 and 11008 in bf16.
 // swz is linear: of rows whose bits do not overlap it is the exclusive or.
 __host__ __device__ constexpr int swz(int r) { return (r >> 3 & 1) | ((r ^ r >> 4) & 2) | ((r ^ r >> 1 ^ r >> 2) & 4); }
 

@@ -1,10 +1,11 @@
 """The gated feed-forward block ``y = (act(x Wg^T) * (x Wu^T)) Wd^T`` with its gradients, in libcame8.
 
 Both projections, the activation and the product are one kernel, the down projection another; backward, the activation's
-gradient is formed where the product ``dy Wd`` ends, and no operand is copied or transposed in memory (16-bit matrices of
-an odd row stride, and rows that end inside 16 bytes, are copied to aligned ones).  Kept for the backward pass: ``x`` and,
-in float32, ``x Wg^T`` and ``x Wu^T`` (8 bytes a hidden value); the product ``h`` is formed again.  The autograd node is
-native (csrc/came8_host.cpp).
+gradient is formed where the product ``dy Wd`` ends, and no operand is transposed in memory.  Calls of more than 16 tokens
+copy rows that end inside 16 bytes, and 16-bit matrices of an odd row stride, to aligned ones; the forward pass reads an
+odd-strided ``w_down`` where it is unless there are many tokens.  Kept for the backward pass: the operands and, in float32,
+``x Wg^T`` and ``x Wu^T`` (8 bytes a hidden value); the product ``h`` is formed again.  The autograd node is native
+(csrc/came8_host.cpp).
 """
 from __future__ import annotations
 

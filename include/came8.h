@@ -372,7 +372,8 @@ int came8_dequantize_second_moment(const uint8_t* q, const float* absmax, int64_
  *   dh = dy w_down,  dg = dh * u * act'(g),  du = dh * act(g)
  *   dx = dg w_gate + du w_up,  dw_gate = dg^T x,  dw_up = du^T x,  dw_down = dy^T h
  * Sums are held in fp32.  h, dg and du are rounded to dtype once: they are operands of products of that type (h of up to 16
- * tokens, forward, is not rounded); g and u enter h and the gradients unrounded.  Every pointer is 4 bytes aligned.  No counterpart in the reference.
+ * tokens, forward, is not rounded, but infinite where its rounding is); g and u enter h and the gradients unrounded.  Every
+ * pointer is 4 bytes aligned.  No counterpart in the reference.
  */
 #define CAME8_ACT_SILU 0
 #define CAME8_ACT_GELU 1      /* the exact one, by erf */
