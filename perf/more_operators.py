@@ -226,7 +226,7 @@ def _int8_plain(s):
         out["h"] = h
     top = y.abs().amax(-1, keepdim=True)
     some = top >= TINY
-    q = torch.round(y * torch.where(some, 127.0 / top, torch.zeros_like(top)))
+    q = torch.round(y * torch.where(some, torch.full_like(top, 127.0) / top, torch.zeros_like(top)))
     z = (q @ s["wq"].float().t()) * torch.where(some, top / 127.0, torch.zeros_like(top)) * s["ws"]
     if s["bias"] is not None:
         z = z + s["bias"].float()
