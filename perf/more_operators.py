@@ -220,14 +220,18 @@ def _norm_plain(s):
 
 def _int8_plain(s):
     h, out = _add(s), {}
-    y = h.float()
+    y = h.double()  # next to a border between two codes, 32 bits take the other one; what scales the row moves no code
     if s["case"]["norm"]:
-        y = y * (1 / torch.sqrt((y * y).mean(-1, keepdim=True) + EPS)) * s["weight"].float()
+        y = y * s["weight"].double()
         out["h"] = h
     top = y.abs().amax(-1, keepdim=True)
     some = top >= TINY
-    q = torch.round(y * torch.where(some, torch.full_like(top, 127.0) / top, torch.zeros_like(top)))
-    z = (q @ s["wq"].float().t()) * torch.where(some, top / 127.0, torch.zeros_like(top)) * s["ws"]
+    q = torch.round(torch.where(some, y * 127.0 / top, torch.zeros_like(y))).float()
+    scale = torch.where(some, top / 127.0, torch.zeros_like(top)).float()
+    if s["case"]["norm"]:
+        hf = h.float()
+        scale = scale * (1 / torch.sqrt((hf * hf).mean(-1, keepdim=True) + EPS))
+    z = (q @ s["wq"].float().t()) * scale * s["ws"]
     if s["bias"] is not None:
         z = z + s["bias"].float()
     out["y"] = z.to(h.dtype)
@@ -361,14 +365,15 @@ def _exact_norm(case, s):
 
 
 def _exact_int8(case, s):
-    x, out = s["x"], {}
+    x, out, scale = s["x"], {}, 1.0 / 127
     y = x.double()
     if case["norm"]:
         out["h"] = h = (y + s["residual"].double()).to(x.dtype).double()
-        y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + EPS) * s["weight"].double()
-    scale = y.abs().amax(-1, keepdim=True) / 127
-    codes = torch.where(scale > 0, torch.round(y / scale), torch.zeros_like(y))
-    z = torch.mm(codes, s["wq"].double().t().contiguous()) * scale * s["ws"].double()
+        scale = scale * torch.rsqrt(h.square().mean(-1, keepdim=True) + EPS)
+        y = h * s["weight"].double()
+    top = y.abs().max(-1, keepdim=True).values
+    codes = torch.where(top > 0, torch.round(127 * y / top), torch.zeros_like(y))
+    z = torch.mm(codes, s["wq"].double().t().contiguous()) * (scale * top) * s["ws"].double()
     out["y"] = z if s["bias"] is None else z + s["bias"].double()
     return out
 
