@@ -51,7 +51,32 @@ EXPORTED_SYMBOLS = (
     "came8_gated_ffn_workspace_size",
     "came8_gated_ffn_forward",
     "came8_gated_ffn_backward",
+    "came8_embedding_forward",
+    "came8_embedding_workspace_size",
+    "came8_embedding_backward",
+    "came8_rms_norm_forward",
+    "came8_rms_norm_workspace_size",
+    "came8_rms_norm_backward",
+    "came8_rms_norm_int8",
+    "came8_quantize_rows",
+    "came8_int8_linear_workspace_size",
+    "came8_int8_linear_forward",
+    "came8_log_probs_workspace_size",
+    "came8_log_probs_forward",
+    "came8_log_probs_backward",
 )
+
+# the entries that csrc/came8_host.h has, in its order
+HOST_ENTRIES = (
+    "came8_last_error",
+    "came8_adamw_step",
+    "came8_grad_norm_workspace_size",
+    "came8_grad_norm",
+    "came8_grad_clip",
+    "came8_gated_ffn_workspace_size",
+    "came8_gated_ffn_forward",
+    "came8_gated_ffn_backward",
+) + EXPORTED_SYMBOLS[EXPORTED_SYMBOLS.index("came8_embedding_forward"):]
 
 
 class Came8Tensor(ctypes.Structure):
@@ -152,6 +177,35 @@ class Came8Ffn(ctypes.Structure):
     _fields_ += [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32)]
 
 
+class Came8Embedding(ctypes.Structure):
+    """Mirror of ``came8_embedding`` (include/came8.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("tokens", "vocab", "dim", "ld_weight", "padding")]
+    _fields_ += [("scale", ctypes.c_float)]
+    _fields_ += [(name, ctypes.c_int32) for name in ("dtype", "token_bytes", "reserved")]
+
+
+class Came8RmsNorm(ctypes.Structure):
+    """Mirror of ``came8_rms_norm`` (include/came8.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("rows", "dim", "ld_x", "ld_residual")]
+    _fields_ += [("eps", ctypes.c_double), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class Came8Int8Linear(ctypes.Structure):
+    """Mirror of ``came8_int8_linear`` (include/came8.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("rows", "in", "out", "ld_q", "ld_w")]
+    _fields_ += [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class Came8LogProbs(ctypes.Structure):
+    """Mirror of ``came8_log_probs`` (include/came8.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in ("rows", "vocab", "ld")]
+    _fields_ += [(name, ctypes.c_int32) for name in ("dtype", "token_bytes", "top", "reserved")]
+
+
 class Came8PhaseStat(ctypes.Structure):
     """Mirror of ``came8_phase_stat`` (include/came8.h)."""
 
@@ -238,6 +292,24 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.came8_gated_ffn_forward.argtypes = [ctypes.POINTER(Came8Ffn), vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
         lib.came8_gated_ffn_backward.restype = ctypes.c_int
         lib.came8_gated_ffn_backward.argtypes = [ctypes.POINTER(Came8Ffn)] + [vp] * 12 + [sz, vp]
+        for name, desc, pointers, space in (
+            ("embedding_forward", Came8Embedding, 3, False), ("embedding_backward", Came8Embedding, 3, True),
+            ("rms_norm_forward", Came8RmsNorm, 5, False), ("rms_norm_backward", Came8RmsNorm, 6, True),
+            ("int8_linear_forward", Came8Int8Linear, 6, True), ("log_probs_forward", Came8LogProbs, 7, True),
+            ("log_probs_backward", Came8LogProbs, 7, False),
+        ):
+            fn = getattr(lib, "came8_" + name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(desc)] + [vp] * pointers + ([vp, sz] if space else []) + [vp]
+        for name, desc in (("embedding", Came8Embedding), ("rms_norm", Came8RmsNorm), ("int8_linear", Came8Int8Linear),
+                           ("log_probs", Came8LogProbs)):
+            fn = getattr(lib, f"came8_{name}_workspace_size")
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(desc), ctypes.POINTER(sz)]
+        lib.came8_rms_norm_int8.restype = ctypes.c_int
+        lib.came8_rms_norm_int8.argtypes = [ctypes.POINTER(Came8RmsNorm)] + [vp] * 4 + [i64] + [vp] * 3
+        lib.came8_quantize_rows.restype = ctypes.c_int
+        lib.came8_quantize_rows.argtypes = [ctypes.POINTER(Came8RmsNorm), vp, vp, i64, vp, vp]
         if lib.came8_abi_version() != ABI_VERSION:
             raise RuntimeError(f"came_amd: {p} has ABI {lib.came8_abi_version()}, expected {ABI_VERSION}")
         _lib = lib
@@ -258,12 +330,18 @@ def host():
                 spec = importlib.util.spec_from_file_location("came8_host", HOST_PATH)
                 mod = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(mod)
-                mod.bind(*(ctypes.cast(entry, ctypes.c_void_p).value for entry in (
-                    lib.came8_last_error, lib.came8_adamw_step, lib.came8_grad_norm_workspace_size, lib.came8_grad_norm,
-                    lib.came8_grad_clip, lib.came8_gated_ffn_workspace_size, lib.came8_gated_ffn_forward,
-                    lib.came8_gated_ffn_backward)))
+                mod.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in HOST_ENTRIES))
                 _host = mod
     return _host
+
+
+def current(t) -> tuple[int, bool]:
+    """The stream that is current on the tensor's device, and whether it is being captured (0, False where it is on no GPU)."""
+    import torch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        return 0, False
+    return torch.cuda.current_stream(t.device).cuda_stream, torch.cuda.is_current_stream_capturing()
 
 
 def check(rc: int, what: str) -> None:

@@ -38,12 +38,16 @@ HIPCC_FLAGS = [
     "-Wno-unused-function",
 ]
 
-# translation units: the host code with the flat-pass kernels, AdamW with the gradient norm, the feed-forward block,
-# and one per band-pass family
-UNITS = [("came8", "came8.hip", []), ("adamw", "came8_adamw.hip", []), ("ffn", "came8_ffn.hip", [])] + [
+# translation units: the host code with the flat-pass kernels, AdamW with the gradient norm, the feed-forward block, what a
+# language model has around it, and one per band-pass family
+UNITS = [("came8", "came8.hip", []), ("adamw", "came8_adamw.hip", []), ("ffn", "came8_ffn.hip", []), ("embed", "came8_embed.hip", []),
+         ("rms", "came8_rms.hip", []), ("int8", "came8_int8.hip", []), ("logprob", "came8_logprob.hip", [])] + [
     (f"band_{t.lower()}_p{p}", "came8_band.hip", [f"-DCAME8_BAND_TYPE={t}", f"-DCAME8_BAND_PASS={p}"])
     for t in ("F32", "BF16", "F16") for p in (1, 2)
 ]
+
+
+HOST_UNITS = ["came8_host", "came8_host_lm"]  # of came8_host.so
 
 
 def hipcc() -> str:
@@ -53,18 +57,21 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-def host_cmd(out: str) -> list[str]:
-    """The compiler line of the host extension: plain C++ against torch's and Python's headers."""
+def host_cmds(out: str) -> tuple[list[list[str]], list[str]]:
+    """The compiler lines of the host extension, plain C++ against torch's and Python's headers: one for each source (to
+    the objects beside ``out``), and the one that links them."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
+    cc = shutil.which("g++") or "g++"
     inc = [f for i in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"]) for f in ("-isystem", i)]
-    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, "-o", out,
-            os.path.join(CSRC, "came8_host.cpp"), *(f"-L{p}" for p in cpp_extension.library_paths()),
-            "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    objs = [os.path.join(OUT_DIR, f"{name}.o") for name in HOST_UNITS]
+    compiles = [[cc, "-O2", "-std=c++17", "-fPIC", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc,
+                 "-c", "-o", obj, os.path.join(CSRC, f"{name}.cpp")] for name, obj in zip(HOST_UNITS, objs)]
+    return compiles, [cc, "-shared", "-o", out, *objs, *(f"-L{p}" for p in cpp_extension.library_paths()),
+                      "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
 def _run(cmd: list[str]) -> tuple[int, str]:
@@ -87,22 +94,24 @@ def build(verbose: bool = True, jobs: int | None = None) -> str:
         objs.append(obj)
         cmds.append([cc, *HIPCC_FLAGS, *defs, *inc, "-c", "-o", obj, os.path.join(CSRC, src)])
     host_tmp = HOST_OUT + ".tmp"
-    cmds.append(host_cmd(host_tmp))
+    host_compiles, host_link = host_cmds(host_tmp)
+    cmds += host_compiles
     jobs = jobs or min(len(cmds), os.cpu_count() or 1)
     if verbose:
         print(f"[came_amd.build] {len(cmds)} units, {jobs} parallel: {' '.join(cmds[0])}", flush=True)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         results = list(ex.map(_run, cmds))
-    for name, (rc, errs) in zip([u[0] for u in UNITS] + ["came8_host"], results):
+    for name, (rc, errs) in zip([u[0] for u in UNITS] + HOST_UNITS, results):
         if rc != 0:
             raise RuntimeError(f"compiling {name} failed ({rc}):\n{errs}")
         if verbose and errs.strip():
             print(errs, file=sys.stderr)
     tmp = OUT + ".tmp"
-    rc, errs = _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs])
-    if rc != 0:
-        raise RuntimeError(f"link failed ({rc}):\n{errs}")
-    for o in objs:
+    for link in ([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs], host_link):
+        rc, errs = _run(link)
+        if rc != 0:
+            raise RuntimeError(f"link failed ({rc}):\n{errs}")
+    for o in objs + [os.path.join(OUT_DIR, f"{name}.o") for name in HOST_UNITS]:
         os.remove(o)
     os.replace(tmp, OUT)
     os.replace(host_tmp, HOST_OUT)

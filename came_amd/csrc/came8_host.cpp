@@ -1,5 +1,5 @@
 // came8_host: descriptors of a param group's tensors for came8_step, filled natively; AdamW's step and the gradient norm with
-// theirs; and the gated feed-forward block as an autograd node.
+// theirs; and the gated feed-forward block as an autograd node.  (The operators around that block: came8_host_lm.cpp.)
 //
 // gather() does what the optimizers' Python does for every parameter of a group before a step (the checks of
 // _prepare_param and _check_state, the fields of _descriptors and _fill_desc, the step counts) for the plain case:
@@ -17,16 +17,20 @@
 
 #include <ATen/ATen.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <cstring>
 #include <string>
 #include <utility>
 #include <vector>
 
-#include "../../include/came8.h"
+#include "came8_host.h"
 
-namespace {
+namespace came8_host {
 
-PyObject* key(const char* name) { return PyUnicode_InternFromString(name); }
+Entries entries;
+
+void entry_check(int rc, const char* what) { TORCH_CHECK(rc == CAME8_OK, what, " failed (", rc, "): ", entries.error()); }
 
 int dtype_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -36,6 +40,33 @@ int dtype_code(const at::Tensor& t) {
     default: return -1;
   }
 }
+
+std::string dtype_name(const at::Tensor& t) {
+  const char* known[3] = {"torch.float32", "torch.bfloat16", "torch.float16"};
+  const int code = dtype_code(t);
+  return code >= 0 ? known[code] : c10::toString(t.scalar_type());
+}
+
+torch::autograd::variable_list differentiable_once(torch::autograd::variable_list grads, const char* what) {
+  const size_t n = grads.size();
+  auto once = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", int(n));
+  torch::autograd::variable_list in(n);
+  for (size_t i = 0; i < n; ++i)
+    if (grads[i].defined()) in[i] = grads[i].detach().set_requires_grad(true);
+  at::AutoGradMode grad(true);
+  auto marked = (*once)(std::move(in));
+  for (size_t i = 0; i < n; ++i)
+    if (grads[i].defined()) grads[i] = marked[i];
+  return grads;
+}
+
+}  // namespace came8_host
+
+using namespace came8_host;
+
+namespace {
+
+PyObject* key(const char* name) { return PyUnicode_InternFromString(name); }
 
 // the tensor under `name` in a state, or null (borrowed)
 const at::Tensor* tensor_of(PyObject* st, PyObject* name) {
@@ -220,20 +251,6 @@ PyObject* gather(PyObject*, PyObject* args) {
   }
 }
 
-// libcame8's entries, which Python has loaded
-struct Entries {
-  decltype(&came8_last_error) error = nullptr;
-  decltype(&came8_adamw_step) adamw = nullptr;
-  decltype(&came8_grad_norm_workspace_size) norm_size = nullptr;
-  decltype(&came8_grad_norm) norm = nullptr;
-  decltype(&came8_grad_clip) clip = nullptr;
-  decltype(&came8_gated_ffn_workspace_size) ffn_size = nullptr;
-  decltype(&came8_gated_ffn_forward) ffn_forward = nullptr;
-  decltype(&came8_gated_ffn_backward) ffn_backward = nullptr;
-} entries;
-
-void entry_check(int rc, const char* what) { TORCH_CHECK(rc == CAME8_OK, what, " failed (", rc, "): ", entries.error()); }
-
 // A tensor that a kernel has written, for the nodes that have saved it (gated_ffn its weights); inference tensors have no
 // version.
 void written(c10::TensorImpl* t) {
@@ -366,12 +383,6 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
 // ------------------------------------------------------------------------------------------- gated feed-forward block
 // The block as an autograd node.  In Python its backward pass, which runs on a thread of the engine's, waits for the
 // interpreter's lock twice: 198 us of host time for 4 tokens of 256 and 512 forward and backward, 81 natively.
-std::string dtype_name(const at::Tensor& t) {
-  const char* known[3] = {"torch.float32", "torch.bfloat16", "torch.float16"};
-  const int code = dtype_code(t);
-  return code >= 0 ? known[code] : c10::toString(t.scalar_type());
-}
-
 // A 2-D tensor whose rows are contiguous and do not overlap, at a 4-byte aligned address: itself, or a copy where it is not
 // or where its rows lie too far apart for the kernels.
 at::Tensor rows_of(const at::Tensor& t) {
@@ -453,14 +464,8 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
                 "came8_gated_ffn_backward");
     }
     if (again) {
-      auto once = std::make_shared<torch::autograd::DelayedError>("gated_ffn is differentiable once", 4);
-      torch::autograd::variable_list in(4);
-      for (size_t i = 0; i < 4; ++i)
-        if (grads[i].defined()) in[i] = grads[i].detach().set_requires_grad(true);
-      at::AutoGradMode grad(true);
-      auto marked = (*once)(std::move(in));
-      for (size_t i = 0; i < 4; ++i)
-        if (grads[i].defined()) grads[i] = marked[i];
+      torch::autograd::variable_list marked = differentiable_once({grads[0], grads[1], grads[2], grads[3]}, "gated_ffn");
+      std::copy(marked.begin(), marked.end(), grads.begin());
     }
     return grads;
   }
@@ -468,17 +473,18 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 
 // bind(*addresses): of libcame8's entries, in the order of Entries
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[8];
-  if (!PyArg_ParseTuple(args, "KKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7])) return nullptr;
-  auto take = [&](auto& entry, int i) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(a[i]); };
-  take(entries.error, 0);
-  take(entries.adamw, 1);
-  take(entries.norm_size, 2);
-  take(entries.norm, 3);
-  take(entries.clip, 4);
-  take(entries.ffn_size, 5);
-  take(entries.ffn_forward, 6);
-  take(entries.ffn_backward, 7);
+  constexpr Py_ssize_t kEntries = sizeof(Entries) / sizeof(void*);
+  if (PyTuple_GET_SIZE(args) != kEntries) {
+    PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", kEntries);
+    return nullptr;
+  }
+  void* a[kEntries];
+  for (Py_ssize_t i = 0; i < kEntries; ++i) {
+    a[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(args, i));
+    if (a[i] == nullptr && PyErr_Occurred()) return nullptr;
+  }
+  static_assert(sizeof(a) == sizeof(entries), "pointers only");
+  std::memcpy(&entries, a, sizeof(a));
   Py_RETURN_NONE;
 }
 
@@ -531,6 +537,12 @@ PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "descriptors of a para
                          {"grad_norm", grad_norm, METH_VARARGS, "the norm of gradients, and the clip by it"},
                          {"bind", bind, METH_VARARGS, "libcame8's entries"},
                          {"gated_ffn", gated_ffn, METH_VARARGS, "the gated feed-forward block"},
+                         {"embedding", embedding, METH_VARARGS, "rows of a table by their tokens"},
+                         {"rms_norm", rms_norm, METH_VARARGS, "the root-mean-square norm"},
+                         {"rms_norm_int8", rms_norm_int8, METH_VARARGS, "the norm's result in 8 bits"},
+                         {"quantize_rows", quantize_rows, METH_VARARGS, "rows in 8 bits"},
+                         {"int8_linear", int8_linear, METH_VARARGS, "the product of 8-bit rows"},
+                         {"token_log_probs", token_log_probs, METH_VARARGS, "log probabilities of tokens"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "came8_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

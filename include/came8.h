@@ -397,6 +397,112 @@ int came8_gated_ffn_backward(const came8_ffn* f, const void* x, const void* w_ga
                              const void* dy, const float* g, const float* u, void* dx, void* dw_gate, void* dw_up,
                              void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * What a language model has around those blocks: the embedding of tokens, the root-mean-square norm with the residual's
+ * addition, rows in 8 bits with the product that reads them, and the log probabilities of tokens.  No counterpart in the
+ * reference.  As above: the caller owns every buffer, everything is enqueued on `stream`, nothing allocates, copies or
+ * synchronises, and a call may be captured in a HIP graph.  Every matrix's rows are contiguous; ld_*: elements from a row to
+ * the next.  Sums have a fixed order: the same inputs give the same bits.
+ * --------------------------------------------------------------------------------------------------------- */
+
+/* y[i] = scale * weight[token[i]]; tokens are int32_t (token_bytes 4) or int64_t (8).  A token outside [0, vocab) gives a row of
+ * zeros and has no gradient (a table whose rows are split over processes). */
+typedef struct came8_embedding {
+  int64_t tokens, vocab, dim; /* tokens below 2^31, vocab in [1, 2^31), dim in [1, 2^23] */
+  int64_t ld_weight;
+  int64_t padding;            /* the token whose row has no gradient, or -1 */
+  float scale;
+  int32_t dtype;              /* of weight, y and their gradients: CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t token_bytes;        /* 4 or 8 */
+  int32_t reserved;
+} came8_embedding;
+
+int came8_embedding_forward(const came8_embedding* e, const void* tokens, const void* weight, void* y, void* stream);
+
+/* Bytes of device workspace for came8_embedding_backward. */
+int came8_embedding_workspace_size(const came8_embedding* e, size_t* bytes);
+
+/* dweight[v] (contiguous, all of it) = scale * the sum of dy[i] (contiguous) over the i with token[i] = v, in float32, in an
+ * order that the tokens alone decide. */
+int came8_embedding_backward(const came8_embedding* e, const void* tokens, const void* dy, void* dweight, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* h = x + residual (rounded to its type; without a residual h = x), r = 1 / sqrt(mean(h^2) + eps), y = h r weight. */
+typedef struct came8_rms_norm {
+  int64_t rows, dim;          /* rows below 2^31, dim in [1, 2^30] */
+  int64_t ld_x, ld_residual;  /* ld_residual: 0 where there is none */
+  double eps;
+  int32_t dtype;              /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t reserved;
+} came8_rms_norm;
+
+/* y and h are contiguous; residual and h are both NULL or both not. */
+int came8_rms_norm_forward(const came8_rms_norm* n, const void* x, const void* residual, const void* weight, void* y, void* h,
+                           void* stream);
+
+/* Bytes of device workspace for came8_rms_norm_backward. */
+int came8_rms_norm_workspace_size(const came8_rms_norm* n, size_t* bytes);
+
+/* dx (of x and of the residual alike) and dweight (contiguous; either may be NULL) from h (rows ld_x apart: x, or what the
+ * forward call wrote), dy and dh (contiguous; dh may be NULL: zeros):
+ *   g = dy weight,  dx = r (g - h r^2 mean(g h)) + dh,  dweight = sum over the rows of dy h r */
+int came8_rms_norm_backward(const came8_rms_norm* n, const void* h, const void* weight, const void* dy, const void* dh, void* dx,
+                            void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The norm's y (not rounded to dtype before) in 8 bits: with p = h weight and a = max |p| of a row, q = p * 127 / a to nearest
+ * even, exactly, and scale = a r / 127.  Rows of q are ld_q bytes apart, a multiple of 16, and are zero from dim to the next
+ * multiple of 16; q is 16 bytes aligned.  A row with a below 2^-100 has codes and scale 0; one where a is infinite or NaN has
+ * codes 0 and a scale that is not finite, so that what is made of it is NaN. */
+int came8_rms_norm_int8(const came8_rms_norm* n, const void* x, const void* residual, const void* weight, int8_t* q, int64_t ld_q,
+                        float* scale, void* h, void* stream);
+
+/* The same of the rows of x as they are: p = x, r = 1 (eps and ld_residual of n are not used). */
+int came8_quantize_rows(const came8_rms_norm* n, const void* x, int8_t* q, int64_t ld_q, float* scale, void* stream);
+
+/* y[i][j] = (sum over k of q[i][k] w[j][k]) * scale[i] * w_scale[j] + bias[j]: the sum exact (in 32 bits), the rest in float32,
+ * rounded to dtype once.  bias has y's type, or is NULL. */
+typedef struct came8_int8_linear {
+  int64_t rows, in, out; /* rows and out at most 2^24, rows * out at most 2^36, in in [1, 131071] */
+  int64_t ld_q, ld_w;    /* bytes, at most 2^20 */
+  int32_t dtype;         /* of y: CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t reserved;
+} came8_int8_linear;
+
+/* Bytes of device workspace for came8_int8_linear_forward. */
+int came8_int8_linear_workspace_size(const came8_int8_linear* l, size_t* bytes);
+
+/* y is contiguous.  Operands whose rows do not start on words (an ld or an address that is not a multiple of 4) are copied to
+ * the workspace first. */
+int came8_int8_linear_forward(const came8_int8_linear* l, const int8_t* q, const float* scale, const int8_t* w,
+                              const float* w_scale, const void* bias, void* y, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Of each row z of logits, with m its largest and l = log(sum exp(z - m)): log_prob = z[token] - m - l (0 for a token outside
+ * [0, vocab): a row without one), entropy = -sum p log p, and the `top` largest with their tokens, the largest first, the
+ * lowest token first of equal ones (a NaN is the largest). */
+typedef struct came8_log_probs {
+  int64_t rows, vocab;  /* rows below 2^31, vocab in [1, 2^20] */
+  int64_t ld;           /* of logits */
+  int32_t dtype;        /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
+  int32_t token_bytes;  /* 4 or 8 */
+  int32_t top;          /* in [0, 64], at most vocab */
+  int32_t reserved;
+} came8_log_probs;
+
+/* Bytes of device workspace for came8_log_probs_forward. */
+int came8_log_probs_workspace_size(const came8_log_probs* p, size_t* bytes);
+
+/* stats[i][2]: m and l of row i, for the backward call.  top_log_prob and top_token [rows][top], NULL where top is 0. */
+int came8_log_probs_forward(const came8_log_probs* p, const void* logits, const void* tokens, float* log_prob, float* entropy,
+                            float* stats, float* top_log_prob, int64_t* top_token, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* dlogits (contiguous) from the gradients of log_prob and entropy (either may be NULL, not both):
+ *   dlogits[v] = dlog_prob ([v = token] - p[v]) - dentropy p[v] (log p[v] + entropy)
+ * A row whose two gradients are zero (dlog_prob counts as zero where there is no token) is zero. */
+int came8_log_probs_backward(const came8_log_probs* p, const void* logits, const void* tokens, const float* stats,
+                             const float* entropy, const float* dlog_prob, const float* dentropy, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
