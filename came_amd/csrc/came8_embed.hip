@@ -56,6 +56,9 @@ struct EmbedBackArgs {
   int32_t* count;    // of sorted positions
   int32_t* position; // [T], sorted by their tokens, and by themselves
   int32_t* token;    // [T], theirs
+  int32_t* cross;    // [shares]: of the token at a share's last position, if it begins there and goes on, the last share that has it;
+                     // else -1
+  uint64_t* empty;   // [ceil(V / range)][kSortWaves]: a workgroup's tokens that have no position
   float* part;       // [shares][2][D]
   int64_t T, V, D, padding;
   int32_t range;     // tokens a workgroup of the sort
@@ -65,17 +68,15 @@ struct EmbedBackArgs {
 };
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr int kSortUnroll = 4;     // tokens a lane has in flight
+constexpr int kSortUnroll = 8;     // tokens a lane has in flight; 8192 in all are read once
 constexpr int kMaxRange = 1000;    // tokens a workgroup: a thread each, and its counters fit 64 KiB
 
 // Every workgroup has `range` tokens and looks through all positions for them: twice, first to count (its own, by wavefront and
 // token, and those below its range, which tell where its part of the sorted list begins), then to place.  A wavefront takes a
-// run of successive positions and places them 64 at a time, so that the order is that of the positions.  No workgroup waits for
-// another.  The tokens stay in L2: 250 workgroups read 8192 of them in a few microseconds; and rows without a token are
-// cleared here.
-template <typename T>
+// run of successive positions and places them 64 at a time, so that the order is that of the positions; the lanes that have the
+// same token find each other by ballots on its bits (the first range has half of a text's tokens: one token at a time, its
+// workgroup took 34 us for 8192 positions, TODO so).  No workgroup waits for another.  The tokens stay in L2.
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const EmbedBackArgs a) {
-  using S = typename T::storage;
   extern __shared__ int32_t counts[];  // [kSortWaves][range], then kSortWaves + 1 words
   int32_t* extra = counts + kSortWaves * a.range;
   const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
@@ -91,15 +92,22 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const EmbedBackArgs
     const int64_t t = i < to ? token_at(a.tokens, i, a.wide) : -1;
     return t < a.V && t != a.padding ? t : -1;
   };
-  for (int64_t i = from; i < to; i += kWave * kSortUnroll) {
+  int32_t key[kSortUnroll];  // of the tokens in flight, less the first of the range; -1 for one of another range
+  auto fetch = [&](int64_t i, bool count) __attribute__((always_inline)) {
     int64_t t[kSortUnroll];
 #pragma unroll
     for (int u = 0; u < kSortUnroll; ++u) t[u] = look(i + u * kWave + lane);
 #pragma unroll
     for (int u = 0; u < kSortUnroll; ++u) {
-      if (t[u] >= first && t[u] < last) atomicAdd(&mine[t[u] - first], 1);
-      below += t[u] >= 0 && t[u] < first ? 1 : 0;
+      key[u] = t[u] >= first && t[u] < last ? int32_t(t[u] - first) : -1;
+      if (count) below += t[u] >= 0 && t[u] < first ? 1 : 0;
     }
+  };
+  for (int64_t i = from; i < to; i += kWave * kSortUnroll) {
+    fetch(i, true);
+#pragma unroll
+    for (int u = 0; u < kSortUnroll; ++u)
+      if (key[u] >= 0) atomicAdd(&mine[key[u]], 1);
   }
   below = wave_sum(below);
   if (lane == 0) extra[wave] = below;
@@ -131,50 +139,59 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const EmbedBackArgs
   }
   if (blockIdx.x + 1 == gridDim.x && r == kSortThreads - 1) gbl(a.count)[0] = start + all;
   __syncthreads();
+  const int bits = 32 - __builtin_clz(a.range);
   for (int64_t i = from; i < to; i += kWave * kSortUnroll) {
-    int64_t t[kSortUnroll];
-#pragma unroll
-    for (int u = 0; u < kSortUnroll; ++u) t[u] = look(i + u * kWave + lane);
+    if (run > kWave * kSortUnroll) fetch(i, false);  // else they are there
 #pragma unroll
     for (int u = 0; u < kSortUnroll; ++u) {
-      const bool here = t[u] >= first && t[u] < last;
-      const int32_t key = here ? int32_t(t[u] - first) : -1;
-      uint64_t left = __builtin_amdgcn_ballot_w64(here);
-      while (left != 0) {  // the lanes of one token at a time
-        const int leader = __builtin_ctzll(left);
-        const int32_t k = __builtin_amdgcn_readlane(key, leader);
-        const uint64_t same = __builtin_amdgcn_ballot_w64(key == k);
-        int32_t at = 0;
-        if (lane == leader) at = atomicAdd(&mine[k], __builtin_popcountll(same));
-        at = __builtin_amdgcn_readlane(at, leader);
-        if (key == k) {
-          const int32_t place = at + __builtin_popcountll(same & ((uint64_t(1) << lane) - 1));
-          gbl(a.position)[place] = int32_t(i + u * kWave + lane);
-          gbl(a.token)[place] = int32_t(t[u]);
-        }
-        left &= ~same;
+      const bool here = key[u] >= 0;
+      uint64_t same = __builtin_amdgcn_ballot_w64(here);  // the lanes with this one's token
+      if (same == 0) continue;
+      for (int b = 0; b < bits; ++b) {
+        const bool one = key[u] >> b & 1;
+        const uint64_t ones = __builtin_amdgcn_ballot_w64(one);
+        same &= one ? ones : ~ones;
+      }
+      const int before = __builtin_popcountll(same & ((uint64_t(1) << lane) - 1));
+      int32_t at = 0;
+      if (here && before == 0) at = atomicAdd(&mine[key[u]], __builtin_popcountll(same));
+      at = __shfl(at, __builtin_ctzll(same | uint64_t(1) << 63), kWave) + before;
+      if (here) {
+        gbl(a.position)[at] = int32_t(i + u * kWave + lane);
+        gbl(a.token)[at] = int32_t(first + key[u]);
       }
     }
   }
-  // rows without a token; `all` of thread r, from its wavefront's lanes
-  constexpr int V = kChunk<T>;
-  uint64_t empty = __builtin_amdgcn_ballot_w64(r < a.range && first + r < last && all == 0);
-  while (empty != 0) {
-    const int64_t v = first + wave * kWave + __builtin_ctzll(empty);
-    empty &= empty - 1;
-    S* row = static_cast<S*>(a.dw) + v * a.D;
-    for (int64_t e = int64_t(lane) * V; e < a.D; e += kWave * V) store_raw<T>(row, e, a.D, u32x4{0u, 0u, 0u, 0u});
-  }
+  const uint64_t empty = __builtin_amdgcn_ballot_w64(r < a.range && first + r < last && all == 0);
+  if (lane == 0) gbl(a.empty)[int64_t(blockIdx.x) * kSortWaves + wave] = empty;
+  // the shares that end within this token's positions
+  for (int64_t s = (start + a.share) / a.share - 1; all > 0 && (s + 1) * a.share <= start + all; ++s)
+    gbl(a.cross)[s] = start >= s * a.share && start + all > (s + 1) * a.share ? int32_t((start + all - 1) / a.share) : -1;
 }
 
 // The rows of dy of `share` successive sorted positions, TPR threads by their 16-byte chunks, summed by token.  A token whose
 // positions end here and began here is written; of one that goes on or began before, the sum goes to part[share][0] (began
-// before) or part[share][1] (begins here and goes on).
-constexpr int kAhead = 4;  // rows in flight
+// before) or part[share][1] (begins here and goes on).  Workgroups past the shares' clear the rows without a token meanwhile.
+constexpr int kAhead = 8;      // rows in flight
+constexpr int kClear = 16;     // tokens a workgroup that clears, of one word of `empty`
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_embed_sum(const EmbedBackArgs a) {
+__global__ __launch_bounds__(kThreads) void k_embed_sum(const EmbedBackArgs a, const int shares) {
   using S = typename T::storage;
   constexpr int V = kChunk<T>;
+  if (int(blockIdx.x) >= shares) {
+    if (blockIdx.y > 0) return;
+    const int64_t id = int64_t(blockIdx.x) - shares, words = (a.range + kWave - 1) / kWave, word = id / (kWave / kClear);
+    const int bit = int(id % (kWave / kClear)) * kClear;
+    const int64_t group = word / words, of = word - group * words;
+    const int64_t v0 = group * a.range + of * kWave + bit;
+    uint64_t empty = gbl(a.empty)[group * kSortWaves + of] >> bit & ((uint64_t(1) << kClear) - 1);
+    while (empty != 0) {
+      S* row = static_cast<S*>(a.dw) + (v0 + __builtin_ctzll(empty)) * a.D;
+      empty &= empty - 1;
+      for (int64_t e = int64_t(threadIdx.x) * V; e < a.D; e += kThreads * V) store_raw<T>(row, e, a.D, u32x4{0u, 0u, 0u, 0u});
+    }
+    return;
+  }
   const int32_t n = gbl(a.count)[0];
   const int64_t begin = int64_t(blockIdx.x) * a.share, end = min(begin + a.share, int64_t(n));
   if (begin >= end) return;
@@ -225,34 +242,25 @@ __global__ __launch_bounds__(kThreads) void k_embed_sum(const EmbedBackArgs a) {
   }
 }
 
-// The tokens that begin in a share and go on: their sums from there on, 256 columns a workgroup, a sixteenth of the shares a
+// The tokens that begin in a share and go on: their sums from there on, 256 columns a workgroup, a quarter of the shares a
 // wavefront.
 template <typename T>
-__global__ __launch_bounds__(1024) void k_embed_join(const EmbedBackArgs a) {
-  __shared__ float lds[16][kWave * 4];
-  const int32_t n = gbl(a.count)[0];
-  const int64_t end = (int64_t(blockIdx.x) + 1) * a.share;
-  if (end >= n) return;
-  const CAME8_GLOBAL int32_t* tokens = gbl(a.token);
-  const int32_t token = tokens[end - 1];
-  if (tokens[end] != token) return;
-  if (blockIdx.x > 0 && tokens[end - a.share] == token && tokens[end - a.share - 1] == token) return;  // began before
-  // the last share that has it: its first position is the token's
-  int64_t lo = blockIdx.x + 1, hi = (n - 1) / a.share;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) / 2;
-    if (tokens[mid * a.share] == token) lo = mid;
-    else hi = mid - 1;
-  }
+__global__ __launch_bounds__(kThreads) void k_embed_join(const EmbedBackArgs a) {
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ float lds[kWaves][kWave * 4];
+  const int64_t first = blockIdx.x, end = (first + 1) * a.share;
+  if (end >= gbl(a.count)[0]) return;
+  const int32_t last = gbl(a.cross)[first];
+  if (last < 0) return;
   const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
   const int64_t c = int64_t(blockIdx.y) * (kWave * 4) + lane * 4;
-  const int64_t shares = lo - blockIdx.x + 1, each = (shares + 15) / 16;
+  const int64_t shares = last - first + 1, each = (shares + kWaves - 1) / kWaves;
   const int64_t from = min(each * wave, shares), to = min(from + each, shares);
   float sum[4] = {};
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t k = from; k < to; ++k) {
     float x[4];
-    load_chunk<F32>(a.part + ((int64_t(blockIdx.x) + k) * 2 + (k == 0 ? 1 : 0)) * a.D, c, a.D, x);
+    load_chunk<F32>(a.part + ((first + k) * 2 + (k == 0 ? 1 : 0)) * a.D, c, a.D, x);
 #pragma unroll
     for (int v = 0; v < 4; ++v) sum[v] += x[v];
   }
@@ -260,11 +268,11 @@ __global__ __launch_bounds__(1024) void k_embed_join(const EmbedBackArgs a) {
   for (int v = 0; v < 4; ++v) lds[wave][lane * 4 + v] = sum[v];
   __syncthreads();
   const int64_t col = int64_t(blockIdx.y) * (kWave * 4) + int(threadIdx.x);
-  if (threadIdx.x < kWave * 4 && col < a.D) {
+  if (col < a.D) {
     float s = lds[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < 16; ++w) s += lds[w][threadIdx.x];
-    gbl(static_cast<typename T::storage*>(a.dw))[int64_t(token) * a.D + col] = T::store(s * a.scale);
+    for (int w = 1; w < kWaves; ++w) s += lds[w][threadIdx.x];
+    gbl(static_cast<typename T::storage*>(a.dw))[int64_t(gbl(a.token)[end]) * a.D + col] = T::store(s * a.scale);
   }
 }
 
@@ -293,25 +301,28 @@ int64_t shares_of(const came8_embedding* e) { return ceil_div(e->tokens, share_o
 int64_t range_of(const came8_embedding* e) { return std::min<int64_t>(kMaxRange, std::max<int64_t>(16, ceil_div(e->vocab, 256))); }
 
 struct Layout {
-  size_t count = 0, position = 0, token = 0, part = 0, bytes = 0;
+  size_t count = 0, position = 0, token = 0, cross = 0, empty = 0, part = 0, bytes = 0;
 };
 Layout layout_of(const came8_embedding* e) {
   Layout l;
   l.position = 256;
   l.token = l.position + size_t(up(e->tokens * 4, 256));
-  l.part = l.token + size_t(up(e->tokens * 4, 256));
+  l.cross = l.token + size_t(up(e->tokens * 4, 256));
+  l.empty = l.cross + size_t(up(shares_of(e) * 4, 256));
+  l.part = l.empty + size_t(up(ceil_div(e->vocab, range_of(e)) * kSortWaves * 8, 256));
   l.bytes = l.part + size_t(shares_of(e) * 2 * e->dim * 4);
   return l;
 }
 
 template <typename T>
 void backward(const came8_embedding* e, const EmbedBackArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(k_embed_sort<T>, dim3(unsigned(ceil_div(e->vocab, a.range))), dim3(kSortThreads),
-                     unsigned((kSortWaves * a.range + kSortWaves + 1) * 4), stream, a);
-  const unsigned shares = unsigned(shares_of(e));
-  hipLaunchKernelGGL(k_embed_sum<T>, dim3(shares, unsigned(ceil_div(e->dim, kThreads * kChunk<T>))), dim3(kThreads), 0, stream, a);
+  const int64_t groups = ceil_div(e->vocab, a.range), clear = groups * ceil_div(a.range, kWave) * (kWave / kClear);
+  hipLaunchKernelGGL(k_embed_sort, dim3(unsigned(groups)), dim3(kSortThreads), unsigned((kSortWaves * a.range + kSortWaves + 1) * 4), stream, a);
+  const int shares = int(shares_of(e));
+  hipLaunchKernelGGL(k_embed_sum<T>, dim3(unsigned(shares + clear), unsigned(ceil_div(e->dim, kThreads * kChunk<T>))), dim3(kThreads), 0,
+                     stream, a, shares);
   if (shares > 1)
-    hipLaunchKernelGGL(k_embed_join<T>, dim3(shares - 1, unsigned(ceil_div(e->dim, kWave * 4))), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL(k_embed_join<T>, dim3(unsigned(shares - 1), unsigned(ceil_div(e->dim, kWave * 4))), dim3(kThreads), 0, stream, a);
 }
 
 int check(const char* what, const came8_embedding* e) {
@@ -391,7 +402,8 @@ int came8_embedding_backward(const came8_embedding* e, const void* tokens, const
       return op_fail(CAME8_ESPACE, std::string(what) + ": workspace too small or misaligned");
     char* ws = static_cast<char*>(workspace);
     const EmbedBackArgs a{tokens, dy, dweight, reinterpret_cast<int32_t*>(ws), reinterpret_cast<int32_t*>(ws + l.position),
-                          reinterpret_cast<int32_t*>(ws + l.token), reinterpret_cast<float*>(ws + l.part), e->tokens, e->vocab, e->dim,
+                          reinterpret_cast<int32_t*>(ws + l.token), reinterpret_cast<int32_t*>(ws + l.cross),
+                          reinterpret_cast<uint64_t*>(ws + l.empty), reinterpret_cast<float*>(ws + l.part), e->tokens, e->vocab, e->dim,
                           e->padding, int32_t(range_of(e)), int32_t(share_of(e)), e->scale, e->token_bytes == 8};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (e->dtype == CAME8_F32) backward<F32>(e, a, s);

@@ -51,43 +51,102 @@ __device__ __forceinline__ void store_scaled(const Int8Args& a, int64_t m, int n
 }
 
 // -------------------------------------------------------------------------------------------------- few rows
-// 16 rows of weights a workgroup, an eighth of k a wavefront: fragments go from memory to the matrix instructions, kDeep steps of
-// 64 codes at a time, and the wavefronts' sums are joined in LDS.
-template <typename T, int FM>
-__global__ __launch_bounds__(512) void k_int8_few(const Int8Args a) {
-  constexpr int kWaves = 8, kDeep = FM == 1 ? 8 : 4;
-  __shared__ i32x4 lds[kWaves][FM * 64];
-  const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave, r = lane % 16, g = lane / 16;
-  const int n0 = int(blockIdx.x) * 16;
-  const int8_t* w = a.w + int64_t(min(n0 + r, a.N - 1)) * a.ld_w;
+// 16 codes from e0 on of a row of K, at least 16, zeros past its end: the row's last 16, shifted, where K cuts them
+__device__ __forceinline__ u32x4 load_cut(const int8_t* row, int e0, int K) {
+  const int left = K - e0, over = left <= 0 ? 16 : left < 16 ? 16 - left : 0;
+  u32x4 v = *(const CAME8_GLOBAL u32x4b*)gbl(row + (left < 16 ? K - 16 : e0));
+  const int words = over / 4;
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t far = e + 3 < 4 ? v[3] : 0u, two = e + 2 < 4 ? v[e + 2 < 4 ? e + 2 : 3] : 0u, one = e + 1 < 4 ? v[e + 1 < 4 ? e + 1 : 3] : 0u;
+    w[e] = words == 0 ? v[e] : words == 1 ? one : words == 2 ? two : words == 3 ? far : 0u;
+  }
+  u32x4 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = __builtin_amdgcn_alignbyte(e < 3 ? w[e < 3 ? e + 1 : 3] : 0u, w[e], over & 3);
+  return out;
+}
+
+// 16 rows of weights at a time for a workgroup, an eighth of k a wavefront: fragments go from memory to the matrix instructions,
+// and the wavefronts' sums are joined in LDS.  FM: 16 rows of q each.
+//
+// DEEP steps of 64 codes are loaded together.  AHEAD: the weights' next ones meanwhile, those of the workgroup's next 16 rows
+// too, so that memory is never waited for by all; two workgroups on a CU.  Without, a workgroup has 16 rows alone, and its
+// loads are as deep as registers go: where there are no more than 256 of them, what counts is how often a wavefront waits.
+template <typename T, int FM, int DEEP, bool AHEAD>
+__global__ __launch_bounds__(512, AHEAD ? 4 : 2) void k_int8_few(const Int8Args a) {
+  constexpr int kWaves = 8;
+  __shared__ i32x4 lds[AHEAD ? 2 : 1][kWaves][FM * 64];
+  const int lane = int(threadIdx.x) % kWave, r = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);  // k's bounds are scalar so
+  const int steps = a.K / 64, first = steps * wave / kWaves, last = steps * (wave + 1) / kWaves;  // what is left: the last wavefront's
+  const int blocks = (a.N + 15) / 16;
   const int8_t* x[FM];
 #pragma unroll
-  for (int f = 0; f < FM; ++f) x[f] = a.q + int64_t(min(f * 16 + r, a.M - 1)) * a.ld_q;
-  const int steps = (a.K + 63) / 64, last = steps * (wave + 1) / kWaves;
-  i32x4 acc[FM] = {};
-  for (int s = steps * wave / kWaves; s < last; s += kDeep) {
-    u32x4 wf[kDeep], xf[kDeep][FM];
+  for (int f = 0; f < FM; ++f) x[f] = a.q + int64_t(min(f * 16 + r, a.M - 1)) * a.ld_q;  // rows past M are not stored
+  auto row = [&](int b) { return a.w + int64_t(min(b * 16 + r, a.N - 1)) * a.ld_w; };
+  u32x4 wf[AHEAD ? 2 : 1][DEEP], xf[DEEP][FM];
+  // steps from s on of block b's weights; none past the last of either
+  auto fetch_w = [&](u32x4(&to)[DEEP], int b, int s) __attribute__((always_inline)) {
+    const CAME8_GLOBAL int8_t* w = gbl(row(b)) + g * 16;
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) wf[d] = load_raw<I8>(w, (s + d) * 64 + g * 16, s + d < last ? a.K : 0);
+    for (int d = 0; d < DEEP; ++d) {
+      to[d] = u32x4{0u, 0u, 0u, 0u};
+      if (s + d < last && b < blocks) {
+        if constexpr (AHEAD) to[d] = ld_nt16((const CAME8_GLOBAL u32x4b*)(w + (s + d) * 64));
+        else to[d] = *(const CAME8_GLOBAL u32x4b*)(w + (s + d) * 64);
+      }
+    }
+  };
+  auto fetch_x = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d)
+    for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-      for (int f = 0; f < FM; ++f) xf[d][f] = load_raw<I8>(x[f], (s + d) * 64 + g * 16, s + d < last && f * 16 + r < a.M ? a.K : 0);
+      for (int f = 0; f < FM; ++f) {
+        xf[d][f] = u32x4{0u, 0u, 0u, 0u};
+        if (s + d < last) xf[d][f] = *(const CAME8_GLOBAL u32x4b*)(gbl(x[f]) + g * 16 + (s + d) * 64);
+      }
+  };
+  const bool once = FM == 1 && last - first <= DEEP;  // q's fragments stay in registers
+  int turn = 0;
+  fetch_w(wf[0], blockIdx.x, first);
+  if (once) fetch_x(first);
+  for (int b = blockIdx.x; b < blocks; b += AHEAD ? int(gridDim.x) : blocks, turn ^= 1) {
+    i32x4 acc[FM] = {};
+    for (int s = first;; s += DEEP) {
+      const bool more = s + DEEP < last;
+      if (!once) fetch_x(s);
+      if constexpr (AHEAD) fetch_w(wf[1], more ? b : b + int(gridDim.x), more ? s + DEEP : first);
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d)
+      for (int d = 0; d < DEEP; ++d)
 #pragma unroll
-      for (int f = 0; f < FM; ++f) acc[f] = mfma_i8(wf[d], xf[d][f], acc[f]);
-  }
-  // a lane holds columns 4 g to 4 g + 3 of row r
+        for (int f = 0; f < FM; ++f) acc[f] = mfma_i8(wf[0][d], xf[d][f], acc[f]);
+      if constexpr (AHEAD) {
 #pragma unroll
-  for (int f = 0; f < FM; ++f) lds[wave][f * 64 + r * 4 + g] = acc[f];
-  __syncthreads();
-  for (int o = int(threadIdx.x); o < FM * 64; o += 512) {
-    i32x4 c = lds[0][o];
+        for (int d = 0; d < DEEP; ++d) wf[0][d] = wf[1][d];
+      } else if (more) {
+        fetch_w(wf[0], b, s + DEEP);
+      }
+      if (!more) break;
+    }
+    if (wave == kWaves - 1 && a.K % 64 != 0) {
+      const u32x4 w = load_cut(row(b), steps * 64 + g * 16, a.K);
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) c += lds[k][o];
-    const int m = o / 4, n = n0 + o % 4 * 4;
-    if (m < a.M && n < a.N) store_scaled<T>(a, m, n, c);
+      for (int f = 0; f < FM; ++f) acc[f] = mfma_i8(w, load_cut(x[f], steps * 64 + g * 16, a.K), acc[f]);
+    }
+    // a lane holds columns 4 g to 4 g + 3 of row r
+    i32x4(&part)[kWaves][FM * 64] = lds[AHEAD ? turn : 0];
+#pragma unroll
+    for (int f = 0; f < FM; ++f) part[wave][f * 64 + r * 4 + g] = acc[f];
+    __syncthreads();  // what is read below is written again after the next block's
+    for (int o = int(threadIdx.x); o < FM * 64; o += 512) {
+      i32x4 c = part[0][o];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) c += part[k][o];
+      const int m = o / 4, n = b * 16 + o % 4 * 4;
+      if (m < a.M && n < a.N) store_scaled<T>(a, m, n, c);
+    }
   }
 }
 
@@ -269,7 +328,9 @@ __global__ __launch_bounds__(kThreads) void k_int8_pack(const int8_t* p, int64_t
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up(int64_t n, int64_t a) { return ceil_div(n, a) * a; }
 
-constexpr int64_t kFew = 64;
+// few rows read the weights once; rows that do not hold 16 codes go through tiles, which copy them
+bool is_few(const came8_int8_linear* l) { return l->rows <= 64 && l->in >= 16; }
+constexpr int64_t kAtOnce = 512;                  // workgroups of 512 threads that the GPU holds at once, two on a CU
 constexpr int64_t kMaxStride = int64_t(1) << 20;  // bytes: a tile's 256 rows stay below 2^31
 constexpr int64_t kMaxIn = 131071;                // 2^31 - 1 holds that many products of -128 by -128
 
@@ -315,7 +376,7 @@ struct Layout {
 // Whether the rows are copied goes by the strides here, by the addresses too where the call is made: room for both copies
 Layout layout_of(const came8_int8_linear* l) {
   Layout o;
-  if (l->rows <= kFew) return o;
+  if (is_few(l)) return o;
   const int64_t ld = up(l->in, 16);
   o.w = size_t(up(l->rows * ld, 256));
   o.part = o.w + size_t(up(l->out * ld, 256));
@@ -327,11 +388,15 @@ Layout layout_of(const came8_int8_linear* l) {
 
 template <typename T>
 void forward(const came8_int8_linear* l, Int8Args a, char* ws, hipStream_t stream) {
-  if (l->rows <= kFew) {
-    const dim3 grid(unsigned(ceil_div(l->out, 16)));
-    if (l->rows <= 16) hipLaunchKernelGGL((k_int8_few<T, 1>), grid, dim3(512), 0, stream, a);
-    else if (l->rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2>), grid, dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((k_int8_few<T, 4>), grid, dim3(512), 0, stream, a);
+  if (is_few(l)) {
+    const int64_t blocks = ceil_div(l->out, 16);
+    const dim3 each{unsigned(blocks)}, ahead{unsigned(std::min(blocks, kAtOnce))};
+    if (l->rows <= 16) hipLaunchKernelGGL((k_int8_few<T, 1, 8, true>), ahead, dim3(512), 0, stream, a);
+    else if (blocks <= kAtOnce / 2 && l->rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2, 12, false>), each, dim3(512), 0, stream, a);
+    else if (blocks <= kAtOnce / 2 && l->rows <= 48) hipLaunchKernelGGL((k_int8_few<T, 3, 11, false>), each, dim3(512), 0, stream, a);
+    else if (blocks <= kAtOnce / 2) hipLaunchKernelGGL((k_int8_few<T, 4, 8, false>), each, dim3(512), 0, stream, a);
+    else if (l->rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2, 4, true>), ahead, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((k_int8_few<T, 4, 3, true>), ahead, dim3(512), 0, stream, a);
     return;
   }
   const Layout o = layout_of(l);
@@ -411,7 +476,7 @@ int came8_int8_linear_forward(const came8_int8_linear* l, const int8_t* q, const
         (rc = check_pointer(what, y, size)) != CAME8_OK || (bias != nullptr && (rc = check_pointer(what, bias, size)) != CAME8_OK))
       return rc;
     const Layout o = layout_of(l);
-    if (l->rows > kFew && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < o.bytes))
+    if (!is_few(l) && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < o.bytes))
       return op_fail(CAME8_ESPACE, std::string(what) + ": workspace too small or misaligned");
     const Int8Args a{q, scale, w, w_scale, bias, y, nullptr, l->ld_q, l->ld_w, int32_t(l->rows), int32_t(l->out), int32_t(l->in), 0, 0, 1};
     hipStream_t s = static_cast<hipStream_t>(stream);

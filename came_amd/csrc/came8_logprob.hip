@@ -36,9 +36,9 @@ struct LogProbArgs {
 };
 
 // A logit and its token as one number: ordered as the values are, of equal ones the lower token the larger; NaN is the largest.
-// 0 is no logit.
+// 0 and the largest number are no logits.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
-  const uint32_t b = __float_as_uint(x != x ? __uint_as_float(0x7fffffffu) : x + 0.0f);  // -0 is 0
+  const uint32_t b = __float_as_uint(x != x ? __uint_as_float(0x7ffffffeu) : x + 0.0f);  // -0 is 0
   return uint64_t(b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u)) << 32 | uint32_t(~token);
 }
 __device__ __forceinline__ float value_of(uint64_t key) {
@@ -47,61 +47,61 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 __device__ __forceinline__ int64_t token_of(uint64_t key) { return int64_t(~uint32_t(key)); }
 
-// The `top` largest keys of a workgroup's elements in order, to out(rank, key); key 0 where there are fewer.  f(g) calls g with
-// every key of the thread.
+// The `top` largest keys of a workgroup's elements in order, to out(rank, key); key 0 where there are fewer.  best: the thread's
+// largest, of numbers.  larger(bound, g) calls g with every key of the thread that is not below the bound (numbers alone), every(g)
+// with all of them.
 //
-// The threads' largest keys, by groups of four threads (a thread each in a workgroup of one wavefront), bound the top-th key from
-// below: the top-th largest of them.  Few keys are not below it (22 of 32000 for the top 20); they go to a list, and each one's
-// place is the number of larger ones.  Where the list is too short (sorted logits, say), the largest below the last is
-// looked for `top` times.
-constexpr int kList = 1024;
-template <int TPB>
+// The largest keys of 64 groups of threads bound the top-th key from below: the top-th largest of them.  Few keys are not below
+// it (24 of 32000 for the top 20); they go to a list, and each one's place is the number of larger ones.  Where the list is too
+// short (sorted logits, say), or a NaN is among the elements, the largest below the last is looked for `top` times.
+constexpr int kList = 1024, kGroups = 64;
 struct TopShared {
-  static constexpr int kGroup = TPB == kWave ? 1 : 4, kGroups = TPB / kGroup;
   uint64_t group[kGroups];
   uint64_t list[kList];
   uint64_t bound;
   int32_t count;
 };
-template <int TPB, typename F, typename O>
-__device__ __forceinline__ void top_keys(F&& f, int top, TopShared<TPB>& s, O&& out) {
-  using Sh = TopShared<TPB>;
+template <int CTRL>
+__device__ __forceinline__ uint64_t max_dpp(uint64_t v) {
+  return max(v, uint64_t(dpp_u32<CTRL>(uint32_t(v >> 32))) << 32 | dpp_u32<CTRL>(uint32_t(v)));
+}
+template <int TPB, typename F, typename G, typename O>
+__device__ __forceinline__ void top_keys(uint64_t best, bool numbers, F&& larger, G&& every, int top, TopShared& s, O&& out) {
+  constexpr int kGroup = TPB / kGroups;
+  static_assert(kGroup == 1 || kGroup == 8, "");
   const int t = int(threadIdx.x);
-  uint64_t best = 0;
-  f([&](uint64_t k) { best = max(best, k); });
-  uint64_t of = best;
-#pragma unroll
-  for (int o = 1; o < Sh::kGroup; o *= 2) of = max_xor(of, o);
-  if (t % Sh::kGroup == 0) s.group[t / Sh::kGroup] = of;
+  if constexpr (kGroup == 8) best = max_dpp<kDppHalfMirror>(max_dpp<kDppXor2>(max_dpp<kDppXor1>(best)));
+  if (t % kGroup == 0) s.group[t / kGroup] = best;
   if (t == 0) {
-    s.bound = 0;
-    s.count = 0;
+    s.bound = 1;
+    s.count = numbers ? 0 : kList + 1;
   }
   __syncthreads();
-  if (t < Sh::kGroups) {
+  if (t < kGroups) {
     const uint64_t k = s.group[t];
-    int larger = 0;
-#pragma unroll 8
-    for (int g = 0; g < Sh::kGroups; ++g) larger += s.group[g] > k ? 1 : 0;
-    if (larger == top - 1 && k != 0) s.bound = k;  // keys other than 0 are different
+    int above = 0;
+#pragma unroll 16
+    for (int g = 0; g < kGroups; ++g) above += s.group[g] > k ? 1 : 0;
+    if (above == top - 1 && k != 0) s.bound = k;  // keys other than 0 are different
   }
   __syncthreads();
-  const uint64_t bound = max(s.bound, uint64_t(1));
-  if (best >= bound)
-    f([&](uint64_t k) {
-      if (k >= bound) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < kList) s.list[at] = k;
-      }
+  const uint64_t bound = s.bound;
+  if (best >= bound && numbers)
+    larger(bound, [&](uint64_t k) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kList) s.list[at] = k;
     });
   __syncthreads();
   const int n = s.count;
   if (n <= kList) {
     for (int i = t; i < n; i += TPB) {
       const uint64_t k = s.list[i];
-      int larger = 0;
-      for (int j = 0; j < n; ++j) larger += s.list[j] > k ? 1 : 0;
-      if (larger < top) out(larger, k);
+      int above = 0;
+      for (int j = 0; j < n; j += 8) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) above += s.list[j + u] > k && j + u < n ? 1 : 0;
+      }
+      if (above < top) out(above, k);
     }
     for (int r = n + t; r < top; r += TPB) out(r, uint64_t(0));
     return;
@@ -110,7 +110,7 @@ __device__ __forceinline__ void top_keys(F&& f, int top, TopShared<TPB>& s, O&& 
 #pragma unroll 1
   for (int r = 0; r < top; ++r) {
     uint64_t k = 0;
-    f([&](uint64_t v) { k = v < last ? max(k, v) : k; });
+    every([&](uint64_t v) { k = v < last ? max(k, v) : k; });
 #pragma unroll
     for (int o = 1; o < kWave; o *= 2) k = max_xor(k, o);
     __syncthreads();  // the last round's are read
@@ -126,24 +126,55 @@ __device__ __forceinline__ void top_keys(F&& f, int top, TopShared<TPB>& s, O&& 
 template <typename T>
 constexpr uint32_t kNone = std::is_same<T, F32>::value ? 0xff800000u : std::is_same<T, BF16>::value ? 0xff80ff80u : 0xfc00fc00u;
 
+// The largest of a thread's elements; fp16: two at a time.  (Where one is a NaN it may be that.)
+template <typename T>
+struct Maximum {
+  float m = -__builtin_inff();
+  __device__ __forceinline__ void add(const u32x4& w) {
+    float x[kChunk<T>];
+    unpack<T>(w, x);
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e) m = fmaxf(m, x[e]);
+  }
+  __device__ __forceinline__ float value() const { return m; }
+};
+template <>
+struct Maximum<F16> {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  f16x2 m = {_Float16(-__builtin_inff()), _Float16(-__builtin_inff())};
+  __device__ __forceinline__ void add(const u32x4& w) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(f16x2, uint32_t(w[e])));
+  }
+  __device__ __forceinline__ float value() const { return fmaxf(float(m.x), float(m.y)); }
+};
+
 // A part of a row a workgroup of TPB threads, NV chunks a thread.
+//
+// Rows that have logits of -inf are gone over again with their terms of t bounded, which would cost all rows an instruction a
+// logit.  8192 rows of 32000 in bf16: TODO us.
 template <typename T, int TPB, int NV, bool TOP>
-__global__ __launch_bounds__(TPB) void k_logprob(const LogProbArgs a) {
+__global__ __launch_bounds__(TPB, 6) void k_logprob(const LogProbArgs a) {
   using S = typename T::storage;
-  constexpr int V = kChunk<T>;
-  __shared__ float lds[2][3 * (TPB / kWave)];
-  __shared__ typename std::conditional<TOP, TopShared<TPB>, char>::type shared;
+  constexpr int V = kChunk<T>, kStep = TPB * V;
+  constexpr int kWaves = TPB / kWave;
+  __shared__ float lds[2][5 * kWaves];
+  __shared__ typename std::conditional<TOP, TopShared, char>::type shared;
   const int t = int(threadIdx.x);
-  const int64_t all = a.rows * a.parts;
+  const int part = int(blockIdx.y), first = part * a.length, n = int(min(int64_t(a.length), a.V - first));
   int turn = 0;
-  for (int64_t id = blockIdx.x; id < all; id += gridDim.x, turn ^= 1) {
-    const int64_t row = id / a.parts;
-    const int part = int(id - row * a.parts);
+  // From the last row on, which may still be in the memory-side cache, and the backward pass from the first on, with loads and
+  // stores that leave what this pass has read there: 8192 rows of 32000 in bf16 271 us in all; 306 without those hints, 316 with
+  // the rows in one order.
+  for (int64_t row = a.rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x, turn ^= 1) {
     const S* z = static_cast<const S*>(a.z) + row * a.ld;
-    const int first = part * a.length, n = int(min(int64_t(a.length), a.V - first));
     u32x4 raw[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = load_raw<T>(z + first, (i * TPB + t) * V, n, kNone<T>);
+    for (int i = 0; i < NV; ++i) {
+      const S* at = z + first + i * kStep;
+      if ((i + 1) * kStep <= n) raw[i] = *(const CAME8_GLOBAL u32x4b*)(gbl(at) + t * V);  // all threads'
+      else raw[i] = load_raw<T>(at, t * V, n - i * kStep, kNone<T>);
+    }
     int64_t token = -1;
     float given = 0.0f;
     if (a.parts == 1 && t == 0) {
@@ -151,25 +182,37 @@ __global__ __launch_bounds__(TPB) void k_logprob(const LogProbArgs a) {
       if (token >= 0 && token < a.V) given = T::load(gbl(z)[token]);
       else token = -1;
     }
-    float m = -__builtin_inff();
+    float own = -__builtin_inff();
+    int which = 0;  // TOP: its first place among the thread's elements
+    if constexpr (TOP) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float x[V];
-      unpack<T>(raw[i], x);
+      for (int i = 0; i < NV; ++i) {
+        float x[V];
+        unpack<T>(raw[i], x);
 #pragma unroll
-      for (int e = 0; e < V; ++e) m = fmaxf(m, x[e]);
+        for (int e = 0; e < V; ++e) {
+          which = x[e] > own ? i * V + e : which;
+          own = x[e] > own ? x[e] : own;
+        }
+      }
+    } else {
+      Maximum<T> largest;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) largest.add(raw[i]);
+      own = largest.value();
     }
+    float m = own;
 #pragma unroll
     for (int o = 1; o < kWave; o *= 2) m = fmaxf(m, __shfl_xor(m, o, kWave));
-    if constexpr (TPB > kWave) {
-      float* most = lds[turn] + 2 * (TPB / kWave);
+    if constexpr (kWaves > 1) {
+      float* most = lds[turn] + 4 * kWaves;
       if (t % kWave == 0) most[t / kWave] = m;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < TPB / kWave; ++w) m = fmaxf(m, most[w]);
+      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, most[w]);
     }
     const float base = m == -__builtin_inff() ? 0.0f : m;  // a part of -inf alone: s = 0
-    float s[2] = {0.0f, 0.0f};
+    float s[2] = {0.0f, 0.0f};  // sums of e^(z - m) and of e^(z - m) (z - m)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float x[V];
@@ -179,11 +222,28 @@ __global__ __launch_bounds__(TPB) void k_logprob(const LogProbArgs a) {
       for (int e = 0; e < V; ++e) {
         const float d = x[e] - base, p = __builtin_amdgcn_exp2f(d * kLog2e);
         s[0] += p;
-        s[1] = fmaf(p, fmaxf(d, kFar), s[1]);
+        s[1] = fmaf(p, (i + 1) * kStep <= n ? d : fmaxf(d, kFar), s[1]);  // past the row's end d is -inf
       }
       __builtin_amdgcn_sched_barrier(0);  // a chunk at a time: with all 64 values on their way registers are out
     }
     row_sum<TPB>(s, lds[turn]);
+    if (s[1] != s[1]) {  // logits of -inf, whose term is no number
+      s[0] = s[1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float x[V];
+        unpack_again(raw[i]);
+        unpack<T>(raw[i], x);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = x[e] - base, p = __builtin_amdgcn_exp2f(d * kLog2e);
+          s[0] += p;
+          s[1] = fmaf(p, fmaxf(d, kFar), s[1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      row_sum<TPB>(s, lds[turn] + 2 * kWaves);
+    }
     const float l = logf(s[0]);
     if (t == 0) {
       if (a.parts == 1) {
@@ -192,33 +252,61 @@ __global__ __launch_bounds__(TPB) void k_logprob(const LogProbArgs a) {
         gbl(a.stats)[2 * row] = m;
         gbl(a.stats)[2 * row + 1] = l;
       } else {
-        CAME8_GLOBAL float* p = gbl(a.part) + id * 4;
+        CAME8_GLOBAL float* p = gbl(a.part) + (row * a.parts + part) * 4;
         p[0] = m;
         p[1] = s[0];
         p[2] = s[1];
       }
     }
     if constexpr (TOP) {
-      auto each = [&](auto&& g) {
+      // chunk i's values and first token, hidden from the compiler: it would keep all of them in registers
+      auto values = [&](int i, float(&x)[V]) {
+        unpack_again(raw[i]);
+        unpack<T>(raw[i], x);
+        int at = i * kStep + t * V;
+        asm volatile("" : "+v"(at));
+        return at;
+      };
+      const int place = which / V * kStep + t * V + which % V;
+      const uint64_t best = place < n ? key_of(own, uint32_t(first + place)) : 0;
+      auto larger = [&](uint64_t bound, auto&& g) {
+        const float least = value_of(bound);  // a bound of 1 is NaN: then nothing is below it
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           float x[V];
-          unpack_again(raw[i]);
-          unpack<T>(raw[i], x);
-          int at = (i * TPB + t) * V;
-          asm volatile("" : "+v"(at));  // likewise: no 64 indices kept
+          const int at = values(i, x);
+          bool any = false;
+#pragma unroll
+          for (int e = 0; e < V; ++e) any |= !(x[e] < least);
+          if (any) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (!(x[e] < least) && at + e < n) {
+                const uint64_t k = key_of(x[e], uint32_t(first + at + e));
+                if (k >= bound) g(k);
+              }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      auto every = [&](auto&& g) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          float x[V];
+          const int at = values(i, x);
 #pragma unroll
           for (int e = 0; e < V; ++e)
             if (at + e < n) g(key_of(x[e], uint32_t(first + at + e)));
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      top_keys<TPB>(each, a.top, shared, [&](int r, uint64_t k) {
+      // s is NaN where an element is, and where one is infinite
+      top_keys<TPB>(best, s[0] == s[0], larger, every, a.top, shared, [&](int r, uint64_t k) {
         if (a.parts == 1) {
           gbl(a.top_log_prob)[row * a.top + r] = (value_of(k) - m) - l;
           gbl(a.top_token)[row * a.top + r] = token_of(k);
         } else {
-          gbl(a.keys)[id * a.top + r] = k;
+          gbl(a.keys)[(row * a.parts + part) * a.top + r] = k;
         }
       });
       __syncthreads();  // before the next row's keys
@@ -226,15 +314,23 @@ __global__ __launch_bounds__(TPB) void k_logprob(const LogProbArgs a) {
   }
 }
 
-// The parts of a row joined, a wavefront a row and a lane a part.  The parts' keys are in order: the largest of the lanes' next
-// ones is the row's next.
+// The parts of a row joined by a workgroup: a lane a part for the sums, and the parts' keys, each in order, merged two lists
+// at a time by a wavefront: of two lists the largest 64 are max(one's i-th, the other's 63 - i-th), which a merging network
+// puts in order.
+constexpr int kMaxTop = 64;
+static_assert(kMaxTop == kWave, "a lane a key");
 template <typename T>
-__global__ __launch_bounds__(kWave) void k_logprob_join(const LogProbArgs a) {
-  extern __shared__ uint64_t keys[];  // [parts][top]
-  const int lane = int(threadIdx.x);
+__global__ __launch_bounds__(kThreads) void k_logprob_join(const LogProbArgs a) {
+  extern __shared__ uint64_t keys[];  // [parts up to a power of two][64], zeros past a list's end
+  const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave, waves = kThreads / kWave;
   const float none = -__builtin_inff();
+  int lists = 1;
+  while (lists < a.parts) lists *= 2;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    for (int k = lane; k < a.parts * a.top; k += kWave) keys[k] = gbl(a.keys)[row * a.parts * a.top + k];
+    if (a.top > 0) {
+      for (int p = wave; p < lists; p += waves)
+        keys[p * kWave + lane] = p < a.parts && lane < a.top ? gbl(a.keys)[(row * a.parts + p) * a.top + lane] : 0;
+    }
     float m = none, s = 0.0f, t = 0.0f;
     if (lane < a.parts) {
       const CAME8_GLOBAL float* p = gbl(a.part) + (row * a.parts + lane) * 4;
@@ -250,7 +346,7 @@ __global__ __launch_bounds__(kWave) void k_logprob_join(const LogProbArgs a) {
     const float shifted = f > 0.0f && m != most ? fmaf(s, d, t) : t;
     const float all = wave_sum(f > 0.0f ? s * f : (s == s ? 0.0f : s)), ent = wave_sum(f > 0.0f ? shifted * f : 0.0f);
     const float l = logf(all);
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
       const int64_t token = token_at(a.tokens, row, a.wide);
       const bool in = token >= 0 && token < a.V;
       const float z = in ? T::load(gbl(static_cast<const typename T::storage*>(a.z))[row * a.ld + token]) : 0.0f;
@@ -259,18 +355,23 @@ __global__ __launch_bounds__(kWave) void k_logprob_join(const LogProbArgs a) {
       gbl(a.stats)[2 * row] = most;
       gbl(a.stats)[2 * row + 1] = l;
     }
-    __syncthreads();
-    int next = 0;
-    uint64_t head = lane < a.parts && a.top > 0 ? keys[lane * a.top] : 0;
-    for (int r = 0; r < a.top; ++r) {
-      uint64_t k = head;
+    if (a.top == 0) continue;
+    for (int left = lists / 2; left > 0; left /= 2) {
+      __syncthreads();
+      for (int p = wave; p < left; p += waves) {  // lists p and p + left
+        uint64_t k = max(keys[p * kWave + lane], keys[(p + left) * kWave + kWave - 1 - lane]);
 #pragma unroll
-      for (int o = 1; o < kWave; o *= 2) k = max_xor(k, o);
-      if (head == k && k != 0) {  // one lane: keys are different
-        gbl(a.top_log_prob)[row * a.top + r] = (value_of(k) - most) - l;
-        gbl(a.top_token)[row * a.top + r] = token_of(k);
-        head = ++next < a.top ? keys[lane * a.top + next] : 0;
+        for (int o = kWave / 2; o > 0; o /= 2) {
+          const uint64_t other = uint64_t(uint32_t(__shfl_xor(int(k >> 32), o, kWave))) << 32 | uint32_t(__shfl_xor(int(uint32_t(k)), o, kWave));
+          k = (lane & o) == 0 ? max(k, other) : min(k, other);
+        }
+        keys[p * kWave + lane] = k;
       }
+    }
+    if (wave == 0 && lane < a.top) {
+      const uint64_t k = keys[lane];  // this wavefront's own merge was the last
+      gbl(a.top_log_prob)[row * a.top + lane] = (value_of(k) - most) - l;
+      gbl(a.top_token)[row * a.top + lane] = token_of(k);
     }
     __syncthreads();
   }
@@ -286,7 +387,6 @@ struct LogProbBackArgs {
   const float* dentropy;   // or null
   void* dz;
   int64_t rows, V, ld;
-  int32_t parts;  // workgroups a row
   int32_t wide;
 };
 
@@ -295,9 +395,8 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void k_logprob_back(const LogProbBackArgs a) {
   using S = typename T::storage;
   constexpr int V = kChunk<T>;
-  const int64_t all = a.rows * a.parts;
-  for (int64_t id = blockIdx.x; id < all; id += gridDim.x) {
-    const int64_t row = id / a.parts, first = (id - row * a.parts) * (kThreads * kBackChunks * V) + int64_t(threadIdx.x) * V;
+  const int64_t first = int64_t(blockIdx.y) * (kThreads * kBackChunks * V) + int64_t(threadIdx.x) * V;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t token = token_at(a.tokens, row, a.wide);
     const bool in = token >= 0 && token < a.V;
     const float g = a.dlog_prob && in ? gbl(a.dlog_prob)[row] : 0.0f, gh = a.dentropy ? gbl(a.dentropy)[row] : 0.0f;
@@ -310,7 +409,7 @@ __global__ __launch_bounds__(kThreads) void k_logprob_back(const LogProbBackArgs
     const S* z = static_cast<const S*>(a.z) + row * a.ld;
     u32x4 raw[kBackChunks];
 #pragma unroll
-    for (int i = 0; i < kBackChunks; ++i) raw[i] = load_raw<T>(z, first + i * kThreads * V, a.V);
+    for (int i = 0; i < kBackChunks; ++i) raw[i] = load_raw<T, true>(z, first + i * kThreads * V, a.V);
     const float m = gbl(a.stats)[2 * row], l = gbl(a.stats)[2 * row + 1], h = gbl(a.entropy)[row];
 #pragma unroll
     for (int i = 0; i < kBackChunks; ++i) {
@@ -326,7 +425,8 @@ __global__ __launch_bounds__(kThreads) void k_logprob_back(const LogProbBackArgs
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] += e0 + e == token ? g : 0.0f;
       }
-      store_chunk<T>(to, e0, a.V, x);
+      if (e0 + V <= a.V) st_nt16((CAME8_GLOBAL u32x4b*)(gbl(to) + e0), pack<T>(x));
+      else store_chunk<T>(to, e0, a.V, x);
     }
   }
 }
@@ -356,16 +456,20 @@ Cut cut_of(const came8_log_probs* p) {
 template <typename T, bool TOP>
 void forward(const LogProbArgs& a, hipStream_t stream) {
   const int64_t chunks = a.length / kChunk<T>;
-  const dim3 grid{unsigned(std::min<int64_t>(a.rows * a.parts, kMaxGroups))};
-  auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(unsigned(threads)), 0, stream, a); };
+  auto go = [&](auto kernel, int threads) {
+    const dim3 grid(unsigned(std::min(a.rows, kMaxGroups / a.parts)), unsigned(a.parts));
+    hipLaunchKernelGGL(kernel, grid, dim3(unsigned(threads)), 0, stream, a);
+  };
   if (chunks <= kWave * 2) go(k_logprob<T, kWave, 2, TOP>, kWave);
   else if (chunks <= kWave * 8 && a.rows * a.parts >= kEnough) go(k_logprob<T, kWave, 8, TOP>, kWave);
   else if (chunks <= kPartThreads) go(k_logprob<T, kPartThreads, 1, TOP>, kPartThreads);
   else if (chunks <= kPartThreads * 2) go(k_logprob<T, kPartThreads, 2, TOP>, kPartThreads);
   else if (chunks <= kPartThreads * 4) go(k_logprob<T, kPartThreads, 4, TOP>, kPartThreads);
   else go(k_logprob<T, kPartThreads, kPartChunks, TOP>, kPartThreads);
+  unsigned lists = 1;
+  while (lists < unsigned(a.parts)) lists *= 2;
   if (a.parts > 1)
-    hipLaunchKernelGGL(k_logprob_join<T>, dim3(unsigned(std::min(a.rows, kMaxGroups))), dim3(kWave), unsigned(a.parts * a.top * 8), stream, a);
+    hipLaunchKernelGGL(k_logprob_join<T>, dim3(unsigned(std::min(a.rows, kMaxGroups))), dim3(kThreads), a.top > 0 ? lists * kMaxTop * 8 : 0u, stream, a);
 }
 
 struct Layout {
@@ -477,9 +581,9 @@ int came8_log_probs_backward(const came8_log_probs* p, const void* logits, const
     by_type(p->dtype, [&](auto t) {
       using T = decltype(t);
       const int64_t parts = ceil_div(p->vocab, kThreads * kBackChunks * kChunk<T>);
-      const LogProbBackArgs a{logits, tokens, stats, entropy, dlog_prob, dentropy, dlogits, p->rows, p->vocab, p->ld, int32_t(parts),
+      const LogProbBackArgs a{logits, tokens, stats, entropy, dlog_prob, dentropy, dlogits, p->rows, p->vocab, p->ld,
                               p->token_bytes == 8};
-      hipLaunchKernelGGL(k_logprob_back<T>, dim3(unsigned(std::min(p->rows * parts, kMaxGroups))), dim3(kThreads), 0,
+      hipLaunchKernelGGL(k_logprob_back<T>, dim3(unsigned(std::min(p->rows, kMaxGroups)), unsigned(parts)), dim3(kThreads), 0,
                          static_cast<hipStream_t>(stream), a);
     });
     return op_check_launch("log_probs_backward");

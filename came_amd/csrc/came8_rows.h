@@ -9,6 +9,10 @@ namespace came8 {
 // 16 bytes at any address
 typedef uint32_t u32x4b __attribute__((ext_vector_type(4), aligned(1)));
 
+// a streamed operand's (came8_device.h: ld_nt, whose template would forget the alignment)
+__device__ __forceinline__ u32x4 ld_nt16(const CAME8_GLOBAL u32x4b* p) { return __builtin_nontemporal_load(p); }
+__device__ __forceinline__ void st_nt16(CAME8_GLOBAL u32x4b* p, u32x4 v) { __builtin_nontemporal_store(v, p); }
+
 // 8-bit codes
 struct I8 {
   using storage = int8_t;
@@ -20,14 +24,16 @@ constexpr int kChunk = 16 / int(sizeof(typename T::storage));
 
 // Chunk at element e0 of a row of D, zeros past its end, or what `fill` holds in each word.  Rows of odd widths start anywhere: gfx950 loads 16 bytes from any
 // address in one instruction.
-template <typename T, typename I>
+// NT: a streamed operand, that no one reads again soon.
+template <typename T, bool NT = false, typename I>
 __device__ __forceinline__ u32x4 load_raw(const typename T::storage* row, I e0, I D, uint32_t fill = 0u) {
   using S = typename T::storage;
   constexpr int V = kChunk<T>;
   const CAME8_GLOBAL S* p = gbl(row) + e0;
   u32x4 w = {fill, fill, fill, fill};
   if (e0 + V <= D) {
-    w = *(const CAME8_GLOBAL u32x4b*)p;
+    if constexpr (NT) w = ld_nt16((const CAME8_GLOBAL u32x4b*)p);
+    else w = *(const CAME8_GLOBAL u32x4b*)p;
   } else if (e0 < D) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
