@@ -1,7 +1,7 @@
 // The product of 8-bit rows, y[i][j] = (sum over k of q[i][k] w[j][k]) * scale[i] * w_scale[j] + bias[j]: the sums exact in 32 bits
 // by v_mfma_i32_16x16x64_i8, the rest in the epilogue.
 //
-// Up to 64 rows read the weights once and are bound by that; more go through tiles in LDS.
+// A few rows read the weights once and are bound by that; more go through tiles in LDS.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -68,12 +68,69 @@ __device__ __forceinline__ u32x4 load_cut(const int8_t* row, int e0, int K) {
   return out;
 }
 
+// One or two rows of q: a wavefront reads rows of weights whole, 1024 codes in a load, four rows and 4096 codes at a time, and
+// takes four products in an instruction (v_dot4_i32_i8); q's codes stay in registers.  Matrix instructions want 64 codes of 16 rows
+// in a load, which memory gives more slowly (1 x 4096 x 32000 21 us, 6.2 TB/s, instead of 28).
+template <typename T, int M>
+__global__ __launch_bounds__(kThreads) void k_int8_vector(const Int8Args a) {
+  constexpr int R = 4, C = 4, kStep = kWave * 16;
+  const int lane = int(threadIdx.x) % kWave, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int n0 = (int(blockIdx.x) * (kThreads / kWave) + wave) * R;
+  if (n0 >= a.N) return;
+  const int8_t* w[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) w[r] = a.w + int64_t(min(n0 + r, a.N - 1)) * a.ld_w;
+  int32_t acc[R][M] = {};
+  for (int k0 = 0; k0 < a.K; k0 += C * kStep) {
+    u32x4 wf[R][C], x[M][C];
+    auto load = [&](const int8_t* row, int c, bool stream) __attribute__((always_inline)) {
+      const int e0 = k0 + c * kStep + lane * 16;
+      if (k0 + (c + 1) * kStep <= a.K) {  // all lanes'
+        const CAME8_GLOBAL u32x4b* p = (const CAME8_GLOBAL u32x4b*)(gbl(row) + e0);
+        return stream ? ld_nt16(p) : u32x4(*p);
+      }
+      return k0 + c * kStep < a.K ? load_cut(row, e0, a.K) : u32x4{0u, 0u, 0u, 0u};
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c) wf[r][c] = load(w[r], c, true);
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[m][c] = load(a.q + int64_t(min(m, a.M - 1)) * a.ld_q, c, false);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int m = 0; m < M; ++m) acc[r][m] = __builtin_amdgcn_sdot4(int(wf[r][c][e]), int(x[m][c][e]), acc[r][m], false);
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    i32x4 sum;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      uint32_t v = uint32_t(acc[r][m]);
+      v += dpp_u32<kDppXor1>(v);
+      v += dpp_u32<kDppXor2>(v);
+      v += dpp_u32<kDppHalfMirror>(v);
+      v += dpp_u32<kDppMirror>(v);
+      v += swz_xor16_u32(v);
+      sum[r] = int32_t(readlane_u32(v, 0) + readlane_u32(v, 32));
+    }
+    if (lane == m && m < a.M) store_scaled<T>(a, m, n0, sum);
+  }
+}
+
 // 16 rows of weights at a time for a workgroup, an eighth of k a wavefront: fragments go from memory to the matrix instructions,
 // and the wavefronts' sums are joined in LDS.  FM: 16 rows of q each.
 //
-// DEEP steps of 64 codes are loaded together.  AHEAD: the weights' next ones meanwhile, those of the workgroup's next 16 rows
-// too, so that memory is never waited for by all; two workgroups on a CU.  Without, a workgroup has 16 rows alone, and its
-// loads are as deep as registers go: where there are no more than 256 of them, what counts is how often a wavefront waits.
+// DEEP steps of 64 codes are loaded together.  AHEAD (16 rows of q at most): the weights' next ones meanwhile, those of the
+// workgroup's next 16 rows too; two workgroups on a CU.  Without, a workgroup has 16 rows alone, and its loads are as deep as
+// registers go: where there are no more than 256 of them, what counts is how often a wavefront waits.
 template <typename T, int FM, int DEEP, bool AHEAD>
 __global__ __launch_bounds__(512, AHEAD ? 4 : 2) void k_int8_few(const Int8Args a) {
   constexpr int kWaves = 8;
@@ -93,10 +150,7 @@ __global__ __launch_bounds__(512, AHEAD ? 4 : 2) void k_int8_few(const Int8Args 
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {
       to[d] = u32x4{0u, 0u, 0u, 0u};
-      if (s + d < last && b < blocks) {
-        if constexpr (AHEAD) to[d] = ld_nt16((const CAME8_GLOBAL u32x4b*)(w + (s + d) * 64));
-        else to[d] = *(const CAME8_GLOBAL u32x4b*)(w + (s + d) * 64);
-      }
+      if (s + d < last && b < blocks) to[d] = *(const CAME8_GLOBAL u32x4b*)(w + (s + d) * 64);
     }
   };
   auto fetch_x = [&](int s) __attribute__((always_inline)) {
@@ -328,8 +382,10 @@ __global__ __launch_bounds__(kThreads) void k_int8_pack(const int8_t* p, int64_t
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up(int64_t n, int64_t a) { return ceil_div(n, a) * a; }
 
-// few rows read the weights once; rows that do not hold 16 codes go through tiles, which copy them
-bool is_few(const came8_int8_linear* l) { return l->rows <= 64 && l->in >= 16; }
+// Up to 16 rows read the weights once; so do up to 64 where there are no more than 256 times 16 rows of weights, which a workgroup
+// each reads in one or two batches of loads (48 x 5461 x 2048 16.0 us, in tiles 17.3; 24 x 4096 x 4096 15.6 and 18.9; but 40 x
+// 11008 x 4096 28.2 and 23.5, 64 x 4096 x 11008 34.7 and 22.2).  Rows that do not hold 16 codes go through tiles, which copy them.
+bool is_few(const came8_int8_linear* l) { return l->in >= 16 && (l->rows <= 16 || (l->rows <= 64 && l->out <= 4096 && l->in <= 6144)); }
 constexpr int64_t kAtOnce = 512;                  // workgroups of 512 threads that the GPU holds at once, two on a CU
 constexpr int64_t kMaxStride = int64_t(1) << 20;  // bytes: a tile's 256 rows stay below 2^31
 constexpr int64_t kMaxIn = 131071;                // 2^31 - 1 holds that many products of -128 by -128
@@ -390,13 +446,15 @@ template <typename T>
 void forward(const came8_int8_linear* l, Int8Args a, char* ws, hipStream_t stream) {
   if (is_few(l)) {
     const int64_t blocks = ceil_div(l->out, 16);
-    const dim3 each{unsigned(blocks)}, ahead{unsigned(std::min(blocks, kAtOnce))};
-    if (l->rows <= 16) hipLaunchKernelGGL((k_int8_few<T, 1, 8, true>), ahead, dim3(512), 0, stream, a);
-    else if (blocks <= kAtOnce / 2 && l->rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2, 12, false>), each, dim3(512), 0, stream, a);
-    else if (blocks <= kAtOnce / 2 && l->rows <= 48) hipLaunchKernelGGL((k_int8_few<T, 3, 11, false>), each, dim3(512), 0, stream, a);
-    else if (blocks <= kAtOnce / 2) hipLaunchKernelGGL((k_int8_few<T, 4, 8, false>), each, dim3(512), 0, stream, a);
-    else if (l->rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2, 4, true>), ahead, dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((k_int8_few<T, 4, 3, true>), ahead, dim3(512), 0, stream, a);
+    const dim3 fours{unsigned(blocks)}, each{unsigned(blocks)}, ahead{unsigned(std::min(blocks, kAtOnce))};
+    // with fewer rows of weights the wavefronts that read them whole are too few (1 x 11008 x 4096 17.5 us, 16.2 so; 1 x 4096 x 32000
+    // 25.0 and 32.0; 4 rows 33.6 and 32.4)
+    if (l->rows == 1 && blocks >= kAtOnce) hipLaunchKernelGGL((k_int8_vector<T, 1>), fours, dim3(kThreads), 0, stream, a);
+    else if (l->rows == 2 && blocks >= kAtOnce) hipLaunchKernelGGL((k_int8_vector<T, 2>), fours, dim3(kThreads), 0, stream, a);
+    else if (l->rows <= 16) hipLaunchKernelGGL((k_int8_few<T, 1, 8, true>), ahead, dim3(512), 0, stream, a);
+    else if (l->rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2, 12, false>), each, dim3(512), 0, stream, a);
+    else if (l->rows <= 48) hipLaunchKernelGGL((k_int8_few<T, 3, 11, false>), each, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((k_int8_few<T, 4, 8, false>), each, dim3(512), 0, stream, a);
     return;
   }
   const Layout o = layout_of(l);

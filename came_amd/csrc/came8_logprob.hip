@@ -152,7 +152,7 @@ struct Maximum<F16> {
 // A part of a row a workgroup of TPB threads, NV chunks a thread.
 //
 // Rows that have logits of -inf are gone over again with their terms of t bounded, which would cost all rows an instruction a
-// logit.  8192 rows of 32000 in bf16: TODO us.
+// logit.  8192 rows of 32000 in bf16: 95 us, 5.5 TB/s.
 template <typename T, int TPB, int NV, bool TOP>
 __global__ __launch_bounds__(TPB, 6) void k_logprob(const LogProbArgs a) {
   using S = typename T::storage;
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void k_logprob_back(const LogProbBackArgs
     S* to = static_cast<S*>(a.dz) + row * a.V;
     if (g == 0.0f && gh == 0.0f) {
 #pragma unroll
-      for (int i = 0; i < kBackChunks; ++i) store_raw<T>(to, first + i * kThreads * V, a.V, u32x4{0u, 0u, 0u, 0u});
+      for (int i = 0; i < kBackChunks; ++i) store_raw<T, true>(to, first + i * kThreads * V, a.V, u32x4{0u, 0u, 0u, 0u});
       continue;
     }
     const S* z = static_cast<const S*>(a.z) + row * a.ld;
@@ -425,8 +425,7 @@ __global__ __launch_bounds__(kThreads) void k_logprob_back(const LogProbBackArgs
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] += e0 + e == token ? g : 0.0f;
       }
-      if (e0 + V <= a.V) st_nt16((CAME8_GLOBAL u32x4b*)(gbl(to) + e0), pack<T>(x));
-      else store_chunk<T>(to, e0, a.V, x);
+      store_chunk<T, true>(to, e0, a.V, x);
     }
   }
 }

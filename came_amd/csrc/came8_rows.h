@@ -72,13 +72,14 @@ __device__ __forceinline__ u32x4 pack(const float (&x)[kChunk<T>]) {
   return w;
 }
 
-template <typename T, typename I>
+template <typename T, bool NT = false, typename I>
 __device__ __forceinline__ void store_raw(typename T::storage* row, I e0, I D, const u32x4& w) {
   using S = typename T::storage;
   constexpr int V = kChunk<T>;
   CAME8_GLOBAL S* p = gbl(row) + e0;
   if (e0 + V <= D) {
-    *(CAME8_GLOBAL u32x4b*)p = w;
+    if constexpr (NT) st_nt16((CAME8_GLOBAL u32x4b*)p, w);
+    else *(CAME8_GLOBAL u32x4b*)p = w;
   } else if (e0 < D) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -89,9 +90,9 @@ __device__ __forceinline__ void store_raw(typename T::storage* row, I e0, I D, c
   }
 }
 
-template <typename T, typename I>
+template <typename T, bool NT = false, typename I>
 __device__ __forceinline__ void store_chunk(typename T::storage* row, I e0, I D, const float (&x)[kChunk<T>]) {
-  store_raw<T>(row, e0, D, pack<T>(x));
+  store_raw<T, NT>(row, e0, D, pack<T>(x));
 }
 
 // Sums over groups of L lanes, L = 16 or 64, in a fixed order

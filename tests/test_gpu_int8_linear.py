@@ -35,7 +35,9 @@ def _check(q, s, w, ws, b, dtype):
 
 @pytest.mark.parametrize("dtype,bias", [(F32, True), (BF16, False), (F16, True)])
 @pytest.mark.parametrize("T,K,N", [(1, 1, 1), (1, 64, 16), (1, 129, 17), (1, 4096, 500), (3, 1000, 33), (15, 63, 100), (16, 512, 48),
-                                   (17, 513, 31), (32, 200, 65), (33, 2731, 90), (48, 5461, 130), (64, 128, 16), (64, 777, 1)])
+                                   (17, 513, 31), (32, 200, 65), (33, 2731, 90), (48, 5461, 130), (64, 128, 16), (64, 777, 1),
+                                   (2, 15, 40), (3, 16, 20), (1, 16, 8193), (1, 4096, 8300), (2, 5461, 8200), (2, 1025, 9001), (1, 9001, 8192),
+                                   (16, 11008, 700), (20, 6144, 4096), (20, 6145, 100), (40, 1000, 4097), (64, 6144, 70)])
 def test_few_rows(T, K, N, dtype, bias):
     gen = torch.Generator().manual_seed(T + K + N)
     _check(*_operands(T, K, N, dtype, bias, gen), dtype)
