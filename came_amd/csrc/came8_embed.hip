@@ -333,8 +333,8 @@ int check(const char* what, const came8_embedding* e) {
     return op_fail(CAME8_EINVAL, at + "unknown dtype " + std::to_string(e->dtype));
   if (e->token_bytes != 4 && e->token_bytes != 8) return op_fail(CAME8_EINVAL, at + "token_bytes must be 4 or 8");
   const int64_t most = int64_t(1) << 31;
-  if (e->tokens < 0 || e->tokens >= most || e->vocab < 1 || e->vocab >= most || e->dim < 1 || e->dim > (int64_t(1) << 23))
-    return op_fail(CAME8_EINVAL, at + "tokens must be in [0, 2^31), vocab in [1, 2^31), dim in [1, 2^23]");
+  if (e->tokens < 0 || e->tokens >= most || e->vocab < 1 || e->vocab > (int64_t(1) << 26) || e->dim < 1 || e->dim > (int64_t(1) << 23))
+    return op_fail(CAME8_EINVAL, at + "tokens must be in [0, 2^31), vocab in [1, 2^26], dim in [1, 2^23]");
   if (e->ld_weight < e->dim || e->ld_weight > most)
     return op_fail(CAME8_EINVAL, at + "a row stride must be at least the row's length and at most 2^31");
   if (e->padding < -1 || e->padding >= e->vocab) return op_fail(CAME8_EINVAL, at + "padding must be a token or -1");

@@ -408,7 +408,7 @@ int came8_gated_ffn_backward(const came8_ffn* f, const void* x, const void* w_ga
 /* y[i] = scale * weight[token[i]]; tokens are int32_t (token_bytes 4) or int64_t (8).  A token outside [0, vocab) gives a row of
  * zeros and has no gradient (a table whose rows are split over processes). */
 typedef struct came8_embedding {
-  int64_t tokens, vocab, dim; /* tokens below 2^31, vocab in [1, 2^31), dim in [1, 2^23] */
+  int64_t tokens, vocab, dim; /* tokens below 2^31, vocab in [1, 2^26], dim in [1, 2^23] */
   int64_t ld_weight;
   int64_t padding;            /* the token whose row has no gradient, or -1 */
   float scale;

@@ -35,7 +35,7 @@ PROBS = (4, 100, 100, L.CAME8_BF16, 8, 5, 0)
 
 @pytest.mark.parametrize("kw,match", [
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(token_bytes=2), "token_bytes"), (dict(tokens=-1), "tokens"),
-    (dict(tokens=1 << 31), "tokens"), (dict(vocab=0), "vocab"), (dict(vocab=1 << 31), "vocab"), (dict(dim=0, ld_weight=0), "dim"),
+    (dict(tokens=1 << 31), "tokens"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 26) + 1), "vocab"), (dict(dim=0, ld_weight=0), "dim"),
     (dict(dim=(1 << 23) + 1, ld_weight=1 << 24), "dim"), (dict(ld_weight=7), "stride"), (dict(ld_weight=(1 << 31) + 1), "stride"),
     (dict(padding=-2), "padding"), (dict(padding=10), "padding")])
 def test_embedding_entries_refuse(kw, match):
