@@ -519,7 +519,15 @@ PyObject* int8_linear(PyObject*, PyObject* args) {
     pybind11::gil_scoped_release no_gil;
     c10::OptionalDeviceGuard guard(q.device());
     y = at::empty(sizes_with(q, w.size(0)), q.options().dtype(type));
-    const Rows rq = rows_of(q, int64_t(1) << 20), rw = rows_of(w, int64_t(1) << 20);
+    auto codes_of = [](const at::Tensor& t) {  // rows that could all start on words do
+      Rows r = rows_of(t, int64_t(1) << 20);
+      if (r.ld % 4 == 0 && reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 4 != 0) {
+        r.t = r.t.clone(at::MemoryFormat::Contiguous);
+        r.ld = r.t.size(1);
+      }
+      return r;
+    };
+    const Rows rq = codes_of(q), rw = codes_of(w);
     if (rq.count > 0) {
       const at::Tensor scale = plain(s), w_scale = plain(ws), bias = b ? plain(*b) : at::Tensor();
       const came8_int8_linear l{rq.count, w.size(1), w.size(0), rq.ld, rw.ld, dtype, 0};

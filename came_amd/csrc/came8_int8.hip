@@ -233,8 +233,9 @@ __host__ __device__ constexpr int half_swz(int r) { return (0x1320 >> (r >> 2 & 
 // give zeros.
 //
 // 8192 x 4096 x 11008 401 us (1840 TOP/s; the library's product, unscaled, 405 to 409 beside it), 8192 x 11008 x 4096 320 (295),
-// 512 x 4096 x 11008 41 (40).  With operands on their way through registers 407, 323 and 44; loads at a step's start 405.  The
-// matrix units are busy about half of the time at the clock that power leaves them.
+// 512 x 4096 x 11008 41 (40).  With operands on their way through registers 407, 323 and 44; loads at a step's start 405.  Matrix
+// units are busy 37% of the cycles, at about 2.05 GHz; five steps' places in LDS (412 and 329 beside 412 and 327), four
+// wavefronts of 128 by 128 (459 and 347) or priority for them (419 and 326) gave nothing.
 template <typename T, int B, int WAVES_N>
 __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_int8_gemm(const Int8Args args) {
   constexpr int kWaves = 2 * WAVES_N, kStep = 2 * B * kHalf, kBlocks = B / 16, kLoads = kBlocks / kWaves;  // of an operand
@@ -438,19 +439,22 @@ Cut cut_of(const came8_int8_linear* l) {
 }
 
 struct Layout {
-  int64_t ld_q = 0, ld_w = 0;  // of the copies; 0: read where it is
-  size_t q = 0, w = 0, part = 0, bytes = 256;
+  int64_t ld = 0;  // of the copies of operands whose rows do not all start on words, which tiles load
+  bool copy_q = false, copy_w = false;
+  size_t q = 0, w = 0, part = 0, bytes = 0;
 };
-// Whether the rows are copied goes by the strides here, by the addresses too where the call is made: room for both copies
 Layout layout_of(const came8_int8_linear* l) {
   Layout o;
-  if (is_few(l)) return o;
-  const int64_t ld = up(l->in, 16);
-  o.w = size_t(up(l->rows * ld, 256));
-  o.part = o.w + size_t(up(l->out * ld, 256));
-  const Cut c = cut_of(l);
-  o.bytes = o.part + 256 + (c.splits > 1 ? size_t(c.splits * l->rows * up(l->out, 4) * 4) : 0);
-  o.ld_q = o.ld_w = ld;
+  if (!is_few(l)) {
+    o.ld = up(l->in, 16);
+    o.copy_q = l->ld_q % 4 != 0;
+    o.copy_w = l->ld_w % 4 != 0;
+    o.w = o.copy_q ? size_t(up(l->rows * o.ld, 256)) : 0;
+    o.part = o.w + (o.copy_w ? size_t(up(l->out * o.ld, 256)) : 0);
+    const Cut c = cut_of(l);
+    o.bytes = o.part + (c.splits > 1 ? size_t(c.splits * l->rows * up(l->out, 4) * 4) : 0);
+  }
+  o.bytes = std::max<size_t>(o.bytes, 256);
   return o;
 }
 
@@ -470,15 +474,14 @@ void forward(const came8_int8_linear* l, Int8Args a, char* ws, hipStream_t strea
     return;
   }
   const Layout o = layout_of(l);
-  auto words = [&](const int8_t*& p, int64_t& ld, int64_t rows, size_t at) {  // tiles load whole words
-    if (ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0) return;
+  auto copy = [&](const int8_t*& p, int64_t& ld, int64_t rows, size_t at) {
     int8_t* to = reinterpret_cast<int8_t*>(ws + at);
-    hipLaunchKernelGGL(k_int8_pack, dim3(unsigned(std::min<int64_t>(rows, 1 << 16))), dim3(kThreads), 0, stream, p, ld, to, o.ld_q, rows, a.K);
+    hipLaunchKernelGGL(k_int8_pack, dim3(unsigned(std::min<int64_t>(rows, 1 << 16))), dim3(kThreads), 0, stream, p, ld, to, o.ld, rows, a.K);
     p = to;
-    ld = o.ld_q;
+    ld = o.ld;
   };
-  words(a.q, a.ld_q, l->rows, o.q);
-  words(a.w, a.ld_w, l->out, o.w);
+  if (o.copy_q) copy(a.q, a.ld_q, l->rows, o.q);
+  if (o.copy_w) copy(a.w, a.ld_w, l->out, o.w);
   const Cut c = cut_of(l);
   a.tiles_m = int32_t(ceil_div(l->rows, c.tile));
   a.tiles_n = int32_t(ceil_div(l->out, c.tile));
@@ -545,6 +548,9 @@ int came8_int8_linear_forward(const came8_int8_linear* l, const int8_t* q, const
         (rc = check_pointer(what, scale, 4)) != CAME8_OK || (rc = check_pointer(what, w_scale, 4)) != CAME8_OK ||
         (rc = check_pointer(what, y, size)) != CAME8_OK || (bias != nullptr && (rc = check_pointer(what, bias, size)) != CAME8_OK))
       return rc;
+    if (!is_few(l))
+      for (const auto& [p, ld] : {std::pair(q, l->ld_q), std::pair(w, l->ld_w)})
+        if (ld % 4 == 0 && (rc = check_pointer(what, p, 4)) != CAME8_OK) return rc;
     const Layout o = layout_of(l);
     if (!is_few(l) && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < o.bytes))
       return op_fail(CAME8_ESPACE, std::string(what) + ": workspace too small or misaligned");

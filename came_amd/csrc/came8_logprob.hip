@@ -154,7 +154,7 @@ struct Maximum<F16> {
 // Rows that have logits of -inf are gone over again with their terms of t bounded, which would cost all rows an instruction a
 // logit.  8192 rows of 32000 in bf16: 95 us, 5.5 TB/s.
 template <typename T, int TPB, int NV, bool TOP>
-__global__ __launch_bounds__(TPB, 6) void k_logprob(const LogProbArgs a) {
+__global__ __launch_bounds__(TPB, TPB == kWave ? 1 : 6) void k_logprob(const LogProbArgs a) {
   using S = typename T::storage;
   constexpr int V = kChunk<T>, kStep = TPB * V;
   constexpr int kWaves = TPB / kWave;

@@ -14,8 +14,9 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, w_q: torch.Tensor, w_scale
 
     q [..., in], w_q [out, in]: int8; scale [...], w_scale [out]: float32 (``rms_norm_int8`` and ``quantize_rows`` give both);
     bias [out] of ``dtype``.  Up to 131071 codes a row, whose sums are exact in 32 bits; the scales and the bias are applied in
-    float32 and the result is rounded once.  Operands whose rows start at words are read where they are; where there are more
-    than 64 rows, others are copied.  No gradient: scales or a bias that require one are refused unless under
+    float32 and the result is rounded once.  Operands whose rows are contiguous are read where they are; others are copied, as are
+    rows a multiple of 4 bytes apart that do not start on words and, for more than 16 rows of q, ones any other distance apart.
+    No gradient: scales or a bias that require one are refused unless under
     ``torch.no_grad()``.
     """
     code = _CODES.get(dtype)

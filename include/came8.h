@@ -471,8 +471,8 @@ typedef struct came8_int8_linear {
 /* Bytes of device workspace for came8_int8_linear_forward. */
 int came8_int8_linear_workspace_size(const came8_int8_linear* l, size_t* bytes);
 
-/* y is contiguous.  Operands whose rows do not start on words (an ld or an address that is not a multiple of 4) are copied to
- * the workspace first. */
+/* y is contiguous.  With more than 16 rows, an operand whose ld is not a multiple of 4 may be copied to the workspace first; one
+ * whose ld is has an address that is a multiple of 4 too. */
 int came8_int8_linear_forward(const came8_int8_linear* l, const int8_t* q, const float* scale, const int8_t* w,
                               const float* w_scale, const void* bias, void* y, void* workspace, size_t workspace_bytes,
                               void* stream);

@@ -89,6 +89,21 @@ def test_operands_where_they_lie(T):
             assert ((want.cpu().double() - exact).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("T", [3, 16, 70, 300])
+@pytest.mark.parametrize("width", [401, 402, 403, 404])
+def test_rows_any_distance_apart(T, width):
+    """Rows that start on words, on two in four, one in four or none, with other codes between them."""
+    from came_amd import int8_linear
+    gen = torch.Generator().manual_seed(width)
+    wide, weights = _codes(T, width, gen=gen), _codes(130, width + 5, gen=gen)
+    s, ws = torch.rand(T, generator=gen).cuda(), torch.rand(130, generator=gen).cuda()
+    for k0, K in ((0, 400), (1, 399), (2, 80), (3, 145)):
+        q, w = wide[:, k0 : k0 + K], weights[:, 3 - k0 : 3 - k0 + K]
+        got = int8_linear(q, s, w, ws, dtype=F32)
+        exact, bound = orc.int8_linear(q, s, w, ws, None, F32)
+        assert ((got.cpu().double() - exact).abs() <= bound).all(), (k0, K)
+
+
 def test_shapes_and_strides():
     from came_amd import int8_linear, quantize_rows
     gen = torch.Generator().manual_seed(3)

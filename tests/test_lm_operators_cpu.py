@@ -128,7 +128,7 @@ def test_product_entries_refuse_pointers_and_workspaces():
     need = _size("int8_linear", l)[1]
     for i in range(6):  # q, scale, w, w_scale, bias, y
         for bad in (None, P + 1):
-            if (i == 4 and bad is None) or (i in (0, 2) and bad):  # no bias; codes lie anywhere
+            if i == 4 and bad is None:  # no bias
                 continue
             p = [P] * 6
             p[i] = bad
