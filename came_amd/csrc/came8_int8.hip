@@ -205,43 +205,19 @@ __global__ __launch_bounds__(512, AHEAD ? 4 : 2) void k_int8_few(const Int8Args 
 }
 
 // ------------------------------------------------------------------------------------------------------ tiles
-// 16 bytes of every lane from a buffer (zeros past its end) to LDS, successive lanes' to successive places from `at` on.  No
-// register is written, and the compiler does not know: wait_loads() waits.
-__device__ __forceinline__ void load_to_lds(uint32_t at, uint32_t offset, u32x4 buffer) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(buffer) : "memory");
-}
-// until at most N of the wavefront's loads are under way (gfx9's encoding; LDS and exports are not waited for)
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(N < 16, "");
-  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
-}
-__device__ __forceinline__ u32x4 buffer_of(const View& v) {
-  const uint64_t p = reinterpret_cast<uint64_t>(v.p);
-  return u32x4{uint32_t(p), uint32_t(p >> 32) & 0xffffu, uint32_t(buffer_bytes(v.left)), 0x00027000u};
-}
-
-constexpr int kHalf = 64;     // codes of a step
-constexpr int kStages = 4;    // steps that have a place in LDS
-// Chunk c of row r of a step lies at c ^ half_swz(r): a fragment's read, row l % 16 and chunk l / 16, goes by 16 lanes together
-// (0-3, 12-15, 20-23, 24-27 and so on), which are in four places each of four rows so.
-__host__ __device__ constexpr int half_swz(int r) { return (0x1320 >> (r >> 2 & 3) * 4) & 3; }
-
-// Tiles of B by B on 2 by WAVES_N wavefronts.  A step is 64 codes of k: 16 rows of an operand are a load to LDS and a fragment
-// out of it.  In step t the fragments of step t + 1 are read while the matrix instructions take those of step t, and the loads
-// of step t + 3 go out; its place in LDS was last read before the barrier at the step's start.  Past the last step, loads
-// give zeros.
+// Tiles of B by B on 2 by WAVES_N wavefronts.  A step is 128 codes of k; its four phases are laid out as in the feed-forward
+// block's products (came8_ffn.h), and so are the rows in LDS.
 //
-// 8192 x 4096 x 11008 401 us (1840 TOP/s; the library's product, unscaled, 405 to 409 beside it), 8192 x 11008 x 4096 320 (295),
-// 512 x 4096 x 11008 41 (40).  With operands on their way through registers 407, 323 and 44; loads at a step's start 405.  Matrix
-// units are busy 37% of the cycles, at about 2.05 GHz; five steps' places in LDS (412 and 329 beside 412 and 327), four
-// wavefronts of 128 by 128 (459 and 347) or priority for them (419 and 326) gave nothing.
+// Codes of normal values, inputs in turn: 8192 x 4096 x 11008 415 us (1780 TOP/s; the library's unscaled product 405 beside it),
+// 8192 x 11008 x 4096 340, 2048 x 4096 x 4096 45, 128 x 4096 x 11008 23.  Power bounds it: 20 calls after a pause run at 1900
+// TOP/s.  Operands loaded straight to LDS, in steps of 64 codes, four of them in flight, were slower on the same inputs (438, 346,
+// 48, 22), with matrix units busy 37% of the cycles at 2.05 GHz, whether five steps were in flight, four wavefronts took 128
+// by 128 each, or not.
 template <typename T, int B, int WAVES_N>
 __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_int8_gemm(const Int8Args args) {
-  constexpr int kWaves = 2 * WAVES_N, kStep = 2 * B * kHalf, kBlocks = B / 16, kLoads = kBlocks / kWaves;  // of an operand
+  constexpr int NT = 2 * WAVES_N * kWave, BK = kRowBytes, kTileBytes = 2 * B * kRowBytes;
   constexpr int WM = B / 2, WN = B / WAVES_N, FM = WM / 16, FN = WN / 16;
-  static_assert(kBlocks % kWaves == 0, "");
-  __shared__ __attribute__((aligned(16))) char lds[kStages * kStep];
+  __shared__ __attribute__((aligned(16))) char lds[2 * kTileBytes];
 
   int tm, tn, split;
   {
@@ -257,95 +233,112 @@ __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_int8_gemm(const Int8
     tn = in / rows;
   }
   const int m0 = tm * B, n0 = tn * B;
-  const int lane = int(threadIdx.x) % kWave, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
   const int wm = wave % 2, wn = wave / 2;
 
-  const int steps = (args.K + kHalf - 1) / kHalf;
+  constexpr int D = B < 256 ? 2 : 1;
+  Stage<I8, B, NT, true> sa[D], sb[D];
+  const int steps = (args.K + BK - 1) / BK;
   const int begin = int(int64_t(steps) * split / args.splits), total = int(int64_t(steps) * (split + 1) / args.splits) - begin;
   auto view = [&](const int8_t* p, int64_t ld, int at, int extent) {
     View v;
     v.p = reinterpret_cast<const char*>(p) + at * ld;
     v.left = view_bytes(true, extent - at, args.K, ld, 1);
-    v.step = kHalf;
+    v.step = kRowBytes;
     v.ld = int32_t(ld);
     v.next(begin);
     return v;
   };
   View va = view(args.q, args.ld_q, m0, args.M), vb = view(args.w, args.ld_w, n0, args.N);
-  const int chunk = (lane & 3) ^ half_swz(lane >> 2);
-  const uint32_t from_a = uint32_t((wave * 16 + lane / 4) * va.ld + chunk * 16), from_b = uint32_t((wave * 16 + lane / 4) * vb.ld + chunk * 16);
-  const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-  int next = 0, left = args.K - begin * kHalf;  // the step that is loaded next, and K less its first k
-  auto load = [&]() __attribute__((always_inline)) {
-    const uint32_t at = base + uint32_t((next % kStages) * kStep + wave * 1024);
-    const bool out = chunk * 16 >= left || next >= total;
-    const u32x4 ba = buffer_of(va), bb = buffer_of(vb);
+  int left = args.K - begin * BK;
+  auto fetch = [&](int slot) __attribute__((always_inline)) {
+    sa[slot].fetch(va, va, left);
+    sb[slot].fetch(vb, vb, left);
+    // a chunk that K cuts: what is past K in q's becomes zero, so w's does not count
+    if (__builtin_expect(left > 0 && left < BK && left % 16 != 0, 0)) {
+      const int in = left - int(threadIdx.x & 7) * 16;
+      if (in > 0 && in < 16) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_to_lds(at + i * kWaves * 1024, out ? kNowhere : from_a + uint32_t(i * kWaves * 16 * va.ld), ba);
+        for (int i = 0; i < Stage<I8, B, NT, true>::kLoads; ++i)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      load_to_lds(at + B * kHalf + i * kWaves * 1024, out ? kNowhere : from_b + uint32_t(i * kWaves * 16 * vb.ld), bb);
+          for (int e = 0; e < 4; ++e) {
+            const int bytes = in - 4 * e;
+            sa[slot].v[i][e] &= bytes >= 4 ? ~0u : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
+          }
+      }
+    }
     va.next();
     vb.next();
-    left -= kHalf;
-    ++next;
+    left -= BK;
   };
   i32x4 acc[FM][FN] = {};
-  u32x4 fa[2][FM], fb[2][FN];
-  const int place = (lane % 16) * kHalf + ((lane / 16) ^ half_swz(lane % 16)) * 16;
-  auto read = [&](int t, int set) __attribute__((always_inline)) {
-    const char* at = lds + (t % kStages) * kStep + place;
-#pragma unroll
-    for (int i = 0; i < FM; ++i) fa[set][i] = *reinterpret_cast<const u32x4*>(at + (wm * WM + i * 16) * kHalf);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) fb[set][j] = *reinterpret_cast<const u32x4*>(at + (B + wn * WN + j * 16) * kHalf);
+  auto put = [&](int t, int slot) __attribute__((always_inline)) {
+    char* to = lds + (t & 1) * kTileBytes;
+    sa[slot].put(to);
+    sb[slot].put(to + B * kRowBytes);
   };
-  // The chunk that K cuts, in step t: what is past K in q's becomes zero in LDS, so w's does not count
-  const int last = total - 1, cut = split + 1 == args.splits ? args.K % 16 : 0;
-  auto trim = [&](int t) __attribute__((always_inline)) {
-    if (t != last || cut == 0) return;
-    const int c = args.K % kHalf / 16;
-    for (int r = int(threadIdx.x); r < B; r += kWaves * kWave) {
-      u32x4* p = reinterpret_cast<u32x4*>(lds + (t % kStages) * kStep + r * kHalf + (c ^ half_swz(r)) * 16);
-      u32x4 v = *p;
+  const int fr = lane % 16;
+  uint32_t pa[4], pb[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int bytes = cut - 4 * e;
-        v[e] &= bytes >= 4 ? ~0u : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
-      }
-      *p = v;
-    }
-    __syncthreads();
-  };
-  load();
-  load();
-  load();
-  wait_loads<4 * kLoads>();
-  __syncthreads();
-  trim(0);
-  read(0, 0);
-  auto step = [&](int t, int set) __attribute__((always_inline)) {
-    wait_loads<2 * kLoads>();  // of steps up to t + 1 none is under way
-    __syncthreads();
-    trim(t + 1);
-    read(t + 1, set ^ 1);
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = mfma_i8(fb[set][j], fa[set][i], acc[i][j]);
-    interleave<kDsRead, FM + FN, FM * FN>();
-    load();
-  };
-  for (int t = 0; t < total; t += 2) {
-    step(t, 0);
-    step(t + 1, 1);  // past the last one of zeros
+  for (int v = 0; v < 4; ++v) {
+    pa[v] = uint32_t((wm * WM + fr) * kRowBytes + (lane / 16 ^ swz(wm * (WM % 64) + fr) ^ (2 * v)) * kChunkBytes);
+    pb[v] = uint32_t((B + wn * WN + fr) * kRowBytes + (lane / 16 ^ swz(wn * (WN % 64) + fr) ^ (2 * v)) * kChunkBytes);
   }
-  wait_loads<0>();  // LDS is used again
+  u32x4 lo[FM / 2], hi[FM / 2], fb[2][FN];
+  auto read_a = [&](u32x4(&f)[FM / 2], int t, int s, int i0) __attribute__((always_inline)) {
+    const char* a = lds + (t & 1) * kTileBytes;
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i)
+      f[i] = *reinterpret_cast<const u32x4*>(a + pa[(4 * s ^ swz(16 * (i0 + i))) / 2] + (i0 + i) * 16 * kRowBytes);
+  };
+  auto read_b = [&](int t, int s) __attribute__((always_inline)) {
+    const char* b = lds + (t & 1) * kTileBytes;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      fb[s][j] = *reinterpret_cast<const u32x4*>(b + pb[(4 * s ^ swz(16 * j)) / 2] + j * 16 * kRowBytes);
+  };
+  auto multiply = [&](const u32x4(&f)[FM / 2], int s, int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i0 + i][j] = mfma_i8(fb[s][j], f[i], acc[i0 + i][j]);
+  };
+  constexpr int kProducts = FM / 2 * FN;  // of a phase
+  fetch(0);
+  put(0, 0);
+#pragma unroll
+  for (int d = 1; d <= D; ++d) fetch(d % D);
+  __syncthreads();
+  read_a(lo, 0, 0, 0);
+  read_b(0, 0);
+  auto step = [&](int t, int slot) __attribute__((always_inline)) {  // slot: of step t + 1
+    read_a(hi, t, 0, FM / 2);
+    read_b(t, 1);
+    multiply(lo, 0, 0);
+    interleave<kDsRead, FM / 2 + FN, kProducts>();
+    read_a(lo, t, 1, 0);
+    put(t + 1, slot);
+    fetch(slot);
+    multiply(hi, 0, FM / 2);
+    interleave<kDsRead | kDsWrite | kVmemRead, FM / 2 + FM + FN + 8, kProducts>();
+    read_a(hi, t, 1, FM / 2);
+    multiply(lo, 1, 0);
+    interleave<kDsRead, FM / 2, kProducts>();
+    __syncthreads();  // every wavefront has read its last of step t, and written its part of step t + 1
+    __builtin_amdgcn_sched_barrier(0);
+    read_a(lo, t + 1, 0, 0);
+    read_b(t + 1, 0);
+    multiply(hi, 1, FM / 2);
+    interleave<kDsRead, FM / 2 + FN, kProducts>();
+  };
+  for (int t = 0; t < total; t += D)
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (d == 0 || t + d < total) step(t + d, (d + 1) % D);
 
   // acc[i][j][e]: row 16 i + lane % 16 of the wavefront's, column 16 j + 4 (lane / 16) + e; through the wavefront's own part of
   // LDS, so that lanes of successive columns write memory together
   constexpr int kPart = FM < 4 ? FM : 4, kChunks = WN / 4;
-  static_assert(kWaves * kPart * 16 * WN * 4 <= kStages * kStep, "");
   constexpr int kRows = kWave / kChunks, kRounds = kPart * 16 / kRows;
   char* mine = lds + wave * (kPart * 16 * WN * 4);
   const int cc = lane % kChunks, r0 = lane / kChunks, n = n0 + wn * WN + cc * 4;
