@@ -218,11 +218,20 @@ __global__ __launch_bounds__(TPB, TPB == kWave ? 1 : 6) void k_logprob(const Log
       float x[V];
       unpack_again(raw[i]);
       unpack<T>(raw[i], x);
+      if ((i + 1) * kStep <= n) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = x[e] - base, p = __builtin_amdgcn_exp2f(d * kLog2e);
-        s[0] += p;
-        s[1] = fmaf(p, (i + 1) * kStep <= n ? d : fmaxf(d, kFar), s[1]);  // past the row's end d is -inf
+        for (int e = 0; e < V; ++e) {
+          const float d = x[e] - base, p = __builtin_amdgcn_exp2f(d * kLog2e);
+          s[0] += p;
+          s[1] = fmaf(p, d, s[1]);
+        }
+      } else {  // past the row's end d is -inf
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = x[e] - base, p = __builtin_amdgcn_exp2f(d * kLog2e);
+          s[0] += p;
+          s[1] = fmaf(p, fmaxf(d, kFar), s[1]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);  // a chunk at a time: with all 64 values on their way registers are out
     }
