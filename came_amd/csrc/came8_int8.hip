@@ -209,10 +209,11 @@ __global__ __launch_bounds__(512, AHEAD ? 4 : 2) void k_int8_few(const Int8Args 
 // block's products (came8_ffn.h), and so are the rows in LDS.
 //
 // Codes of normal values, inputs in turn: 8192 x 4096 x 11008 415 us (1780 TOP/s; the library's unscaled product 405 beside it),
-// 8192 x 11008 x 4096 340, 2048 x 4096 x 4096 45, 128 x 4096 x 11008 23.  Power bounds it: 20 calls after a pause run at 1900
-// TOP/s.  Operands loaded straight to LDS, in steps of 64 codes, four of them in flight, were slower on the same inputs (438, 346,
-// 48, 22), with matrix units busy 37% of the cycles at 2.05 GHz, whether five steps were in flight, four wavefronts took 128
-// by 128 each, or not.
+// 8192 x 11008 x 4096 340, 2048 x 4096 x 4096 45, 128 x 4096 x 11008 23.  Matrix units are busy 40% of the cycles, at 1.96 GHz; a
+// step of the large tiles takes 4240 cycles, of which their instructions need 2048, while its 260 KB through LDS take 4060 at 64
+// bytes a cycle.  What was slower: operands loaded straight to LDS in steps of 64 codes, four or five in flight (438, 346, 48,
+// 22); four wavefronts of 128 by 128, which read less of LDS (459); the weights' fragments loaded from memory past LDS (517 where
+// this took 394).
 template <typename T, int B, int WAVES_N>
 __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_int8_gemm(const Int8Args args) {
   constexpr int NT = 2 * WAVES_N * kWave, BK = kRowBytes, kTileBytes = 2 * B * kRowBytes;

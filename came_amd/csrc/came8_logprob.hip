@@ -164,7 +164,7 @@ __global__ __launch_bounds__(TPB, TPB == kWave ? 1 : 6) void k_logprob(const Log
   const int part = int(blockIdx.y), first = part * a.length, n = int(min(int64_t(a.length), a.V - first));
   int turn = 0;
   // From the last row on, which may still be in the memory-side cache, and the backward pass from the first on, with loads and
-  // stores that leave what this pass has read there: 8192 rows of 32000 in bf16 271 us in all; 306 without those hints, 316 with
+  // stores that leave what this pass has read there: 8192 rows of 32000 in bf16 267 us in all; 306 without those hints, 316 with
   // the rows in one order.
   for (int64_t row = a.rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x, turn ^= 1) {
     const S* z = static_cast<const S*>(a.z) + row * a.ld;

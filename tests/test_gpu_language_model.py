@@ -164,3 +164,76 @@ def test_a_leaf_whose_gradient_lies_on_another_stream(op):
         call(True).sum().backward()
     torch.cuda.synchronize()
     assert torch.equal(leaf.grad, 3 * other)
+
+
+def test_saved_tensors_that_are_made_again():
+    """Checkpointed, the operators' saved tensors are thrown away and the forward pass is run again: the same bits."""
+    from torch.utils.checkpoint import checkpoint
+
+    from came_amd import embedding, rms_norm, token_log_probs
+    gen = torch.Generator().manual_seed(9)
+    table, w, head = (torch.randn(*s, generator=gen).cuda().requires_grad_() for s in ((50, 24), (24,), (50, 24)))
+    tokens = torch.randint(0, 50, (40,), generator=gen).cuda()
+
+    def loss(table, w, head):
+        h = embedding(tokens[:-1], table)
+        y, h = rms_norm(h, w, residual=h)
+        out = token_log_probs((y + h) @ head.t(), tokens[1:])
+        return out.log_probs.sum() + out.entropy.sum()
+
+    want = torch.autograd.grad(loss(table, w, head), (table, w, head))
+    got = torch.autograd.grad(checkpoint(loss, table, w, head, use_reentrant=False), (table, w, head))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_saved_tensors_that_are_written():
+    """A backward pass whose saved tensors were written after the forward pass raises."""
+    from came_amd import embedding, rms_norm, token_log_probs
+    w, x = torch.ones(16, device="cuda", requires_grad=True), torch.randn(3, 16, device="cuda", requires_grad=True)
+    table, tokens = torch.randn(9, 16, device="cuda", requires_grad=True), torch.zeros(3, dtype=torch.int64, device="cuda")
+    y, h = rms_norm(x, w, residual=x)
+    h += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = embedding(tokens, table)
+    tokens += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    z = x * 1.0
+    out = token_log_probs(z, tokens)
+    z *= 2
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.log_probs.sum().backward()
+
+
+def test_calls_of_threads_on_streams_of_their_own():
+    """Calls that run at once share nothing."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from came_amd import int8_linear, quantize_rows, rms_norm_int8, token_log_probs
+    gen = torch.Generator().manual_seed(4)
+    w = torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    rows = [torch.randn(t, 512, generator=gen).bfloat16().cuda() for t in (1, 3, 40, 200)]
+    weights = quantize_rows(torch.randn(9000, 512, generator=gen).bfloat16().cuda())
+    tokens = [torch.randint(0, 9000, (len(x),), generator=gen).cuda() for x in rows]
+
+    def serve(k):
+        with torch.no_grad():
+            logits = int8_linear(*rms_norm_int8(rows[k], w), *weights)
+            return token_log_probs(logits, tokens[k], top=5)
+
+    def in_thread(k):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(stream):
+            out = [serve(k) for _ in range(20)]
+        stream.synchronize()
+        return out
+
+    want = [serve(k) for k in range(4)]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(in_thread, range(4)))
+    for k in range(4):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
