@@ -96,7 +96,7 @@ std::vector<int64_t> sizes_with(const at::Tensor& t, int64_t width) {
   return s;
 }
 
-c10::DataPtr workspace(size_t bytes) { return c10::GetAllocator(at::kCUDA)->allocate(bytes); }
+c10::DataPtr workspace(size_t bytes) { return bytes > 0 ? c10::GetAllocator(at::kCUDA)->allocate(bytes) : c10::DataPtr(); }
 
 void* stream_of(long long stream) { return reinterpret_cast<void*>(stream); }
 
@@ -298,14 +298,15 @@ came8_log_probs log_probs_of(const Rows& z, const at::Tensor& tokens, int64_t to
   return came8_log_probs{z.count, z.t.size(1), z.ld, dtype_code(z.t), tokens.scalar_type() == at::kLong ? 8 : 4, int32_t(top), 0};
 }
 
-// log_probs, entropy and what the backward pass takes beside them
-variable_list log_probs_forward(const at::Tensor& logits, const at::Tensor& tokens, int64_t top, long long stream, Tops* tops) {
+// log_probs, entropy and, with `keep`, what the backward pass takes beside them
+variable_list log_probs_forward(const at::Tensor& logits, const at::Tensor& tokens, int64_t top, long long stream, bool keep, Tops* tops) {
   c10::OptionalDeviceGuard guard(logits.device());
   const Rows z = rows_of(logits, kFar);
   const at::Tensor t = tokens.contiguous();
   const at::TensorOptions f32 = logits.options().dtype(at::kFloat);
   const auto rows = tokens.sizes();
-  at::Tensor lp = at::empty(rows, f32), entropy = at::empty(rows, f32), stats = at::empty({z.count, 2}, f32);
+  at::Tensor lp = at::empty(rows, f32), entropy = at::empty(rows, f32), stats;
+  if (keep) stats = at::empty({z.count, 2}, f32);
   std::vector<int64_t> sizes = rows.vec();
   sizes.push_back(top);
   tops->log_probs = at::empty(sizes, f32);
@@ -314,9 +315,11 @@ variable_list log_probs_forward(const at::Tensor& logits, const at::Tensor& toke
     const came8_log_probs p = log_probs_of(z, t, top);
     size_t bytes = 0;
     entry_check(entries.logprob_size(&p, &bytes), "came8_log_probs_workspace_size");
-    const c10::DataPtr ws = workspace(bytes);
-    entry_check(entries.logprob_forward(&p, z.t.data_ptr(), t.data_ptr(), lp.data_ptr<float>(), entropy.data_ptr<float>(),
-                                        stats.data_ptr<float>(), top > 0 ? tops->log_probs.data_ptr<float>() : nullptr,
+    bytes = (bytes + 15) / 16 * 16;
+    const c10::DataPtr ws = workspace(bytes + (keep ? 0 : size_t(z.count) * 8));
+    float* m_and_l = keep ? stats.data_ptr<float>() : reinterpret_cast<float*>(static_cast<char*>(ws.get()) + bytes);
+    entry_check(entries.logprob_forward(&p, z.t.data_ptr(), t.data_ptr(), lp.data_ptr<float>(), entropy.data_ptr<float>(), m_and_l,
+                                        top > 0 ? tops->log_probs.data_ptr<float>() : nullptr,
                                         top > 0 ? tops->tokens.data_ptr<int64_t>() : nullptr, ws.get(), bytes, stream_of(stream)),
                 "came8_log_probs_forward");
   }
@@ -327,7 +330,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& tokens, int64_t top, int64_t stream,
                                bool captured, Tops* tops) {
     ctx->set_materialize_grads(false);
-    const variable_list out = log_probs_forward(logits, tokens, top, stream, tops);
+    const variable_list out = log_probs_forward(logits, tokens, top, stream, true, tops);
     ctx->save_for_backward({logits, tokens, out[1], out[2]});
     ctx->saved_data["stream"] = stream;
     ctx->saved_data["captured"] = captured;
@@ -567,7 +570,7 @@ PyObject* token_log_probs(PyObject*, PyObject* args) {
     if (at::GradMode::is_enabled() && z.requires_grad())
       out = TokenLogProbs::apply(z, tokens, int64_t(top), int64_t(stream), captured != 0, &tops);
     else
-      out = log_probs_forward(z, tokens, top, stream, &tops);
+      out = log_probs_forward(z, tokens, top, stream, false, &tops);
   }
   return tuple_of({out[0], out[1], tops.log_probs, tops.tokens});
   END_HANDLE_TH_ERRORS

@@ -476,7 +476,6 @@ Layout layout_of(const came8_int8_linear* l) {
     const Cut c = cut_of(l);
     o.bytes = o.part + (c.splits > 1 ? size_t(c.splits * l->rows * up(l->out, 4) * 4) : 0);
   }
-  o.bytes = std::max<size_t>(o.bytes, 256);
   return o;
 }
 
@@ -574,7 +573,7 @@ int came8_int8_linear_forward(const came8_int8_linear* l, const int8_t* q, const
       for (const auto& [p, ld] : {std::pair(q, l->ld_q), std::pair(w, l->ld_w)})
         if (ld % 4 == 0 && (rc = check_pointer(what, p, 4)) != CAME8_OK) return rc;
     const Layout o = layout_of(l);
-    if (!is_few(l) && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < o.bytes))
+    if (o.bytes > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < o.bytes))
       return op_fail(CAME8_ESPACE, std::string(what) + ": workspace too small or misaligned");
     const Int8Args a{q, scale, w, w_scale, bias, y, nullptr, l->ld_q, l->ld_w, int32_t(l->rows), int32_t(l->out), int32_t(l->in), 0, 0, 1};
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -336,6 +336,9 @@ __global__ __launch_bounds__(kThreads) void k_logprob_join(const LogProbArgs a) 
   int lists = 1;
   while (lists < a.parts) lists *= 2;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t token = token_at(a.tokens, row, a.wide);
+    const bool in = token >= 0 && token < a.V;
+    const float z = in ? T::load(gbl(static_cast<const typename T::storage*>(a.z))[row * a.ld + token]) : 0.0f;
     if (a.top > 0) {
       for (int p = wave; p < lists; p += waves)
         keys[p * kWave + lane] = p < a.parts && lane < a.top ? gbl(a.keys)[(row * a.parts + p) * a.top + lane] : 0;
@@ -356,9 +359,6 @@ __global__ __launch_bounds__(kThreads) void k_logprob_join(const LogProbArgs a) 
     const float all = wave_sum(f > 0.0f ? s * f : (s == s ? 0.0f : s)), ent = wave_sum(f > 0.0f ? shifted * f : 0.0f);
     const float l = logf(all);
     if (threadIdx.x == 0) {
-      const int64_t token = token_at(a.tokens, row, a.wide);
-      const bool in = token >= 0 && token < a.V;
-      const float z = in ? T::load(gbl(static_cast<const typename T::storage*>(a.z))[row * a.ld + token]) : 0.0f;
       gbl(a.log_prob)[row] = in ? (z - most) - l : 0.0f;
       gbl(a.entropy)[row] = l - ent / all;
       gbl(a.stats)[2 * row] = most;
@@ -481,14 +481,14 @@ void forward(const LogProbArgs& a, hipStream_t stream) {
 }
 
 struct Layout {
-  size_t part = 0, keys = 0, bytes = 256;
+  size_t part = 0, keys = 0, bytes = 0;
 };
 Layout layout_of(const came8_log_probs* p) {
   Layout l;
   const Cut c = cut_of(p);
   if (c.parts == 1) return l;
   l.keys = size_t(p->rows * c.parts) * 16;
-  l.bytes = l.keys + size_t(p->rows * c.parts * p->top) * 8 + 256;
+  l.bytes = l.keys + size_t(p->rows * c.parts * p->top) * 8;
   return l;
 }
 

@@ -468,7 +468,7 @@ typedef struct came8_int8_linear {
   int32_t reserved;
 } came8_int8_linear;
 
-/* Bytes of device workspace for came8_int8_linear_forward. */
+/* Bytes of device workspace for came8_int8_linear_forward; where they are 0 it may be NULL. */
 int came8_int8_linear_workspace_size(const came8_int8_linear* l, size_t* bytes);
 
 /* y is contiguous.  With more than 16 rows, an operand whose ld is not a multiple of 4 may be copied to the workspace first; one
@@ -489,7 +489,7 @@ typedef struct came8_log_probs {
   int32_t reserved;
 } came8_log_probs;
 
-/* Bytes of device workspace for came8_log_probs_forward. */
+/* Bytes of device workspace for came8_log_probs_forward; where they are 0 it may be NULL. */
 int came8_log_probs_workspace_size(const came8_log_probs* p, size_t* bytes);
 
 /* stats[i][2]: m and l of row i, for the backward call.  top_log_prob and top_token [rows][top], NULL where top is 0. */

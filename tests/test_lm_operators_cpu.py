@@ -133,6 +133,9 @@ def test_product_entries_refuse_pointers_and_workspaces():
             p = [P] * 6
             p[i] = bad
             assert lib.came8_int8_linear_forward(ctypes.byref(l), *p, P, need, None) == L.CAME8_EINVAL
+    l = _desc(L.Came8Int8Linear, INT8, ld_q=1001)  # copied
+    need = _size("int8_linear", l)[1]
+    assert need >= l.rows * getattr(l, "in")
     for ws, size in ((None, need), (P + 8, need), (P, need - 1)):
         assert lib.came8_int8_linear_forward(ctypes.byref(l), P, P, P, P, None, P, ws, size, None) == L.CAME8_ESPACE
     none = _desc(L.Came8Int8Linear, INT8, rows=0)
