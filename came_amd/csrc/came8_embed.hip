@@ -8,6 +8,7 @@
 #include "../../include/came8.h"
 #include "came8_ops.h"
 #include "came8_rows.h"
+#include "came8_shares.h"
 
 namespace came8 {
 namespace {
@@ -165,8 +166,7 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const EmbedBackArgs
   const uint64_t empty = __builtin_amdgcn_ballot_w64(r < a.range && first + r < last && all == 0);
   if (lane == 0) gbl(a.empty)[int64_t(blockIdx.x) * kSortWaves + wave] = empty;
   // the shares that end within this token's positions
-  for (int64_t s = (start + a.share) / a.share - 1; all > 0 && (s + 1) * a.share <= start + all; ++s)
-    gbl(a.cross)[s] = start >= s * a.share && start + all > (s + 1) * a.share ? int32_t((start + all - 1) / a.share) : -1;
+  share_ends(start, all, a.share, [&](int64_t s, int32_t last) { gbl(a.cross)[s] = last; });
 }
 
 // The rows of dy of `share` successive sorted positions, TPR threads by their 16-byte chunks, summed by token.  A token whose
