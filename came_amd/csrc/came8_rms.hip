@@ -14,6 +14,7 @@
 
 #include "../../include/came8.h"
 #include "came8_ops.h"
+#include "came8_rms_grid.h"
 #include "came8_rows.h"
 
 namespace came8 {
@@ -422,35 +423,37 @@ __global__ __launch_bounds__(1024) void k_rms_back_long(const RmsBackArgs a, flo
 // dw of 32 columns: the sum of the partial sums' rows, 128 of them at a time (8 lanes of 4 columns each).
 template <typename T>
 __global__ __launch_bounds__(1024) void k_rms_join(const float* part, int32_t parts, int64_t D, void* dw) {
-  __shared__ float lds[16][32];
+  __shared__ float lds[16][kRmsJoinColumns];
   const int lane = int(threadIdx.x) % kWave, wave = int(threadIdx.x) / kWave;
-  const int64_t c = int64_t(blockIdx.x) * 32 + lane % 8 * 4;
-  float v[4] = {};
+  for (int64_t c0 = int64_t(blockIdx.x) * kRmsJoinColumns; c0 < D; c0 += int64_t(gridDim.x) * kRmsJoinColumns) {
+    const int64_t c = c0 + lane % 8 * 4;
+    float v[4] = {};
 #pragma unroll 4
-  for (int r = wave * 8 + lane / 8; r < parts; r += 128) {
-    float p[4];
-    load_chunk<F32>(part + int64_t(r) * D, c, D, p);
+    for (int r = wave * 8 + lane / 8; r < parts; r += 128) {
+      float p[4];
+      load_chunk<F32>(part + int64_t(r) * D, c, D, p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += p[e];
-  }
+      for (int e = 0; e < 4; ++e) v[e] += p[e];
+    }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-    for (int o = 8; o < kWave; o *= 2) v[e] += __shfl_xor(v[e], o, kWave);
-    if (lane < 8) lds[wave][lane * 4 + e] = v[e];
-  }
-  __syncthreads();
-  const int64_t col = int64_t(blockIdx.x) * 32 + int(threadIdx.x);
-  if (threadIdx.x < 32 && col < D) {
-    float s = lds[0][threadIdx.x];
+      for (int o = 8; o < kWave; o *= 2) v[e] += __shfl_xor(v[e], o, kWave);
+      if (lane < 8) lds[wave][lane * 4 + e] = v[e];
+    }
+    __syncthreads();
+    const int64_t col = c0 + int(threadIdx.x);
+    if (threadIdx.x < kRmsJoinColumns && col < D) {
+      float s = lds[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < 16; ++w) s += lds[w][threadIdx.x];
-    gbl(static_cast<typename T::storage*>(dw))[col] = T::store(s);
+      for (int w = 1; w < 16; ++w) s += lds[w][threadIdx.x];
+      gbl(static_cast<typename T::storage*>(dw))[col] = T::store(s);
+    }
+    __syncthreads();  // before the next columns' sums
   }
 }
 
 // ------------------------------------------------------------------------------------------------------ launches
-constexpr int64_t kMaxGroups = 1 << 20;  // workgroups a launch; the rest of the rows in turns
 constexpr int64_t kMaxParts = 512;       // workgroups that share dw's sum
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -474,13 +477,12 @@ void by_width(int64_t D, F&& f) {
 template <typename T, Output OUT>
 void forward(const came8_rms_norm* n, const RmsArgs& a, hipStream_t stream) {
   if (is_long(n)) {
-    hipLaunchKernelGGL((k_rms_long<T, OUT>), dim3(unsigned(std::min(n->rows, kMaxGroups))), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((k_rms_long<T, OUT>), dim3(unsigned(rms_row_groups(n->rows, 1))), dim3(1024), 0, stream, a);
     return;
   }
   by_width<T>(n->dim, [&](auto tpr, auto nv) {
     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, kBlock = TPR < kThreads ? kThreads : TPR;
-    const int64_t groups = std::min(ceil_div(n->rows, kBlock / TPR), kMaxGroups);
-    hipLaunchKernelGGL((k_rms<T, TPR, NV, OUT>), dim3(unsigned(groups)), dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((k_rms<T, TPR, NV, OUT>), dim3(unsigned(rms_row_groups(n->rows, kBlock / TPR))), dim3(kBlock), 0, stream, a);
   });
 }
 
@@ -503,9 +505,9 @@ void backward(const came8_rms_norm* n, RmsBackArgs a, void* dw, void* ws, hipStr
   a.part = dw ? static_cast<float*>(ws) : nullptr;
   if (is_long(n)) {
     float* inverse = dw ? a.part + parts * n->dim : nullptr;
-    hipLaunchKernelGGL((k_rms_back_long<T, false>), dim3(unsigned(std::min(n->rows, kMaxGroups))), dim3(1024), 0, stream, a, inverse);
+    hipLaunchKernelGGL((k_rms_back_long<T, false>), dim3(unsigned(rms_row_groups(n->rows, 1))), dim3(1024), 0, stream, a, inverse);
     if (dw)
-      hipLaunchKernelGGL((k_rms_back_long<T, true>), dim3(unsigned(ceil_div(n->dim, 1024 * kChunk<T>)), unsigned(parts)), dim3(1024), 0,
+      hipLaunchKernelGGL((k_rms_back_long<T, true>), dim3(unsigned(rms_column_groups(n->dim, kChunk<T>)), unsigned(parts)), dim3(1024), 0,
                          stream, a, inverse);
   } else {
     by_width<T>(n->dim, [&](auto tpr, auto nv) {
@@ -514,7 +516,7 @@ void backward(const came8_rms_norm* n, RmsBackArgs a, void* dw, void* ws, hipStr
     });
   }
   if (dw)
-    hipLaunchKernelGGL(k_rms_join<T>, dim3(unsigned(ceil_div(n->dim, 32))), dim3(1024), 0, stream, a.part, int32_t(parts), n->dim, dw);
+    hipLaunchKernelGGL(k_rms_join<T>, dim3(unsigned(rms_join_groups(n->dim))), dim3(1024), 0, stream, a.part, int32_t(parts), n->dim, dw);
 }
 
 int check(const char* what, const came8_rms_norm* n, bool residual) {
@@ -522,7 +524,7 @@ int check(const char* what, const came8_rms_norm* n, bool residual) {
   if (n == nullptr) return op_fail(CAME8_EINVAL, at + "no description given");
   if (n->dtype != CAME8_F32 && n->dtype != CAME8_BF16 && n->dtype != CAME8_F16)
     return op_fail(CAME8_EINVAL, at + "unknown dtype " + std::to_string(n->dtype));
-  if (n->rows < 0 || n->rows >= (int64_t(1) << 31) || n->dim < 1 || n->dim > (int64_t(1) << 30))
+  if (n->rows < 0 || n->rows >= (int64_t(1) << 31) || n->dim < 1 || n->dim > kRmsMaxDim)
     return op_fail(CAME8_EINVAL, at + "rows must be in [0, 2^31), dim in [1, 2^30]");
   if (n->ld_x < n->dim || (residual && n->ld_residual < n->dim))
     return op_fail(CAME8_EINVAL, at + "a row stride must be at least the row's length");
