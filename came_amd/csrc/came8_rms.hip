@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "../../include/came8.h"
+#include "came8_codes.h"
 #include "came8_ops.h"
 #include "came8_rms_grid.h"
 #include "came8_rows.h"
@@ -37,7 +38,9 @@ struct RmsArgs {
 // ------------------------------------------------------------------------------------------------- 8 bits
 // A code is p * 127 / a rounded to nearest even, with a the largest |p| of the row: what the norm multiplies the row by moves
 // none.  In fp32, p * (127 / a) is off by at most 4 roundings of 127, 3.1e-5 of a code; a value that is so near to a border
-// between two is taken again in 64 bits, where p is exact (16-bit types: in fp32 already).
+// between two is taken again from p and a in 64 bits, which hold both: from their quotient where p has 24 bits at most (16-bit
+// types, rows as they are), since that is a tie or further from one than its rounding, and by nearest_code where p has 48 (8192 x
+// 4096 with the residual 83 us with either; in 16 bits the quotient takes 39 and 44, nearest_code 42 and 48).
 constexpr float kTiny = 0x1p-100f;  // the largest of a row below holds zeros: 127 / it may be infinite
 constexpr float kBorder = 0.5f - 4e-5f;
 
@@ -62,7 +65,8 @@ struct Largest {
 
 __device__ __forceinline__ uint64_t magnitude(double p) { return __builtin_bit_cast(uint64_t, p) & 0x7fffffffffffffffull; }
 
-template <int V>
+// WIDE: products of two float32 values
+template <int V, bool WIDE>
 __device__ __forceinline__ void store_codes(int8_t* row, int64_t e0, int64_t D, const Factors<V>& f, const Largest& a) {
   if (e0 >= ((D + 15) & ~int64_t(15))) return;
   float c[V];
@@ -75,8 +79,11 @@ __device__ __forceinline__ void store_codes(int8_t* row, int64_t e0, int64_t D, 
   }
   if (near) {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      c[v] = float(__builtin_rint(double(f.h[v]) * double(f.w[v]) * 127.0 / __builtin_bit_cast(double, a.bits)));
+    for (int v = 0; v < V; ++v) {
+      const double p = double(f.h[v]) * double(f.w[v]), top = __builtin_bit_cast(double, a.bits);
+      if constexpr (WIDE) c[v] = nearest_code(f.h[v] * f.w[v] * a.inv, c[v], p, top);
+      else c[v] = float(__builtin_rint(p * 127.0 / top));
+    }
   }
   uint32_t w[V / 4];
 #pragma unroll
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void k_rms(const R
       const Largest most = top.template of_row<TPR>(reinterpret_cast<uint32_t*>(lds[turn] + 2 * (TPR / kWave + 1)));
       if (t == 0) gbl(a.scale)[row] = most.scale(r);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) store_codes<V>(a.q + row * a.ld_q, int64_t(i * TPR + t) * V, a.D, factors(i), most);
+      for (int i = 0; i < NV; ++i) store_codes<V, Top<T, OUT == kNormed8>::kWide>(a.q + row * a.ld_q, int64_t(i * TPR + t) * V, a.D, factors(i), most);
     }
   }
 }
@@ -256,7 +263,7 @@ __global__ __launch_bounds__(1024) void k_rms_long(const RmsArgs a) {
       if (threadIdx.x == 0) gbl(a.scale)[row] = most.scale(rr);
       // up to the next multiple of 16 codes, whose chunks past D hold zeros
       for (int64_t e0 = int64_t(threadIdx.x) * V; e0 < ((a.D + 15) & ~int64_t(15)); e0 += kTpr * V)
-        store_codes<V>(a.q + row * a.ld_q, e0, a.D, factors(e0, true), most);
+        store_codes<V, Top<T, OUT == kNormed8>::kWide>(a.q + row * a.ld_q, e0, a.D, factors(e0, true), most);
     }
   }
 }

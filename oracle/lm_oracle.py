@@ -5,6 +5,7 @@ The bounds follow one evaluation in float32, U = 2^-24 a rounding, with every re
 sum of n terms in any order is off by at most n U of the sum of magnitudes; a row's sums go through CHAIN additions at most (the
 elements of a thread, the lanes of a wavefront, the wavefronts).  The hardware's exponential is off by 2 U, and its argument's
 roundings by 2 U of the argument."""
+import numpy as np
 import torch
 
 U = 2.0**-24
@@ -72,13 +73,28 @@ def rms_norm_gradients(h, weight, eps, dy, dh=None):
     return (dx, rounded(ex, dx, dy.dtype)), (dw, rounded(ew, dw, dy.dtype))
 
 
+def codes(p, top):
+    """127 p / top to nearest, ties to even, exactly, where p and top are products of two float32 values (48 bits): next to a border
+    between two codes, border * top and 127 p are compared in numbers of 64 bits' mantissa, which hold both (56 and 55)."""
+    q = p * 127 / top
+    lower = torch.floor(q)
+    near = (q - lower - 0.5).abs() < 1e-9
+    out = torch.round(q)
+    if near.any():
+        assert np.finfo(np.longdouble).nmant >= 63
+        k, v, a = (t[near].numpy().astype(np.longdouble) for t in (lower, p, top.expand_as(p)))
+        above = 127 * v - (k + np.longdouble(0.5)) * a
+        up = (above > 0) | ((above == 0) & (k % 2 != 0))
+        out[near] = torch.from_numpy((k + up).astype(np.float64))
+    return out
+
+
 def quantize_rows(x):
-    """(codes, scales) of values x, the codes exactly those of x * 127 / max |x| (a product in 64 bits is exact for float32
-    values, and a quotient that is no tie is further than 64 bits' rounding from one); the scales unrounded."""
+    """(codes, scales) of values x, or of products of two of them; the scales unrounded."""
     x = x.detach().cpu().double()
     top = x.abs().amax(-1, keepdim=True)
     fine = torch.isfinite(top) & (top >= 2.0**-100)
-    q = torch.where(fine, torch.round(x * 127 / top), torch.zeros_like(x)).to(torch.int8)
+    q = torch.where(fine, codes(torch.where(fine, x, 0.0), torch.where(fine, top, 1.0)), 0.0).to(torch.int8)
     return q, torch.where(top < 2.0**-100, torch.zeros_like(top), top / 127).squeeze(-1)
 
 
