@@ -136,7 +136,7 @@ came8_embedding embedding_of(const at::Tensor& tokens, const Rows& w, double sca
 
 at::Tensor embedding_forward(const at::Tensor& weight, const at::Tensor& tokens, double scale, int64_t padding, long long stream) {
   c10::OptionalDeviceGuard guard(weight.device());
-  const at::Tensor t = tokens.contiguous();
+  const at::Tensor t = plain(tokens);
   const Rows w = rows_of(weight, kFar);
   std::vector<int64_t> sizes = tokens.sizes().vec();
   sizes.push_back(weight.size(1));
@@ -167,7 +167,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     at::NoGradGuard no_grad;
     c10::OptionalDeviceGuard guard(dys[0].device());
     check_captured(ctx->saved_data["captured"].toBool(), "embedding", dys[0].device());
-    const at::Tensor tokens = ctx->get_saved_variables()[0].contiguous();
+    const at::Tensor tokens = plain(ctx->get_saved_variables()[0]);
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const at::Tensor dy = plain(dys[0]);
     if (tokens.numel() == 0) {
@@ -302,7 +302,7 @@ came8_log_probs log_probs_of(const Rows& z, const at::Tensor& tokens, int64_t to
 variable_list log_probs_forward(const at::Tensor& logits, const at::Tensor& tokens, int64_t top, long long stream, bool keep, Tops* tops) {
   c10::OptionalDeviceGuard guard(logits.device());
   const Rows z = rows_of(logits, kFar);
-  const at::Tensor t = tokens.contiguous();
+  const at::Tensor t = plain(tokens);
   const at::TensorOptions f32 = logits.options().dtype(at::kFloat);
   const auto rows = tokens.sizes();
   at::Tensor lp = at::empty(rows, f32), entropy = at::empty(rows, f32), stats;
@@ -345,7 +345,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     c10::OptionalDeviceGuard guard(saved[0].device());
     check_captured(ctx->saved_data["captured"].toBool(), "token_log_probs", saved[0].device());
     const Rows z = rows_of(saved[0], kFar);
-    const at::Tensor t = saved[1].contiguous();
+    const at::Tensor t = plain(saved[1]);
     grads[0] = at::empty(saved[0].sizes(), saved[0].options());
     if (z.count > 0) {
       const at::Tensor dlp = dys[0].defined() ? plain(dys[0]) : at::Tensor(), dent = dys[1].defined() ? plain(dys[1]) : at::Tensor();
