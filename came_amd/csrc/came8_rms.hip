@@ -3,6 +3,8 @@
 //   h = x + residual,  r = 1 / sqrt(mean(h^2) + eps),  y = h r w
 //   g = dy w,  dx = r (g - h r^2 mean(g h)) + dh,  dw = sum over the rows of dy h r
 //
+// (r^2 is taken as two factors: without eps, of rows of 1e-20 say, it is no float32.)
+//
 // A row lies in the registers of the threads that share it from its one read on: 16 lanes, a wavefront, 256 threads or 1024, by
 // its width.  All of it is bound by memory; widths that fit no registers are read again.
 #include <hip/hip_runtime.h>
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(TPR < kThreads ? kThreads : TPR) void k_rms_back(co
       }
     }
     row_sum<TPR>(s, lds[turn]);
-    const float r = 1.0f / sqrtf(s[0] / float(a.D) + a.eps), c = r * r * (s[1] / float(a.D));
+    const float r = 1.0f / sqrtf(s[0] / float(a.D) + a.eps), c = r * (r * (s[1] / float(a.D)));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float h[V], g[V], w[V], d[V];
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(1024) void k_rms_back_long(const RmsBackArgs a, flo
         s[1] += q;
       }
       row_sum<kTpr>(s, lds[turn]);
-      const float r = 1.0f / sqrtf(s[0] / float(a.D) + a.eps), c = r * r * (s[1] / float(a.D));
+      const float r = 1.0f / sqrtf(s[0] / float(a.D) + a.eps), c = r * (r * (s[1] / float(a.D)));
       if (threadIdx.x == 0 && inverse != nullptr) gbl(inverse)[row] = r;
       if (a.dx == nullptr) continue;
       for (int64_t e0 = int64_t(threadIdx.x) * V; e0 < a.D; e0 += kTpr * V) {

@@ -32,3 +32,30 @@ def test_tokens_that_are_negative_views(dtype):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
         dlp = torch.randn(want.shape, generator=gen).cuda()
         assert torch.equal(torch.autograd.grad(a.log_probs, z, dlp)[0], torch.autograd.grad(b.log_probs, z, dlp)[0])
+
+
+@pytest.mark.parametrize("D", [64, 3000, 20000])
+@pytest.mark.parametrize("size", [3e-20, 1e-18, 1.0, 1e17])
+def test_norm_gradients_of_small_and_large_rows_without_eps(D, size):
+    """1/sqrt(mean(h^2)) squared is no float32 for rows of 3e-20, but nothing that the gradient is made of is that large.  Squares
+    of 9e-40 are subnormal: a term's rounding is 2^-150, D of them in the mean 2^-150 / 9e-40 = 8e-7 of it, 13 U.  With the oracle's
+    (CHAIN / 2 + 4) U of r and (CHAIN + 1) U of the other sum, which r enters twice: below 300 U, of the terms' magnitudes.  A sum of
+    squares past float32 (20000 of 1e34 and up to 4e34: 4.7e38, where 3.4e38 is the largest) makes r zero, as is documented, and the
+    gradients with it."""
+    from came_amd import rms_norm
+    gen = torch.Generator().manual_seed(D)
+    x = (size * (1 + torch.rand(6, D, generator=gen)) * (2.0 * torch.randint(0, 2, (6, D), generator=gen) - 1)).cuda().requires_grad_()
+    w = (1 + 0.2 * torch.randn(D, generator=gen)).cuda().requires_grad_()
+    dy = torch.randn(6, D, generator=gen).cuda()
+    dx, dw = torch.autograd.grad(rms_norm(x, w, eps=0.0), (x, w), dy)
+    h, g, v = x.detach().cpu().double(), dy.cpu().double(), w.detach().cpu().double()
+    if (h.square().sum(-1) > 1.01 * torch.finfo(torch.float32).max).all():
+        assert not dx.any() and not dw.any()
+        return
+    r = 1 / h.square().mean(-1, keepdim=True).sqrt()
+    gw = g * v
+    want = r * (gw - h * (r * r * (gw * h).mean(-1, keepdim=True)))
+    size_of = r * (gw.abs() + h.abs() * r * r * (gw * h).abs().mean(-1, keepdim=True))
+    assert ((dx.cpu().double() - want).abs() <= 300 * orc.U * size_of).all()
+    terms = g * h * r
+    assert ((dw.cpu().double() - terms.sum(0)).abs() <= 300 * orc.U * terms.abs().sum(0)).all()
