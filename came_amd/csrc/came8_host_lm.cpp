@@ -275,7 +275,7 @@ void check_norm(const char* op, const at::Tensor& x, const at::Tensor& weight, c
   check_alike(op, "weight", weight, "x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && weight.dim() == 1 && weight.size(0) == x.size(-1), op,
                     ": x [..., dim] and weight [dim]; got ", x.sizes(), " and ", weight.sizes());
-  TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0.0, op, ": eps must be finite and at least 0, is ", eps);
+  TORCH_CHECK_VALUE(std::isfinite(float(eps)) && eps >= 0.0, op, ": eps must be finite in float32 and at least 0, is ", eps);
   if (has(residual)) {
     check_alike(op, "residual", *residual, "x", x);
     TORCH_CHECK_VALUE(residual->sizes() == x.sizes(), op, ": the residual has x's shape; got ", residual->sizes(), " and ", x.sizes());

@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <limits>
 #include <type_traits>
 
 #include "../../include/came8.h"
@@ -543,8 +544,13 @@ int check(const char* what, const came8_rms_norm* n, bool residual) {
 }
 
 int check_eps(const char* what, const came8_rms_norm* n) {
-  if (std::isfinite(n->eps) && n->eps >= 0.0) return CAME8_OK;
-  return op_fail(CAME8_EINVAL, std::string(what) + ": eps must be finite and at least 0");
+  if (std::isfinite(n->eps) && n->eps >= 0.0 && std::isfinite(float(n->eps))) return CAME8_OK;
+  return op_fail(CAME8_EINVAL, std::string(what) + ": eps must be finite, in float32 too, and at least 0");
+}
+// in float32; above 0 where eps is, so that a row of zeros is not divided by it
+float eps_of(const came8_rms_norm* n) {
+  const float e = float(n->eps);
+  return n->eps > 0.0 ? std::max(e, std::numeric_limits<float>::denorm_min()) : e;
 }
 
 // every pointer is there and aligned to its elements
@@ -579,7 +585,7 @@ int came8_rms_norm_forward(const came8_rms_norm* n, const void* x, const void* r
     if ((rc = check_pointers(what, n->dtype, {x, weight, y})) != CAME8_OK) return rc;
     if ((residual == nullptr) != (h == nullptr)) return op_fail(CAME8_EINVAL, std::string(what) + ": a residual and h go together");
     if (residual && (rc = check_pointers(what, n->dtype, {residual, h})) != CAME8_OK) return rc;
-    const RmsArgs a{x, residual, weight, y, h, nullptr, nullptr, n->rows, n->dim, n->ld_x, n->ld_residual, 0, float(n->eps)};
+    const RmsArgs a{x, residual, weight, y, h, nullptr, nullptr, n->rows, n->dim, n->ld_x, n->ld_residual, 0, eps_of(n)};
     forward_of<kNormed>(n, a, static_cast<hipStream_t>(stream));
     return op_check_launch("rms_norm_forward");
   } catch (const std::exception& e) {
@@ -598,7 +604,7 @@ int came8_rms_norm_int8(const came8_rms_norm* n, const void* x, const void* resi
     if ((rc = check_codes(what, n, q, ld_q, scale)) != CAME8_OK) return rc;
     if ((residual == nullptr) != (h == nullptr)) return op_fail(CAME8_EINVAL, std::string(what) + ": a residual and h go together");
     if (residual && (rc = check_pointers(what, n->dtype, {residual, h})) != CAME8_OK) return rc;
-    const RmsArgs a{x, residual, weight, nullptr, h, q, scale, n->rows, n->dim, n->ld_x, n->ld_residual, ld_q, float(n->eps)};
+    const RmsArgs a{x, residual, weight, nullptr, h, q, scale, n->rows, n->dim, n->ld_x, n->ld_residual, ld_q, eps_of(n)};
     forward_of<kNormed8>(n, a, static_cast<hipStream_t>(stream));
     return op_check_launch("rms_norm_int8");
   } catch (const std::exception& e) {
@@ -650,7 +656,7 @@ int came8_rms_norm_backward(const came8_rms_norm* n, const void* h, const void* 
     if ((rc = came8_rms_norm_workspace_size(n, &need)) != CAME8_OK) return rc;
     if (dweight && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < need))
       return op_fail(CAME8_ESPACE, std::string(what) + ": workspace too small or misaligned");
-    const RmsBackArgs a{h, weight, dy, dh, dx, nullptr, n->rows, n->dim, n->ld_x, float(n->eps)};
+    const RmsBackArgs a{h, weight, dy, dh, dx, nullptr, n->rows, n->dim, n->ld_x, eps_of(n)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (n->dtype == CAME8_F32) backward<F32>(n, a, dweight, workspace, s);
     else if (n->dtype == CAME8_BF16) backward<BF16>(n, a, dweight, workspace, s);

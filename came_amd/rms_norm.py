@@ -15,8 +15,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     ``(it, h)``.
 
     x, residual [..., dim], weight [dim]: one type (float32, bfloat16 or float16), one GPU.  ``h`` is rounded to that type, and
-    the norm is that of the rounded values; sums are float32.  Differentiable once in every operand, in reverse mode.  Operands
-    whose rows are contiguous are read where they are, others are copied.
+    the norm is that of the rounded values; sums are float32, and so is ``eps`` (finite, at least 0).  Differentiable once in every
+    operand, in reverse mode.  Operands whose rows are contiguous are read where they are, others are copied.
     """
     out = _lib.host().rms_norm(x, weight, residual, eps, *_lib.current(x))
     return out[0] if residual is None else out

@@ -431,7 +431,7 @@ int came8_embedding_backward(const came8_embedding* e, const void* tokens, const
 typedef struct came8_rms_norm {
   int64_t rows, dim;          /* rows below 2^31, dim in [1, 2^30] */
   int64_t ld_x, ld_residual;  /* ld_residual: 0 where there is none */
-  double eps;
+  double eps;                 /* at least 0; taken in float32, where it is finite, and above 0 if it is */
   int32_t dtype;              /* CAME8_F32 / CAME8_BF16 / CAME8_F16 */
   int32_t reserved;
 } came8_rms_norm;

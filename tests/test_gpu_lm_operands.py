@@ -59,3 +59,18 @@ def test_norm_gradients_of_small_and_large_rows_without_eps(D, size):
     assert ((dx.cpu().double() - want).abs() <= 300 * orc.U * size_of).all()
     terms = g * h * r
     assert ((dw.cpu().double() - terms.sum(0)).abs() <= 300 * orc.U * terms.abs().sum(0)).all()
+
+
+def test_an_eps_that_float32_does_not_hold():
+    """One that would be infinite there is refused; one that would be 0 is kept above it, and so is a row of zeros finite."""
+    from came_amd import rms_norm, rms_norm_int8
+    x, w = torch.zeros(3, 40, device="cuda"), torch.ones(40, device="cuda")
+    x[1] = 1.0
+    for op in (rms_norm, rms_norm_int8):
+        for eps in (1e39, 1e300):
+            with pytest.raises(ValueError, match="eps"):
+                op(x, w, eps=eps)
+    leaf = x.clone().requires_grad_()
+    y = rms_norm(leaf, w, eps=1e-60)
+    assert not y[0].any() and (y[1] == 1).all()
+    assert torch.isfinite(torch.autograd.grad(y, leaf, torch.full_like(y, 1e-3))[0]).all()
