@@ -384,6 +384,8 @@ PyObject* embedding(PyObject*, PyObject* args) {
   check_floating(op, "weight", weight);
   check_tokens(op, tokens, "weight", weight);
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.numel() > 0, op, ": weight [vocab, dim], not empty; got ", weight.sizes());
+  TORCH_CHECK_VALUE(!std::isfinite(scale) || (std::isfinite(float(scale)) && (scale == 0.0 || float(scale) != 0.0f)), op,
+                    ": float32 does not hold the scale ", scale);
   pybind11::gil_scoped_release no_gil;
   at::Tensor y = at::GradMode::is_enabled() && weight.requires_grad()
                      ? Embedding::apply(weight, tokens, scale, int64_t(padding), int64_t(stream), captured != 0)

@@ -13,10 +13,11 @@ from . import _lib
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
     """``scale * weight[tokens]``, [..., dim].
 
-    tokens [...]: int64 or int32; weight [vocab, dim]: float32, bfloat16 or float16; one GPU.  ``padding_idx``: a token whose row
-    has no gradient (a negative one counts from the end).  A token outside of [0, vocab) gives zeros and has no gradient: where a
-    table's rows are split over processes, each looks its own up and the results add.  Nothing raises for one, since the host
-    does not read the tokens.  Differentiable once in ``weight``, in reverse mode.
+    tokens [...]: int64 or int32; weight [vocab, dim]: float32, bfloat16 or float16; one GPU.  ``scale`` is taken in float32; one
+    that would become infinite or 0 there is refused.  ``padding_idx``: a token whose row has no gradient (a negative one counts
+    from the end).  A token outside of [0, vocab) gives zeros and has no gradient: where a table's rows are split over processes,
+    each looks its own up and the results add.  Nothing raises for one, since the host does not read the tokens.  Differentiable
+    once in ``weight``, in reverse mode.
     """
     padding = -1
     if padding_idx is not None:

@@ -74,3 +74,15 @@ def test_an_eps_that_float32_does_not_hold():
     y = rms_norm(leaf, w, eps=1e-60)
     assert not y[0].any() and (y[1] == 1).all()
     assert torch.isfinite(torch.autograd.grad(y, leaf, torch.full_like(y, 1e-3))[0]).all()
+
+
+def test_a_scale_that_float32_does_not_hold():
+    """One that would be infinite or 0 there is refused."""
+    from came_amd import embedding
+    x, t = torch.zeros(3, 40, device="cuda"), torch.tensor([1, 7], device="cuda")
+    x[1] = 1.0
+    for scale in (1e39, -1e39, 1e-60):
+        with pytest.raises(ValueError, match="scale"):
+            embedding(t, x, scale=scale)
+    assert not embedding(t, x, scale=0.0).any() and torch.isnan(embedding(t, x, scale=float("nan"))[0]).all()
+    assert (embedding(t, x, scale=1e38)[0] == 1e38).all() and (embedding(t, x, scale=1e-40)[0] > 0).all()
