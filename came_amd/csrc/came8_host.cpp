@@ -431,11 +431,12 @@ std::pair<at::Tensor, at::Tensor> ffn_forward(const at::Tensor& x, const at::Ten
 
 struct GatedFfn : torch::autograd::Function<GatedFfn> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate, const at::Tensor& up,
-                            const at::Tensor& down, int64_t act, int64_t stream) {
+                            const at::Tensor& down, int64_t act, int64_t stream, bool captured) {
     auto [y, gu] = ffn_forward(x, gate, up, down, act, stream, true);
     ctx->save_for_backward({x, gate, up, down, gu});
     ctx->saved_data["act"] = act;
     ctx->saved_data["stream"] = stream;  // the engine runs the backward pass on the forward's stream
+    ctx->saved_data["captured"] = captured;
     return y;
   }
 
@@ -444,10 +445,11 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
     at::NoGradGuard no_grad;
     const auto saved = ctx->get_saved_variables();
     c10::OptionalDeviceGuard guard(saved[0].device());
+    check_captured(ctx->saved_data["captured"].toBool(), "gated_ffn", saved[0].device());
     const FfnOperands o = ffn_operands(saved[0], saved[1], saved[2], saved[3], ctx->saved_data["act"].toInt());
     const int64_t T = o.f.tokens, F = o.f.hidden;
     const at::Tensor* ops[4] = {&saved[0], &saved[1], &saved[2], &saved[3]};
-    torch::autograd::variable_list grads(6);
+    torch::autograd::variable_list grads(7);
     for (size_t i = 0; i < 4; ++i)
       if (ctx->needs_input_grad(i))
         grads[i] = T > 0 ? at::empty(ops[i]->sizes(), ops[i]->options()) : at::zeros(ops[i]->sizes(), ops[i]->options());
@@ -488,12 +490,13 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// gated_ffn(x, w_gate, w_up, w_down, activation: int, stream: int) -> y
+// gated_ffn(x, w_gate, w_up, w_down, activation: int, stream: int, captured: bool) -> y
 PyObject* gated_ffn(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   PyObject* po[4];
   long long act, stream;
-  if (!PyArg_ParseTuple(args, "OOOOLL", &po[0], &po[1], &po[2], &po[3], &act, &stream)) return nullptr;
+  int captured;
+  if (!PyArg_ParseTuple(args, "OOOOLLp", &po[0], &po[1], &po[2], &po[3], &act, &stream, &captured)) return nullptr;
   TORCH_CHECK(!torch::jit::tracer::isTracing(), "gated_ffn: cannot be traced; a trace would hold the result's allocation alone");
   const char* names[4] = {"x", "w_gate", "w_up", "w_down"};
   at::Tensor t[4];
@@ -519,7 +522,7 @@ PyObject* gated_ffn(PyObject*, PyObject* args) {
   const at::Tensor rows = x.dim() == 2 ? x : x.reshape({tokens, x.size(-1)});
   at::Tensor y;
   if (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || up.requires_grad() || down.requires_grad()))
-    y = GatedFfn::apply(rows, gate, up, down, int64_t(act), int64_t(stream));
+    y = GatedFfn::apply(rows, gate, up, down, int64_t(act), int64_t(stream), captured != 0);
   else
     y = ffn_forward(rows, gate, up, down, act, stream, false).first;
   if (x.dim() != 2) {

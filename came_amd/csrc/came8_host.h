@@ -47,6 +47,11 @@ std::string dtype_name(const at::Tensor& t);
 // The gradients, marked so that a gradient of one of them raises
 torch::autograd::variable_list differentiable_once(torch::autograd::variable_list grads, const char* what);
 
+// A leaf's gradient is accumulated on the stream that was current when the first living graph of the leaf was made.  Where that
+// was outside of a capture, accumulating during one waits across streams that the capture does not have, on a thread of the
+// engine's that has no one to raise to.  So a node raises before it comes to that.  `captured`: its forward pass was.
+void check_captured(bool captured, const char* op, const at::Device& device);
+
 PyObject* embedding(PyObject*, PyObject* args);
 PyObject* rms_norm(PyObject*, PyObject* args);
 PyObject* rms_norm_int8(PyObject*, PyObject* args);

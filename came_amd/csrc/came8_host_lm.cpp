@@ -100,31 +100,7 @@ c10::DataPtr workspace(size_t bytes) { return bytes > 0 ? c10::GetAllocator(at::
 
 void* stream_of(long long stream) { return reinterpret_cast<void*>(stream); }
 
-// -------------------------------------------------------------------------------------------- captured backwards
-// A leaf's gradient is accumulated on the stream that was current when the first living graph of the leaf was made.  Where that
-// was outside of a capture, accumulating during one waits across streams that the capture does not have, on a thread of the
-// engine's that has no one to raise to.  So the node raises before it comes to that.  `captured`: its forward pass was.
-void check_captured(bool captured, const char* op, const at::Device& device) {
-  if (!captured) return;
-  const auto node = torch::autograd::get_current_node();
-  if (node == nullptr) return;
-  const auto* run = torch::autograd::get_current_graph_task_exec_info();
-  const c10::Stream here = c10::impl::VirtualGuardImpl(device.type()).getStream(device);
-  for (const auto& edge : node->next_edges()) {
-    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
-    if (leaf == nullptr) continue;
-    if (run != nullptr && !run->empty()) {  // autograd.grad: no gradient is accumulated
-      const auto found = run->find(leaf);
-      if (found == run->end() || !found->second.needed_) continue;
-    }
-    const auto its = leaf->stream();
-    TORCH_CHECK(!its.has_value() || *its == here, op,
-                ": a backward pass that is captured would accumulate a leaf's gradient on another stream: a graph of that leaf "
-                "from outside of the capture is alive. Drop it before the capture, or run the warm-up on the capture's stream");
-  }
-}
-
-// A parsed argument tuple and the guard of the operands' device
+// A parsed argument tuple
 #define CAME8_PARSE(format, ...) \
   if (!PyArg_ParseTuple(args, format, __VA_ARGS__)) return nullptr
 
@@ -369,6 +345,39 @@ PyObject* tuple_of(const variable_list& out) {
 }
 
 }  // namespace
+
+// -------------------------------------------------------------------------------------------- captured backwards
+namespace {
+
+// the leaf that an edge leads to, itself or (a reshaped, transposed or converted operand) through one node
+template <typename F>
+void each_leaf(const torch::autograd::Node& node, F&& f, bool through = true) {
+  for (const auto& edge : node.next_edges()) {
+    if (edge.function == nullptr) continue;
+    if (auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) f(leaf);
+    else if (through) each_leaf(*edge.function, f, false);
+  }
+}
+
+}  // namespace
+
+void check_captured(bool captured, const char* op, const at::Device& device) {
+  if (!captured) return;
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr) return;
+  const auto* run = torch::autograd::get_current_graph_task_exec_info();
+  const c10::Stream here = c10::impl::VirtualGuardImpl(device.type()).getStream(device);
+  each_leaf(*node, [&](torch::autograd::AccumulateGrad* leaf) {
+    if (run != nullptr && !run->empty()) {  // autograd.grad: no gradient is accumulated
+      const auto found = run->find(leaf);
+      if (found == run->end() || !found->second.needed_) return;
+    }
+    const auto its = leaf->stream();
+    TORCH_CHECK(!its.has_value() || *its == here, op,
+                ": a backward pass that is captured would accumulate a leaf's gradient on another stream: a graph of that leaf "
+                "from outside of the capture is alive. Drop it before the capture, or run the warm-up on the capture's stream");
+  });
+}
 
 // embedding(tokens, weight, scale: float, padding: int (-1: none), stream: int, captured: bool) -> y
 PyObject* embedding(PyObject*, PyObject* args) {

@@ -28,5 +28,4 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    stream = torch.cuda.current_stream(x.device).cuda_stream if isinstance(x, torch.Tensor) and x.is_cuda else 0
-    return _lib.host().gated_ffn(x, w_gate, w_up, w_down, act, stream)
+    return _lib.host().gated_ffn(x, w_gate, w_up, w_down, act, *_lib.current(x))
