@@ -86,3 +86,25 @@ def test_a_scale_that_float32_does_not_hold():
             embedding(t, x, scale=scale)
     assert not embedding(t, x, scale=0.0).any() and torch.isnan(embedding(t, x, scale=float("nan"))[0]).all()
     assert (embedding(t, x, scale=1e38)[0] == 1e38).all() and (embedding(t, x, scale=1e-40)[0] > 0).all()
+
+
+def test_batched_gradients_and_function_transforms_raise():
+    """Tensors that stand for several have no memory that a kernel could read."""
+    from came_amd import embedding, int8_linear, quantize_rows, rms_norm, rms_norm_int8, token_log_probs
+    x, w = torch.randn(4, 16, device="cuda"), torch.randn(16, device="cuda")
+    t = torch.zeros(4, dtype=torch.long, device="cuda")
+    calls = [lambda x: embedding(t, x), lambda x: rms_norm(x, w), lambda x: token_log_probs(x, t).log_probs]
+    for fn in calls:
+        leaf = x.clone().requires_grad_()
+        y = fn(leaf)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf, torch.randn(3, *y.shape, device="cuda"), is_grads_batched=True)
+        torch.cuda.synchronize()
+        for transform in (torch.func.vmap, torch.func.jacfwd, torch.func.jacrev):
+            with pytest.raises(RuntimeError):
+                transform(fn)(x[None] if transform is torch.func.vmap else x)
+    q, s = quantize_rows(x)
+    for fn in (lambda x: rms_norm_int8(x, w)[1], lambda x: quantize_rows(x)[1], lambda x: int8_linear(q, s, q, x[:, 0])):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(fn)(x[None])
+    torch.cuda.synchronize()
