@@ -1,0 +1,55 @@
+"""_lib.current asks for the stream of the tensor's device, and whether that one is captured, whichever device is current."""
+import pytest
+import torch
+
+from came_amd import _lib
+
+
+class OnGpu(torch.Tensor):
+    """A tensor that says it lies on GPU `at`."""
+
+    at = 0
+    is_cuda = True
+
+    def get_device(self):
+        return self.at
+
+    @property
+    def device(self):
+        return torch.device("cuda", self.at)
+
+
+@pytest.mark.parametrize("raw", [True, False])
+@pytest.mark.parametrize("captured", [0, 1, None])
+@pytest.mark.parametrize("at,now", [(0, 0), (1, 0), (0, 1), (1, 1)])
+def test_the_tensors_device_is_asked(monkeypatch, at, now, captured, raw):
+    current = [now]
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.device
+
+        def __exit__(self, *_):
+            current[0] = self.was
+
+    class Stream:
+        def __init__(self, device):
+            self.cuda_stream = 100 + torch.device("cuda", device).index if isinstance(device, int) else 100 + device.index
+
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", (lambda d: 100 + d) if raw else None, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == captured)
+    t = torch.zeros(2).as_subclass(OnGpu)
+    t.at = at
+    assert _lib.current(t) == (100 + at, captured == at)
+    assert current == [now]
+
+
+def test_what_is_on_no_gpu():
+    assert _lib.current(torch.zeros(2)) == _lib.current(None) == (0, False)
