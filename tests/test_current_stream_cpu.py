@@ -19,10 +19,9 @@ class OnGpu(torch.Tensor):
         return torch.device("cuda", self.at)
 
 
-@pytest.mark.parametrize("raw", [True, False])
 @pytest.mark.parametrize("captured", [0, 1, None])
 @pytest.mark.parametrize("at,now", [(0, 0), (1, 0), (0, 1), (1, 1)])
-def test_the_tensors_device_is_asked(monkeypatch, at, now, captured, raw):
+def test_the_tensors_device_is_asked(monkeypatch, at, now, captured):
     current = [now]
 
     class Device:
@@ -35,16 +34,10 @@ def test_the_tensors_device_is_asked(monkeypatch, at, now, captured, raw):
         def __exit__(self, *_):
             current[0] = self.was
 
-    class Stream:
-        def __init__(self, device):
-            self.cuda_stream = 100 + torch.device("cuda", device).index if isinstance(device, int) else 100 + device.index
-
-    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", (lambda d: 100 + d) if raw else None, raising=False)
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
-    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
-    monkeypatch.setattr(torch.cuda, "device", Device)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == captured)
+    monkeypatch.setattr(_lib, "_raw_stream", lambda d: 100 + d)
+    monkeypatch.setattr(_lib, "_current_device", lambda: current[0])
+    monkeypatch.setattr(_lib, "_Device", Device)
+    monkeypatch.setattr(_lib, "_capturing", lambda: current[0] == captured)
     t = torch.zeros(2).as_subclass(OnGpu)
     t.at = at
     assert _lib.current(t) == (100 + at, captured == at)
