@@ -236,12 +236,13 @@ __global__ __launch_bounds__(512, AHEAD ? 4 : 2) void k_int8_few(const Int8Args 
 // Tiles of B by B on 2 by WAVES_N wavefronts.  A step is 128 codes of k; its four phases are laid out as in the feed-forward
 // block's products (came8_ffn.h), and so are the rows in LDS.
 //
-// Codes of normal values, inputs in turn: 8192 x 4096 x 11008 415 us (1780 TOP/s; the library's unscaled product 405 beside it),
-// 8192 x 11008 x 4096 340, 2048 x 4096 x 4096 45, 128 x 4096 x 11008 23.  Matrix units are busy 40% of the cycles, at 1.96 GHz; a
-// step of the large tiles takes 4240 cycles, of which their instructions need 2048, while its 260 KB through LDS take 4060 at 64
-// bytes a cycle.  What was slower: operands loaded straight to LDS in steps of 64 codes, four or five in flight (438, 346, 48,
-// 22); four wavefronts of 128 by 128, which read less of LDS (459); the weights' fragments loaded from memory past LDS (517 where
-// this took 394).
+// Codes of normal values, inputs in turn: 8192 x 4096 x 11008 374 to 415 us (1970 to 1780 TOP/s; the library's unscaled product 405
+// beside the 415), 8192 x 11008 x 4096 325 to 340, 2048 x 4096 x 4096 42 to 45, 128 x 4096 x 11008 23 to 25.  By the counters, a
+// step of a large tile takes 3330 cycles, of which matrix instructions have 2048 and LDS 1280 (no conflicts; a CU reads 234 bytes
+// a cycle in this layout): neither is the limit, and what a step waits for beside them is not known.  A tile's first loads and its
+// epilogue take 31 thousand cycles that nothing overlaps, as much as 9 steps: 8192 x 4096 x 11008 is 5.4 rounds of tiles of 32
+// steps, paid as 6.  What was slower: operands loaded straight to LDS in steps of 64 codes, four or five in flight (438, 346, 48,
+// 22); four wavefronts of 128 by 128 (459); the weights' fragments loaded from memory past LDS (517 where this took 394).
 template <typename T, int B, int WAVES_N>
 __global__ __launch_bounds__(2 * WAVES_N * kWave, 2) void k_int8_gemm(const Int8Args args) {
   constexpr int NT = 2 * WAVES_N * kWave, BK = kRowBytes, kTileBytes = 2 * B * kRowBytes;
