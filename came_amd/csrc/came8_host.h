@@ -49,7 +49,8 @@ torch::autograd::variable_list differentiable_once(torch::autograd::variable_lis
 
 // A leaf's gradient is accumulated on the stream that was current when the first living graph of the leaf was made.  Where that
 // was outside of a capture, accumulating during one waits across streams that the capture does not have, on a thread of the
-// engine's that has no one to raise to.  So a node raises before it comes to that.  `captured`: its forward pass was.
+// engine's that has no one to raise to.  So a node raises before it comes to that, unless the other stream is captured too.
+// `captured`: the node's forward pass was.
 void check_captured(bool captured, const char* op, const at::Device& device);
 
 PyObject* embedding(PyObject*, PyObject* args);

@@ -359,6 +359,18 @@ void each_leaf(const torch::autograd::Node& node, F&& f, bool through = true) {
   }
 }
 
+// Whether a stream of the current device is being captured: a question of torch's about the current stream
+bool captures(const c10::Stream& stream) {
+  struct Current {
+    c10::impl::VirtualGuardImpl impl;
+    c10::Stream was;
+    explicit Current(const c10::Stream& s) : impl(s.device_type()), was(impl.exchangeStream(s)) {}
+    ~Current() { impl.exchangeStream(was); }
+  } current(stream);
+  pybind11::gil_scoped_acquire gil;
+  return pybind11::module_::import("torch").attr("_C").attr("_cuda_isCurrentStreamCapturing")().cast<bool>();
+}
+
 }  // namespace
 
 void check_captured(bool captured, const char* op, const at::Device& device) {
@@ -373,7 +385,8 @@ void check_captured(bool captured, const char* op, const at::Device& device) {
       if (found == run->end() || !found->second.needed_) return;
     }
     const auto its = leaf->stream();
-    TORCH_CHECK(!its.has_value() || *its == here, op,
+    if (!its.has_value() || its->device() != here.device() || *its == here) return;
+    TORCH_CHECK(captures(*its), op,
                 ": a backward pass that is captured would accumulate a leaf's gradient on another stream: a graph of that leaf "
                 "from outside of the capture is alive. Drop it before the capture, or run the warm-up on the capture's stream");
   });

@@ -60,6 +60,25 @@ def test_a_leaf_whose_gradient_lies_on_another_stream(name):
     assert torch.equal(leaf.grad, 3 * other)
 
 
+def test_a_leaf_whose_stream_is_captured_too(monkeypatch):
+    """A capture of two streams: the leaf's gradient may be accumulated on the other one.  (torch is made to say that it is
+    captured.)"""
+    for name, (shape, fn) in _calls().items():
+        leaf = torch.randn(shape, device="cuda", requires_grad=True)
+        first, side = torch.cuda.current_stream(), torch.cuda.Stream()
+        alive = leaf * 2
+        with monkeypatch.context() as m:
+            m.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: torch.cuda.current_stream() == first)
+            side.wait_stream(first)
+            with torch.cuda.stream(side):
+                fn(leaf, side.cuda_stream, True).sum().backward()
+        torch.cuda.synchronize()
+        got, leaf.grad = leaf.grad, None
+        fn(leaf, first.cuda_stream, False).sum().backward()
+        assert torch.equal(got, leaf.grad), name
+        assert torch.cuda.current_stream() == first and alive.shape == shape
+
+
 def test_a_block_is_captured_and_replayed():
     """The block's backward pass in a graph, against eager work between the replays."""
     from came_amd import gated_ffn
